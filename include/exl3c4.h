@@ -262,6 +262,65 @@ int exl3c4_router_topk_scatter(const void* logits, int32_t logits_dtype, int64_t
 int exl3c4_moe_gather(const void* y, int32_t y_dtype, int64_t y_pitch, const float* expert_w, const int32_t* row_of,
                       int64_t n_tok, int32_t top_k, int64_t cols, void* out, int64_t out_pitch, void* stream);
 
+/* ------------------------------------------------------------------ experts that are not trellis codes (device)
+ * The products of a layer's experts kept in 16 bits or in microscaled 4-bit floats (MX4), over the same sorted rows as
+ * the EXL3 ops, and the quantisation that makes MX4 operands. With n_expert 1 and expert_offset {0, T} the product is a
+ * plain linear layer (a router's logits, a shared expert). No counterpart in the reference, whose engine runs such layers
+ * itself. Launches allocate nothing, synchronise nothing, keep no state between calls, and refuse before anything is
+ * written.
+ *
+ * MX4 (the microscaling format with e2m1 elements): a row of `cols` values in blocks of 32 columns (the last one filled up
+ * with zeros), each block 16 bytes of codes, two a byte, the lower column in the low half (bit 3 the sign, bits 0..2 one of
+ * 0, 1/2, 1, 3/2, 2, 3, 4, 6), and one scale byte s: an element is its code's value times 2^(s - 127); every element of a
+ * block with s = 255 is NaN. Codes of a row start codes_pitch bytes apart (a multiple of 16, at least 16 ceil(cols / 32)),
+ * its scales scales_pitch bytes apart (a multiple of 4, at least ceil(cols / 32); a product reads them in whole words). */
+enum { EXL3C4_MX4 = 3 };                                      /* beside EXL3C4_F16, EXL3C4_BF16 and EXL3C4_F32 */
+enum { EXL3C4_ACT_NONE = 0, EXL3C4_ACT_SWIGLU = 1 };
+
+/* x [rows, cols] (f16, bf16 or f32, rows x_pitch elements apart) to MX4: s = max(floor(log2(max |x| of the block)) - 2, -127)
+ * + 127, codes x / 2^(s - 127) rounded to nearest, ties to the even code, magnitudes past 6 to 6. A block of zeros: s = 0. A block that
+ * holds an infinity or a NaN: s = 255 and codes 0. Every code byte of a row's blocks and every scale byte of a block is written; pitch
+ * bytes past them are left. Any x alignment that its elements have; codes 16-byte aligned, scales 4. */
+int exl3c4_mx4_quant(const void* x, int32_t x_dtype, int64_t rows, int64_t cols, int64_t x_pitch, void* codes,
+                     int64_t codes_pitch, void* scales, int64_t scales_pitch, void* stream);
+
+/* The values of MX4 rows as f16, bf16 or f32 [rows, cols], out_pitch elements apart, rounded to nearest even (f32 and bf16 hold
+ * every value of magnitude at least 2^-133, but for overflow; f16 those of its range). */
+int exl3c4_mx4_dequant(const void* codes, int64_t codes_pitch, const void* scales, int64_t scales_pitch, int64_t rows,
+                       int64_t cols, void* out, int32_t out_dtype, int64_t out_pitch, void* stream);
+
+/* moe_gemm: for each sorted row i of expert e's run [expert_offset[e], expert_offset[e + 1]),
+ *     act NONE     y[i][n] = sum over k of W_e[n][k] x[r][k],                       n = 0 .. N - 1
+ *     act SWIGLU   y[i][n] = silu(g) u, g = W_e[n] . x[r], u = W_e[N / 2 + n] . x[r],  n = 0 .. N / 2 - 1
+ * with r = sorted_tok[i] / top_k, or r = i where sorted_tok is null (down: x holds sorted rows). Sums and the activation in f32, rounded
+ * once. Rows outside the runs, and rows whose sorted_tok is negative or names no row of x, are written as zeros, as the EXL3 ops write
+ * them; runs are clamped to [0, T). The same bits on every launch.
+ *   x_type, w_type   F16, F16 | BF16, BF16 | F16, MX4 | BF16, MX4 | MX4, MX4
+ *   y_type           F16, BF16 or F32
+ *   x   [x_rows, K], rows x_pitch apart: elements (16 bits) or bytes (MX4's codes, with x_scales xs_pitch bytes apart)
+ *   w   expert e's [N, K] at w + e * w_stride bytes, or at ((void**)w)[e] where w_stride is 0; rows w_pitch apart, in the units of
+ *       x_pitch; MX4: w_scales, ws_stride and ws_pitch likewise (ws_stride 0: a pointer array)
+ *   y   [T, N or N / 2], y_pitch elements apart; shares no memory with the operands
+ * 16-bit operands: K % 8 == 0, base, pitch and stride in multiples of 16 bytes; with an MX4 operand K % 32 == 0; scale bases, pitches
+ * and strides in multiples of 4 bytes. N is any. Refusals: INVAL (an unknown act, a required operand absent), DTYPE (another pair of
+ * types), SHAPE (extents below one, K or N as above, fewer x rows than read, extents past 2^31 - 1 or more tiles than a launch holds),
+ * STRIDE (a pitch or a stride below what it steps over), ALIGN. */
+typedef struct Exl3c4Gemm {
+    int32_t        x_type, w_type, y_type, act;
+    int64_t        N, K, n_expert, top_k, T;
+    const void*    x;
+    const void*    x_scales;
+    int64_t        x_rows, x_pitch, xs_pitch;
+    const void*    w;
+    const void*    w_scales;
+    int64_t        w_pitch, ws_pitch, w_stride, ws_stride;
+    const int32_t* sorted_tok;                /* [>= T] or null */
+    const int32_t* expert_offset;             /* [n_expert + 1] */
+    void*          y;
+    int64_t        y_pitch;
+} Exl3c4Gemm;
+int exl3c4_moe_gemm(const Exl3c4Gemm* g, void* stream);
+
 /* ------------------------------------------------------------------ the stored form (host, load time) */
 /* Bytes of the stored record of a [rows, cols] weight at K bits: rows * cols * K / 8. */
 int64_t exl3c4_record_bytes(int64_t rows, int64_t cols, int32_t bits);

@@ -154,6 +154,27 @@ int exl3c4_dev_route_scatter(const void* logits, int32_t dtype, int32_t n_tok, i
                              int32_t* count, int32_t* row_of, void* stream);
 int exl3c4_dev_gather(const void* y, int32_t y_dtype, int64_t y_pitch, const float* w, const int32_t* row_of,
                       int64_t n_tok, int32_t top_k, int64_t cols, void* out, int64_t out_pitch, void* stream);
+/* the products of 16-bit and MX4 experts, and MX4's conversions (exl3c4_gemm.hip, exl3c4_mx4.hip) */
+typedef struct Exl3c4DevGemm {
+    const char*    x;              /* rows x_pitch bytes apart */
+    const uint8_t* xs;
+    const char*    w;              /* entry e at w + e * w_stride, or ((void**)w)[e] where w_stride is 0; rows w_pitch bytes apart */
+    const char*    ws;
+    const int32_t* sorted;
+    const int32_t* off;
+    char*          y;              /* rows y_pitch bytes apart */
+    int64_t        x_pitch, xs_pitch, w_pitch, ws_pitch, w_stride, ws_stride, y_pitch;
+    int32_t        x_rows, T, n_expert, top_k;
+    int32_t        N, K;           /* the weight's rows and columns */
+    int32_t        n_out;          /* y's columns: N, or N / 2 with SwiGLU */
+    int32_t        y_type;
+    int32_t        tiles;          /* column tiles of y */
+} Exl3c4DevGemm;
+int exl3c4_dev_gemm(const Exl3c4DevGemm* g, int32_t x_type, int32_t w_type, int32_t act, void* stream);
+int exl3c4_dev_mx4_quant(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t pitch, uint8_t* codes,
+                         int64_t codes_pitch, uint8_t* scales, int64_t scales_pitch, void* stream);
+int exl3c4_dev_mx4_dequant(const uint8_t* codes, int64_t codes_pitch, const uint8_t* scales, int64_t scales_pitch,
+                           int64_t rows, int64_t cols, void* out, int32_t dtype, int64_t out_pitch, void* stream);
 int exl3c4_dev_dequant(const void* record, int32_t rows, int32_t cols, int32_t bits, int32_t codebook, void* w_hat,
                        int64_t w_pitch, void* stream);
 

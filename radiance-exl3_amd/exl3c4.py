@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from typing import NamedTuple
 
 import numpy as np
 
@@ -19,6 +20,8 @@ K_PREP, K_GATE_UP, K_EPI_GU, K_DOWN, K_GATE_UP_DOWN = 0, 1, 2, 3, 4
 GD_FUSE_MIN_T = 32                  # gate_up_down runs as one kernel at decode from this many sorted rows
 CB = {"3inst": 0, "mcg": 1, "mul1": 2}
 F16, BF16 = 0, 1
+MX4 = 3
+ACT_NONE, ACT_SWIGLU = 0, 1
 STATUS = {0: "OK", -1: "RAD_E_SHAPE", -2: "RAD_E_DTYPE", -3: "RAD_E_ALIGN", -4: "RAD_E_STRIDE", -9: "RAD_E_SCHEMA",
           -12: "RAD_E_INVAL", -18: "RAD_E_UNSUPPORTED", -20: "RAD_E_SCRATCH", -21: "RAD_E_DEVICE",
           -5: "RAD_E_FORMAT", -30: "RAD_E_NOTFOUND", -31: "RAD_E_IO"}
@@ -44,6 +47,22 @@ class Op(C.Structure):
                 ("x", _p), ("x_dtype", _i32), ("x_rows", _i64), ("x_cols", _i64), ("x_pitch", _i64),
                 ("sorted_tok", _p), ("expert_offset", _p),
                 ("y", _p), ("T", _i64), ("y_cols", _i64), ("y_pitch", _i64), ("dn_bits", _i32)]
+
+
+class Gemm(C.Structure):
+    _fields_ = [("x_type", _i32), ("w_type", _i32), ("y_type", _i32), ("act", _i32),
+                ("N", _i64), ("K", _i64), ("n_expert", _i64), ("top_k", _i64), ("T", _i64),
+                ("x", _p), ("x_scales", _p), ("x_rows", _i64), ("x_pitch", _i64), ("xs_pitch", _i64),
+                ("w", _p), ("w_scales", _p), ("w_pitch", _i64), ("ws_pitch", _i64), ("w_stride", _i64),
+                ("ws_stride", _i64), ("sorted_tok", _p), ("expert_offset", _p), ("y", _p), ("y_pitch", _i64)]
+
+
+class Mx4(NamedTuple):
+    """MX4 rows (include/exl3c4.h): codes uint8 [..., rows, >= 16 ceil(cols / 32)], scales uint8 [..., rows,
+    >= ceil(cols / 32) up to a multiple of 4], the columns they stand for."""
+    codes: object
+    scales: object
+    cols: int
 
 
 def lib():
@@ -114,6 +133,12 @@ def lib():
         L.exl3c4_prefill_min_rows.argtypes = [_i64]
         L.exl3c4_check_narrow.restype = C.c_int
         L.exl3c4_check_narrow.argtypes = [_p, _p, _p, _i64, _p]
+        L.exl3c4_mx4_quant.restype = C.c_int
+        L.exl3c4_mx4_quant.argtypes = [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]
+        L.exl3c4_mx4_dequant.restype = C.c_int
+        L.exl3c4_mx4_dequant.argtypes = [_p, _i64, _p, _i64, _i64, _i64, _p, _i32, _i64, _p]
+        L.exl3c4_moe_gemm.restype = C.c_int
+        L.exl3c4_moe_gemm.argtypes = [C.POINTER(Gemm), _p]
         L.exl3c4_build_target.restype = C.c_char_p
         L.exl3c4_abi_version.restype = C.c_int
         _lib = L
@@ -458,6 +483,124 @@ def moe_gather(y, y_bf16: bool, w, row_of, out, stream=None) -> int:
     n_tok, top_k = w.shape
     return int(lib().exl3c4_moe_gather(_ptr(y), 1 if y_bf16 else 0, y.stride(0), _ptr(w), _ptr(row_of), n_tok, top_k,
                                        y.shape[1], _ptr(out), out.stride(0), _stream(stream)))
+
+
+# ------------------------------------------------------------------------------------------ 16-bit and MX4 experts
+def _launch_on(t, stream, call) -> int:
+    """call(stream) with t's device current and, by default, on that device's current stream."""
+    import torch
+    if t.device.index == torch.cuda.current_device():
+        return int(call(_stream(stream)))
+    with torch.cuda.device(t.device):
+        return int(call(_stream(stream)))
+
+
+def _rows(t):
+    """(rows, pitch in elements) of a tensor whose leading dimensions step evenly as one."""
+    cols = t.shape[-1]
+    if t.is_contiguous():
+        return (t.numel() // cols if cols else 0), cols
+    if cols > 1 and t.stride(-1) != 1:
+        raise ValueError("rows have to be contiguous")
+    rows, pitch = 1, None
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] == 1:
+            continue
+        if pitch is None:
+            pitch = t.stride(d)
+        elif t.stride(d) != rows * pitch:
+            raise ValueError("the leading dimensions do not step evenly: flatten them or call once for each")
+        rows *= t.shape[d]
+    return rows, cols if pitch is None else pitch
+
+
+def _check_mx4(q: Mx4, lead, cols: int):
+    nb = (cols + 31) // 32
+    if q.cols != cols or q.codes.shape[:-1] != lead or q.scales.shape[:-1] != lead or \
+            q.codes.shape[-1] < 16 * nb or q.scales.shape[-1] < nb:
+        raise ValueError("the MX4 planes do not fit the values' shape")
+
+
+def mx4_empty(shape, device="cuda") -> Mx4:
+    """Uninitialised MX4 rows for values of `shape` ([..., rows, cols])."""
+    import torch
+    *lead, cols = shape
+    nb = (cols + 31) // 32
+    return Mx4(torch.empty((*lead, 16 * nb), dtype=torch.uint8, device=device),
+               torch.empty((*lead, (nb + 3) // 4 * 4), dtype=torch.uint8, device=device), cols)
+
+
+def mx4_quant(x, q: Mx4, stream=None) -> int:
+    """exl3c4_mx4_quant of x [..., cols] (f32 / f16 / bf16) into q; returns the status."""
+    _check_mx4(q, x.shape[:-1], x.shape[-1])
+    (n, pitch), cp, sp = _rows(x), _rows(q.codes)[1], _rows(q.scales)[1]
+    return _launch_on(x, stream, lambda st: lib().exl3c4_mx4_quant(_ptr(x), _dt(x), n, q.cols, pitch, _ptr(q.codes), cp,
+                                                                   _ptr(q.scales), sp, st))
+
+
+def mx4_dequant(q: Mx4, out, stream=None) -> int:
+    """exl3c4_mx4_dequant of q into out [..., cols] (f32 / f16 / bf16); returns the status."""
+    _check_mx4(q, out.shape[:-1], out.shape[-1])
+    (n, pitch), cp, sp = _rows(out), _rows(q.codes)[1], _rows(q.scales)[1]
+    return _launch_on(out, stream, lambda st: lib().exl3c4_mx4_dequant(_ptr(q.codes), cp, _ptr(q.scales), sp, n, q.cols,
+                                                                       _ptr(out), _dt(out), pitch, st))
+
+
+def _planes(t):
+    """(values or codes, scales or None, columns, type) of an operand of moe_gemm."""
+    if isinstance(t, Mx4):
+        return t.codes, t.scales, t.cols, MX4
+    return t, None, t.shape[-1], _dt(t)
+
+
+def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT_NONE) -> Gemm:
+    """One moe_gemm: x [x_rows, K] and w [n_expert, N, K], each a 16-bit tensor or Mx4, sorted_tok i32 [T] (None: x holds
+    sorted rows), expert_offset i32 [n_expert + 1], y [T, N] ([T, N / 2] with ACT_SWIGLU) f16, bf16 or f32."""
+    xv, xs, K, xt = _planes(x)
+    wv, ws, Kw, wt = _planes(w)
+    g = Gemm()
+    g.x_type, g.w_type, g.y_type, g.act = xt, wt, _dt(y), act
+    E, N = wv.shape[0], wv.shape[1]
+    g.N, g.K, g.n_expert, g.top_k, g.T = N, K, E, top_k, y.shape[0]
+    if Kw != K or y.shape[1] != (N // 2 if act == ACT_SWIGLU else N) or \
+            expert_offset.numel() < E + 1:
+        raise ValueError("x, w, expert_offset and y do not fit together")
+    for t, q in ((xv, x), (wv, w)):
+        if isinstance(q, Mx4):
+            _check_mx4(q, t.shape[:-1], K)
+    for t, n in ((sorted_tok, g.T), (expert_offset, E + 1)):
+        if t is not None and (t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous() or t.numel() < n):
+            raise ValueError("sorted_tok and expert_offset are contiguous int32, of T and n_expert + 1 values at least")
+    for t in (xv, xs, wv, ws, y):
+        if t is not None and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError("rows have to be contiguous")
+    for t in (xv, xs, wv, ws, sorted_tok, expert_offset):
+        if t is not None and t.device != y.device:
+            raise ValueError("the operands are on other devices")
+    for t in (wv, ws):                                         # a stride of 0 would name a pointer array
+        if t is not None and E > 1 and t.stride(0) == 0:
+            raise ValueError("the experts' weights are one: pass n_expert 1")
+
+    def pitch(t, d):                                           # of one row alone: any that is large enough
+        return t.stride(d) if t.shape[d] > 1 else max(t.stride(d), t.shape[-1])
+
+    def stride(t):
+        return (t.stride(0) if E > 1 else N * pitch(t, 1)) * t.element_size()
+    g.x, g.x_rows, g.x_pitch = xv.data_ptr(), xv.shape[0], pitch(xv, 0)
+    g.w, g.w_pitch, g.w_stride = wv.data_ptr(), pitch(wv, 1), stride(wv)
+    if xs is not None:
+        g.x_scales, g.xs_pitch = xs.data_ptr(), pitch(xs, 0)
+    if ws is not None:
+        g.w_scales, g.ws_pitch, g.ws_stride = ws.data_ptr(), pitch(ws, 1), stride(ws)
+    g.sorted_tok = None if sorted_tok is None else sorted_tok.data_ptr()
+    g.expert_offset, g.y, g.y_pitch = expert_offset.data_ptr(), y.data_ptr(), pitch(y, 0)
+    g.device, g.tensors = y.device, (xv, xs, wv, ws, sorted_tok, expert_offset, y)     # alive as long as g
+    return g
+
+
+def moe_gemm(g: Gemm, stream=None) -> int:
+    """exl3c4_moe_gemm on the device of g's tensors; returns the status."""
+    return _launch_on(g, stream, lambda st: lib().exl3c4_moe_gemm(C.byref(g), st))
 
 
 def alloc_scratch(o: Op, device="cuda"):
