@@ -45,7 +45,6 @@ struct Chunk { int expert, row0, rows; };                       // expert -1: ro
 // chunks of at most 2^MT_LOG2 rows, numbered in this order. Every wave finds its own (the offsets come from L2; nine
 // loads and one scan for 512 segments), so a launch needs no plan before it. The offsets are clamped to [0, T] and a run
 // that ends before it starts is empty: whatever the table holds, every row is in [0, T). False past the last chunk.
-// *total: the launch's chunks, when asked.
 template <int MT_LOG2>
 __device__ __forceinline__ bool find_chunk(const Exl3c4DevGemm& a, int c, int lane, Chunk& out) {
     const int n_seg = a.n_expert + 2;
@@ -115,6 +114,25 @@ __device__ __forceinline__ void store(char* p, int type, float v) {
     else *(_Float16*)p = (_Float16)v;
 }
 
+// Four columns of a row, `left` of them inside y.
+__device__ __forceinline__ void store4(char* p, int type, const f32x4& v, int left, bool whole) {
+    if (left >= 4 && whole) {
+        if (type == EXL3C4_F32) {
+            *(f32x4*)p = v;
+        } else if (type == BF16) {
+            typedef __bf16 t4 __attribute__((ext_vector_type(4)));
+            *(t4*)p = t4{ (__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3] };
+        } else {
+            typedef _Float16 t4 __attribute__((ext_vector_type(4)));
+            *(t4*)p = t4{ (_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3] };
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) store(p + i * (type == EXL3C4_F32 ? 4 : 2), type, v[i]);
+    }
+}
+
 // ------------------------------------------------------------------------------------------ the matrix step
 __device__ __forceinline__ f32x4 mma16(const uint4& a, const uint4& b, f32x4 c, half8_t*) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
@@ -127,10 +145,11 @@ template <> struct Elem<BF16> { typedef bf8_t type; };
 template <int XT> __device__ __forceinline__ f32x4 mma(const uint4& a, const uint4& b, f32x4 c) {
     return mma16(a, b, c, (typename Elem<XT>::type*)nullptr);
 }
+template <int BYTE = 0>
 __device__ __forceinline__ f32x4 mma_mx4(const uint4& a, int sa, const uint4& b, int sb, f32x4 c) {
     const i32x8 A = { (int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0 };
     const i32x8 B = { (int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0 };
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, 0, sa, 0, sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, BYTE, sa, BYTE, sb);
 }
 
 // 8 codes (a word) as 8 bf16 with their scale, or 8 f16 without.
@@ -299,8 +318,290 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
     if (!SW && n0 + 16 + j < a.n_out) store(y + (int64_t)(n0 + 16 + j) * ysz, a.y_type, v[1]);
 }
 
+// ------------------------------------------------------------------------------------------ many rows an expert
+// A workgroup: a tile of MT rows of one expert against NT weight rows (with SwiGLU 16 gate rows and their 16 up rows in turn,
+// so that a lane holds both), k in stages. A stage's rows go from memory to LDS without registers
+// (global_load_lds_dwordx4), BUFS - 1 stages ahead of the products; a wave waits for its own loads by count, and one barrier
+// a stage both publishes them and frees the buffer that the next ones fill.
+//
+// LDS. A row of a stage is 128 bytes (64 columns in 16 bits, 256 in MX4; x beside MX4 weights: two such halves, and the
+// weights' rows 64 bytes). The loads write lane after lane, 16 bytes each, so the order within a row is chosen at the
+// source: the chunk at place p of row r is p ^ (r & 7) (of 64-byte rows p ^ ((r >> 1) & 3)), and the 16 rows that a matrix
+// operand reads at one column fall on all the banks evenly.
+//
+// Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, one store.
+__device__ const uint4 k_zero = { 0, 0, 0, 0 };                 // what loads read past the end of a row
+
+__device__ __forceinline__ void dma16(const void* from, void* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
+                                     (__attribute__((address_space(3))) uint32_t*)lds, 16, 0, 0);
+}
+__device__ __forceinline__ void dma4(const void* from, void* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
+                                     (__attribute__((address_space(3))) uint32_t*)lds, 4, 0, 0);
+}
+// Until at most N of the wave's loads are out, and none of its LDS reads.
+template <int N> __device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+}
+
+template <int XT, int WT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS> struct Tile {
+    static constexpr int MT = 1 << MT_LOG2, WAVES_ = WM * WN;
+    static constexpr bool MIXED = WT == MX4 && XT != MX4;
+    static constexpr int KS = WT != MX4 ? 64 : MIXED ? 128 : 256;            // columns a stage
+    static constexpr int XROW = MIXED ? 256 : 128, WROW = MIXED ? 64 : 128;  // bytes of a row a stage
+    static constexpr int XG = MT * XROW / 1024, WG = NT * WROW / 1024;       // 1-KiB loads a stage
+    static constexpr int XS = XT == MX4 ? MT * 8 / 256 : 0, WS = WT == MX4 ? NT * (KS / 32) / 256 : 0;   // of scales, 256 bytes
+    static constexpr int XL = XG / WAVES_, WL = WG / WAVES_;
+    static constexpr int XSL = (XS + WAVES_ - 1) / WAVES_, WSL = (WS + WAVES_ - 1) / WAVES_;
+    static constexpr int LOADS = XL + WL + XSL + WSL;                        // a wave's, every stage
+    static constexpr int AT_W = XG * 1024, AT_XS = AT_W + WG * 1024, AT_WS = AT_XS + XS * 256, STAGE = AT_WS + WS * 256;
+    static constexpr int TM = MT / WM / 16, TN = NT / WN / 16;               // matrix tiles a wave
+    static_assert(XG % WAVES_ == 0 && WG % WAVES_ == 0 && LOADS * (BUFS - 1) < 64 && TN % 2 == 0, "tile");
+};
+
+template <int XT, int WT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS>
+__global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
+    typedef Tile<XT, WT, SW, MT_LOG2, NT, WM, WN, BUFS> G;
+    constexpr int MT = G::MT, WV = WM * WN, KS = G::KS, TM = G::TM, TN = G::TN;
+    __shared__ __align__(1024) char lds[BUFS * G::STAGE];
+    __shared__ int rows_x[MT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+    Chunk ch;
+    const int c = blockIdx.x / a.tiles, tile = blockIdx.x - c * a.tiles;
+    if (!find_chunk<MT_LOG2>(a, c, lane, ch)) return;
+    const int n0 = tile * (SW ? NT / 2 : NT);                    // the tile's first column of y
+    // row r of the tile -> a row of the weight (past the last one: it again, not stored)
+    auto w_row = [&](int r) {
+        if (!SW) return min(n0 + r, a.N - 1);
+        const int s = r >> 4;
+        return min(n0 + 16 * (s >> 1) + (r & 15), a.n_out - 1) + (s & 1) * a.n_out;
+    };
+    f32x4 acc[TN][TM] = {};
+    for (int r = threadIdx.x; r < MT; r += 64 * WV) rows_x[r] = ch.expert >= 0 && r < ch.rows ? x_row(a, ch.row0 + r) : -1;
+    __syncthreads();
+    if (ch.expert >= 0) {
+        const char* we = entry(a.w, a.w_stride, ch.expert);
+        const char* wse = WT == MX4 ? entry((const char*)a.ws, a.ws_stride, ch.expert) : nullptr;
+        // where each of the wave's loads starts, for this lane: in 128-byte rows lane l takes place l % 8 of row l / 8
+        const char* xp[G::XL];
+        const char* wp[G::WL];
+        const char* xsp[G::XSL + 1];
+        const char* wsp[G::WSL + 1];
+#pragma unroll
+        for (int i = 0; i < G::XL; ++i) {
+            const int q = wave + i * WV, r = 8 * (G::MIXED ? q >> 1 : q) + (lane >> 3);
+            xp[i] = a.x + (int64_t)max(rows_x[r], 0) * a.x_pitch + 16 * ((lane & 7) ^ (r & 7)) + (G::MIXED ? 128 * (q & 1) : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < G::WL; ++i) {
+            const int q = wave + i * WV;
+            const int r = G::MIXED ? 16 * q + (lane >> 2) : 8 * q + (lane >> 3);
+            wp[i] = we + (int64_t)w_row(r) * a.w_pitch +
+                    16 * (G::MIXED ? (lane & 3) ^ ((r >> 1) & 3) : (lane & 7) ^ (r & 7));
+        }
+#pragma unroll
+        for (int i = 0; i < G::XSL; ++i) {
+            const int r = 32 * ((wave + i * WV) % max(G::XS, 1)) + (lane >> 1);
+            xsp[i] = (const char*)a.xs + (int64_t)max(rows_x[r], 0) * a.xs_pitch + 4 * (lane & 1);
+        }
+#pragma unroll
+        for (int i = 0; i < G::WSL; ++i) {
+            const int q = (wave + i * WV) % max(G::WS, 1), r = G::MIXED ? 64 * q + lane : 32 * q + (lane >> 1);
+            wsp[i] = wse + (int64_t)w_row(r) * a.ws_pitch + (G::MIXED ? 0 : 4 * (lane & 1));
+        }
+        const int stages = (a.K + KS - 1) / KS;
+        auto load = [&](int t, int buf) {
+            char* to = lds + buf * G::STAGE;
+            const int64_t k = (int64_t)t * KS;
+            const bool full = k + KS <= a.K;
+#pragma unroll
+            for (int i = 0; i < G::XL; ++i) {
+                const int q = wave + i * WV, r = 8 * (G::MIXED ? q >> 1 : q) + (lane >> 3);
+                const int col = XT == MX4 ? 32 * ((lane & 7) ^ (r & 7)) : 8 * ((lane & 7) ^ (r & 7)) + (G::MIXED ? 64 * (q & 1) : 0);
+                const char* p = xp[i] + (int64_t)t * G::XROW;
+                if (!full && k + col >= a.K) p = (const char*)&k_zero;
+                dma16(p, to + q * 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < G::WL; ++i) {
+                const int q = wave + i * WV, r = G::MIXED ? 16 * q + (lane >> 2) : 8 * q + (lane >> 3);
+                const int col = G::MIXED ? 32 * ((lane & 3) ^ ((r >> 1) & 3)) : (WT == MX4 ? 32 : 8) * ((lane & 7) ^ (r & 7));
+                const char* p = wp[i] + (int64_t)t * G::WROW;
+                if (!full && k + col >= a.K) p = (const char*)&k_zero;
+                dma16(p, to + G::AT_W + q * 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < G::XSL; ++i) {
+                const char* p = xsp[i] + (int64_t)t * 8;
+                if (!full && k + 128 * (lane & 1) >= a.K) p = (const char*)&k_zero;
+                dma4(p, to + G::AT_XS + ((wave + i * WV) % max(G::XS, 1)) * 256);
+            }
+#pragma unroll
+            for (int i = 0; i < G::WSL; ++i) {
+                const char* p = wsp[i] + (int64_t)t * (KS / 32);
+                if (!full && k + (G::MIXED ? 0 : 128 * (lane & 1)) >= a.K) p = (const char*)&k_zero;
+                dma4(p, to + G::AT_WS + ((wave + i * WV) % max(G::WS, 1)) * 256);
+            }
+        };
+        // the products of one stage; last: scale bytes past K (in a word that begins before it) count as 0
+        auto multiply = [&](int t, int buf, bool last) {
+            const char* X = lds + buf * G::STAGE;
+            const char* W = X + G::AT_W;
+            const int xr = wm * TM * 16 + l16, wr = wn * TN * 16 + l16;      // the lane's row in the first tile of each
+            if constexpr (WT != MX4) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint4 xv[TM], wv[TN];
+#pragma unroll
+                    for (int i = 0; i < TN; ++i) wv[i] = *(const uint4*)(W + (wr + 16 * i) * 128 + 16 * ((4 * h + g) ^ (l16 & 7)));
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) xv[i] = *(const uint4*)(X + (xr + 16 * i) * 128 + 16 * ((4 * h + g) ^ (l16 & 7)));
+#pragma unroll
+                    for (int n = 0; n < TN; ++n)
+#pragma unroll
+                        for (int m = 0; m < TM; ++m) acc[n][m] = mma<XT>(wv[n], xv[m], acc[n][m]);
+                }
+            } else if constexpr (XT == MX4) {
+                // lane group g takes blocks 2 g and 2 g + 1: their scales are neighbours, and the instruction picks the byte
+                const char* XS = X + G::AT_XS + 2 * g;
+                const char* WS = X + G::AT_WS + 2 * g;
+                int sx[TM], sw[TN], live = 0xFFFF;
+                if (last) {
+                    const int n = (a.K - t * KS) / 32 - 2 * g;
+                    live = n >= 2 ? 0xFFFF : n == 1 ? 0xFF : 0;
+                }
+#pragma unroll
+                for (int i = 0; i < TN; ++i) sw[i] = *(const uint16_t*)(WS + (wr + 16 * i) * 8) & live;
+#pragma unroll
+                for (int i = 0; i < TM; ++i) sx[i] = *(const uint16_t*)(XS + (xr + 16 * i) * 8) & live;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint4 xv[TM], wv[TN];
+#pragma unroll
+                    for (int i = 0; i < TN; ++i) wv[i] = *(const uint4*)(W + (wr + 16 * i) * 128 + 16 * ((2 * g + h) ^ (l16 & 7)));
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) xv[i] = *(const uint4*)(X + (xr + 16 * i) * 128 + 16 * ((2 * g + h) ^ (l16 & 7)));
+#pragma unroll
+                    for (int n = 0; n < TN; ++n)
+#pragma unroll
+                        for (int m = 0; m < TM; ++m)
+                            acc[n][m] = h == 0 ? mma_mx4<0>(wv[n], sw[n], xv[m], sx[m], acc[n][m])
+                                               : mma_mx4<1>(wv[n], sw[n], xv[m], sx[m], acc[n][m]);
+                }
+            } else {
+                const char* WS = X + G::AT_WS;
+                uint32_t live = 0xFFFFFFFFu;
+                if (last) {
+                    const int n = (a.K - t * KS) / 32;
+                    live = n >= 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+                }
+                uint4 q[TN];
+#pragma unroll
+                for (int i = 0; i < TN; ++i) q[i] = *(const uint4*)(W + (wr + 16 * i) * 64 + 16 * (g ^ ((l16 >> 1) & 3)));
+                // x's 16 bytes of columns 8 u .. 8 u + 7 of the stage
+                auto x_at = [&](int m, int u) {
+                    return *(const uint4*)(X + ((xr >> 3) + 2 * m) * 2048 + (u >> 3) * 1024 + (l16 & 7) * 128 + 16 * ((u & 7) ^ (l16 & 7)));
+                };
+                if constexpr (XT == BF16) {
+                    float f[TN];
+#pragma unroll
+                    for (int i = 0; i < TN; ++i)
+                        f[i] = scale_arg(((*(const uint32_t*)(WS + (wr + 16 * i) * 4) & live) >> (8 * g)) & 255);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 xv[TM];
+#pragma unroll
+                        for (int m = 0; m < TM; ++m) xv[m] = x_at(m, 4 * g + j);
+#pragma unroll
+                        for (int n = 0; n < TN; ++n) {
+                            const uint32_t word[4] = { q[n].x, q[n].y, q[n].z, q[n].w };
+                            const uint4 wv = to_bf16(word[j], f[n]);
+#pragma unroll
+                            for (int m = 0; m < TM; ++m) acc[n][m] = mma<BF16>(wv, xv[m], acc[n][m]);
+                        }
+                    }
+                } else {
+                    // D's rows are the weights': lane group g's are 4 g + r, whose scale words are 16 bytes in LDS
+                    uint4 sw[TN];
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) {
+                        q[n] = exchange(q[n]);
+                        sw[n] = *(const uint4*)(WS + (wr - l16 + 16 * n + 4 * g) * 4);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 xv[TM];
+#pragma unroll
+                        for (int m = 0; m < TM; ++m) xv[m] = x_at(m, 4 * j + g);
+#pragma unroll
+                        for (int n = 0; n < TN; ++n) {
+                            const uint32_t word[4] = { q[n].x, q[n].y, q[n].z, q[n].w };
+                            const uint32_t sc[4] = { sw[n].x, sw[n].y, sw[n].z, sw[n].w };
+                            float f[4];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) f[r] = scale_f32(((sc[r] & live) >> (8 * j)) & 255);
+                            const uint4 wv = to_f16(word[j]);
+#pragma unroll
+                            for (int m = 0; m < TM; ++m) {
+                                const f32x4 p = mma<F16>(wv, xv[m], f32x4{ 0, 0, 0, 0 });
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) acc[n][m][r] = __builtin_fmaf(p[r], f[r], acc[n][m][r]);
+                            }
+                        }
+                    }
+                }
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < BUFS - 1; ++i)
+            if (i < stages) load(i, i);
+        int buf = 0;
+        for (int t = 0; t < stages; ++t) {
+            if (BUFS == 2 || t + 1 >= stages) wait_loads<0>();
+            else wait_loads<G::LOADS>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const int next = buf == 0 ? BUFS - 1 : buf - 1;      // the buffer of stage t - 1, read by all before the barrier
+            if (t + BUFS - 1 < stages) load(t + BUFS - 1, next);
+            multiply(t, buf, t + 1 == stages);
+            asm volatile("" ::: "memory");
+            buf = buf + 1 == BUFS ? 0 : buf + 1;
+        }
+    }
+    // lane: row 16 m + l16 of the wave's rows, columns 16 n + 4 g .. + 3 (SwiGLU: of gate tile 2 n and up tile 2 n + 1)
+    const int ysz = a.y_type == EXL3C4_F32 ? 4 : 2;
+    const bool whole = ((uintptr_t)a.y | (uintptr_t)a.y_pitch) % (4 * ysz) == 0;      // four columns are one aligned store
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+        const int r = (wm * TM + m) * 16 + l16;
+        if (r >= ch.rows) continue;
+        const bool alive = rows_x[r] >= 0;
+        char* y = a.y + (int64_t)(ch.row0 + r) * a.y_pitch;
+#pragma unroll
+        for (int n = 0; n < (SW ? TN / 2 : TN); ++n) {
+            const int col = n0 + (wn * (SW ? TN / 2 : TN) + n) * 16 + 4 * g;
+            f32x4 v = SW ? acc[2 * n][m] : acc[n][m];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (SW) v[i] = swiglu(v[i], acc[(SW ? 2 * n + 1 : n)][m][i]);
+                if (!alive) v[i] = 0.f;
+            }
+            store4(y + (int64_t)col * ysz, a.y_type, v, a.n_out - col, whole);
+        }
+    }
+}
+
 int launched() { return hipGetLastError() == hipSuccess ? 0 : EXL3C4_E_DEVICE; }
 
+#ifndef ROWS_MAX
+#define ROWS_MAX 8
+#endif
+#ifndef TILE_MAX
+#define TILE_MAX 128
+#endif
 // Chunks of at most `rows` that the launch's segments (the runs, and the rows before and behind them) can make.
 int64_t chunk_bound(const Exl3c4DevGemm& a, int rows) {
     const int64_t seg = (int64_t)a.n_expert + 2;
@@ -308,12 +609,34 @@ int64_t chunk_bound(const Exl3c4DevGemm& a, int rows) {
 }
 
 template <int XT, int WT, bool SW>
-int launch(Exl3c4DevGemm& a, hipStream_t st) {
+int launch_rows(Exl3c4DevGemm& a, hipStream_t st) {
     a.tiles = (a.n_out + (SW ? 15 : 31)) / (SW ? 16 : 32);
     const int64_t grid = chunk_bound(a, 1 << ROWS_LOG2) * a.tiles;
     if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
     hipLaunchKernelGGL((k_mg_rows<XT, WT, SW>), dim3((unsigned)grid), dim3(64 * WAVES), 0, st, a);
     return launched();
+}
+
+template <int XT, int WT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS>
+int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
+    constexpr int cols = SW ? NT / 2 : NT;
+    a.tiles = (a.n_out + cols - 1) / cols;
+    const int64_t grid = chunk_bound(a, 1 << MT_LOG2) * a.tiles;
+    if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
+    hipLaunchKernelGGL((k_mg_tile<XT, WT, SW, MT_LOG2, NT, WM, WN, BUFS>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
+    return launched();
+}
+
+template <int XT, int WT, bool SW>
+int launch(Exl3c4DevGemm& a, hipStream_t st) {
+    const int64_t T = a.T, live = a.n_expert < T ? a.n_expert : T;
+    if (T <= ROWS_MAX * live) return launch_rows<XT, WT, SW>(a, st);
+    if constexpr (WT == MX4 && XT != MX4) {
+        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
+    } else {
+        if (T <= TILE_MAX * live) return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
+        return launch_tile<XT, WT, SW, 8, 256, 2, 4, 2>(a, st);
+    }
 }
 
 template <int XT, int WT>
