@@ -39,53 +39,115 @@ __device__ __forceinline__ int wave_scan_incl(int v) {
     return v;
 }
 
-struct Chunk { int expert, row0, rows; };                       // expert -1: rows that no run holds (zeros)
+struct Chunk { int expert, row0, rows, tile; };                 // expert -1: rows that no run holds (zeros)
 
-// Chunk c of the launch: the rows before the first run, the experts' runs and the rows behind the last one, each cut into
-// chunks of at most 2^MT_LOG2 rows, numbered in this order. Every wave finds its own (the offsets come from L2; nine
-// loads and one scan for 512 segments), so a launch needs no plan before it. The offsets are clamped to [0, T] and a run
-// that ends before it starts is empty: whatever the table holds, every row is in [0, T). False past the last chunk.
-template <int MT_LOG2>
-__device__ __forceinline__ bool find_chunk(const Exl3c4DevGemm& a, int c, int lane, Chunk& out) {
-    const int n_seg = a.n_expert + 2;
-    int before = 0;
-    for (int base = 0; base < n_seg; base += 512) {
-        int v[9], total = 0;
+// 512 experts from `base` on, eight a lane: where each run starts, and the wave's inclusive sum of their chunks. The offsets are
+// clamped to [0, T] and a run that ends before it starts is empty: whatever the table holds, every chunk's rows are in [0, T).
+template <int MT_LOG2> struct Runs {
+    int v[9], own, incl;
+    static __device__ __forceinline__ int chunks(int len) { return (max(len, 0) + (1 << MT_LOG2) - 1) >> MT_LOG2; }
+    __device__ __forceinline__ void read(const Exl3c4DevGemm& a, int base, int lane) {
+        struct __attribute__((packed, aligned(4))) Four { int v[4]; };
+        const int i = base + 8 * lane;
+        if (i + 8 <= a.n_expert) {                               // (16-byte loads: a load a value costs nine times the requests)
+            const Four p = *(const Four*)(a.off + i), q = *(const Four*)(a.off + i + 4);
 #pragma unroll
-        for (int j = 0; j < 9; ++j) {                            // where segment i starts
-            const int i = base + 8 * lane + j;
-            const int o = a.off[min(max(i - 1, 0), a.n_expert)];
-            v[j] = i <= 0 ? 0 : i > a.n_expert + 1 ? a.T : min(max(o, 0), a.T);
+            for (int j = 0; j < 4; ++j) v[j] = p.v[j], v[4 + j] = q.v[j];
+            v[8] = a.off[i + 8];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 9; ++j) v[j] = a.off[min(i + j, a.n_expert)];
         }
+        own = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) total += (max(v[j + 1] - v[j], 0) + (1 << MT_LOG2) - 1) >> MT_LOG2;
-        const int incl = wave_scan_incl(total);
-        int r = c - before - (incl - total);                     // the chunk's number among this lane's
-        const uint64_t hit = __ballot(r >= 0 && r < total);
-        if (hit) {
-            int seg = 0, row0 = 0, rows = 0;
-            bool found = false;
+        for (int j = 0; j < 9; ++j) v[j] = min(max(v[j], 0), a.T);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int len = max(v[j + 1] - v[j], 0), n = (len + (1 << MT_LOG2) - 1) >> MT_LOG2;
-                if (!found && r < n) {
-                    found = true;
-                    seg = base + 8 * lane + j;
-                    row0 = v[j] + (r << MT_LOG2);
-                    rows = min(1 << MT_LOG2, len - (r << MT_LOG2));
-                }
-                r -= n;
-            }
-            const int from = __builtin_ctzll(hit);
-            seg = __builtin_amdgcn_readlane(seg, from);
-            out.row0 = __builtin_amdgcn_readlane(row0, from);
-            out.rows = __builtin_amdgcn_readlane(rows, from);
-            out.expert = seg == 0 || seg == n_seg - 1 ? -1 : seg - 1;
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(incl, 63);
+        for (int j = 0; j < 8; ++j) own += chunks(v[j + 1] - v[j]);
+        incl = wave_scan_incl(own);
     }
-    return false;
+    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(incl, 63); }
+    // chunk c of these (c < total())
+    __device__ __forceinline__ void find(int base, int lane, int c, Chunk& out) const {
+        int r = c - (incl - own), e = 0, row0 = 0, rows = 0;
+        const uint64_t hit = __ballot(r >= 0 && r < own);
+        bool found = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int len = max(v[j + 1] - v[j], 0), n = chunks(len);
+            if (!found && r < n) {
+                found = true;
+                e = base + 8 * lane + j;
+                row0 = v[j] + (r << MT_LOG2);
+                rows = min(1 << MT_LOG2, len - (r << MT_LOG2));
+            }
+            r -= n;
+        }
+        const int from = __builtin_ctzll(hit);
+        out.expert = __builtin_amdgcn_readlane(e, from);
+        out.row0 = __builtin_amdgcn_readlane(row0, from);
+        out.rows = __builtin_amdgcn_readlane(rows, from);
+    }
+};
+
+// The workgroup's chunk of at most 2^MT_LOG2 rows and its column tile, rows 0 if it has none. The launch's units are its chunks -- the
+// experts', then those of the rows before the first run and behind the last one -- each with its column tiles in turn. One wave of the workgroup
+// finds its unit from the offsets (one read and one scan for 512 experts), so a launch needs no plan before it.
+// XCD: the units are cut into eight ranges, one an XCD (workgroups go to the XCDs in turn), whose L2 then holds a chunk's rows for all its
+// tiles and an expert's weights for all its chunks. Else neighbouring units go to different XCDs, which read one stretch
+// of weights together: faster where each weight is read about once (512 experts of about 12 rows in bf16: 579 us against 597; of 40 in MX4 154
+// against 174).
+template <int MT_LOG2, bool XCD>
+__device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
+    typedef Runs<MT_LOG2> R;
+    Chunk out = { -1, 0, 0, 0 };
+    R s;
+    int live = 0;
+    for (int base = 0; base < a.n_expert; base += 512) {
+        s.read(a, base, lane);
+        live += s.total();
+    }
+    const int head = min(max(a.off[0], 0), a.T), tail = min(max(a.off[a.n_expert], 0), a.T);
+    const int n_head = R::chunks(head), total = live + n_head + R::chunks(a.T - tail);
+    const uint32_t units = (uint32_t)total * (uint32_t)a.tiles, x = blockIdx.x & 7u, i = blockIdx.x >> 3;
+    uint32_t unit = blockIdx.x;
+    if (XCD) {
+        if (i >= (units >> 3) + (x < (units & 7u))) return out;
+        unit = x * (units >> 3) + min(x, units & 7u) + i;
+    } else if (unit >= units) {
+        return out;
+    }
+    int c = (int)(unit / (uint32_t)a.tiles);
+    out.tile = (int)(unit - (uint32_t)c * (uint32_t)a.tiles);
+    if (c >= live) {
+        c -= live;
+        const int start = c < n_head ? 0 : tail, end = c < n_head ? head : a.T;
+        out.row0 = start + ((c < n_head ? c : c - n_head) << MT_LOG2);
+        out.rows = min(1 << MT_LOG2, end - out.row0);
+    } else if (a.n_expert <= 512) {
+        s.find(0, lane, c, out);
+    } else {
+        for (int base = 0;; base += 512) {
+            s.read(a, base, lane);
+            if (c < s.total()) {
+                s.find(base, lane, c, out);
+                break;
+            }
+            c -= s.total();
+        }
+    }
+    return out;
+}
+// The same for the whole workgroup, by its first wave.
+template <int MT_LOG2, bool XCD>
+__device__ __forceinline__ Chunk my_unit(const Exl3c4DevGemm& a, int lane, int wave) {
+    __shared__ Chunk unit;
+    if (wave == 0) {
+        const Chunk c = find_unit<MT_LOG2, XCD>(a, lane);
+        if (lane == 0) unit = c;
+    }
+    __syncthreads();
+    return { __builtin_amdgcn_readfirstlane(unit.expert), __builtin_amdgcn_readfirstlane(unit.row0),
+             __builtin_amdgcn_readfirstlane(unit.rows), __builtin_amdgcn_readfirstlane(unit.tile) };
 }
 
 // The row of x that sorted row i reads, or -1: none (the row is zeros).
@@ -262,10 +324,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
     __shared__ int alive[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const int c = blockIdx.x / a.tiles, tile = blockIdx.x - c * a.tiles;
-    Chunk ch;
-    if (!find_chunk<ROWS_LOG2>(a, c, lane, ch)) return;
-    const int n0 = tile * (SW ? 16 : 32);
+    const Chunk ch = my_unit<ROWS_LOG2, false>(a, lane, wave);
+    if (ch.rows == 0) return;
+    const int n0 = ch.tile * (SW ? 16 : 32);
     const int ysz = a.y_type == EXL3C4_F32 ? 4 : 2;
     if (ch.expert >= 0) {
         const int xr = l16 < ch.rows ? x_row(a, ch.row0 + l16) : -1;
@@ -332,14 +393,18 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 // Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, one store.
 __device__ const uint4 k_zero = { 0, 0, 0, 0 };                 // what loads read past the end of a row
 
-__device__ __forceinline__ void dma16(const void* from, void* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
-                                     (__attribute__((address_space(3))) uint32_t*)lds, 16, 0, 0);
+// 16 or 4 bytes a lane from memory to LDS at `lds` (uniform; lane after lane). As asm, so that the compiler does not hold every
+// later LDS read until it is done (it cannot tell one stage's buffer from another's): wait_loads and the barriers order
+// them. No register is written; the address is read at issue, and s_nop keeps m0's wait state.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"                   // that m0 is reserved: nothing holds a value in it here
+__device__ __forceinline__ void dma16(const void* from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
-__device__ __forceinline__ void dma4(const void* from, void* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
-                                     (__attribute__((address_space(3))) uint32_t*)lds, 4, 0, 0);
+__device__ __forceinline__ void dma4(const void* from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // Until at most N of the wave's loads are out, and none of its LDS reads.
 template <int N> __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
@@ -369,10 +434,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
-    Chunk ch;
-    const int c = blockIdx.x / a.tiles, tile = blockIdx.x - c * a.tiles;
-    if (!find_chunk<MT_LOG2>(a, c, lane, ch)) return;
-    const int n0 = tile * (SW ? NT / 2 : NT);                    // the tile's first column of y
+    const Chunk ch = my_unit<MT_LOG2, (MT_LOG2 >= 7)>(a, lane, wave);
+    if (ch.rows == 0) return;
+    const int n0 = ch.tile * (SW ? NT / 2 : NT);                    // the tile's first column of y
     // row r of the tile -> a row of the weight (past the last one: it again, not stored)
     auto w_row = [&](int r) {
         if (!SW) return min(n0 + r, a.N - 1);
@@ -413,8 +477,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
             wsp[i] = wse + (int64_t)w_row(r) * a.ws_pitch + (G::MIXED ? 0 : 4 * (lane & 1));
         }
         const int stages = (a.K + KS - 1) / KS;
+        const uint32_t at0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
         auto load = [&](int t, int buf) {
-            char* to = lds + buf * G::STAGE;
+            const uint32_t to = at0 + buf * G::STAGE;
             const int64_t k = (int64_t)t * KS;
             const bool full = k + KS <= a.K;
 #pragma unroll
@@ -611,7 +676,7 @@ int64_t chunk_bound(const Exl3c4DevGemm& a, int rows) {
 template <int XT, int WT, bool SW>
 int launch_rows(Exl3c4DevGemm& a, hipStream_t st) {
     a.tiles = (a.n_out + (SW ? 15 : 31)) / (SW ? 16 : 32);
-    const int64_t grid = chunk_bound(a, 1 << ROWS_LOG2) * a.tiles;
+    const int64_t grid = (chunk_bound(a, 1 << ROWS_LOG2) * a.tiles + 7) / 8 * 8;
     if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
     hipLaunchKernelGGL((k_mg_rows<XT, WT, SW>), dim3((unsigned)grid), dim3(64 * WAVES), 0, st, a);
     return launched();
@@ -621,7 +686,7 @@ template <int XT, int WT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS
 int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr int cols = SW ? NT / 2 : NT;
     a.tiles = (a.n_out + cols - 1) / cols;
-    const int64_t grid = chunk_bound(a, 1 << MT_LOG2) * a.tiles;
+    const int64_t grid = (chunk_bound(a, 1 << MT_LOG2) * a.tiles + 7) / 8 * 8;
     if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
     hipLaunchKernelGGL((k_mg_tile<XT, WT, SW, MT_LOG2, NT, WM, WN, BUFS>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
     return launched();

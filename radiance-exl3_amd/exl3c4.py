@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-from typing import NamedTuple
 
 import numpy as np
 
@@ -57,12 +56,24 @@ class Gemm(C.Structure):
                 ("ws_stride", _i64), ("sorted_tok", _p), ("expert_offset", _p), ("y", _p), ("y_pitch", _i64)]
 
 
-class Mx4(NamedTuple):
-    """MX4 rows (include/exl3c4.h): codes uint8 [..., rows, >= 16 ceil(cols / 32)], scales uint8 [..., rows,
-    >= ceil(cols / 32) up to a multiple of 4], the columns they stand for."""
-    codes: object
-    scales: object
-    cols: int
+class Mx4:
+    """MX4 rows (include/exl3c4.h) of values [..., rows, cols]: codes uint8 [..., rows, >= 16 ceil(cols / 32)], scales uint8
+    [..., rows, >= ceil(cols / 32)], the columns they stand for. The conversions take a row's pitches from the tensors once,
+    here; leading dimensions have to step evenly as one for them (for moe_gemm they need not)."""
+    __slots__ = ("codes", "scales", "cols", "shape", "c_ptr", "s_ptr", "c_pitch", "s_pitch")
+
+    def __init__(self, codes, scales, cols: int):
+        nb = (cols + 31) // 32
+        if codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] < 16 * nb or scales.shape[-1] < nb or \
+                codes.element_size() != 1 or scales.element_size() != 1 or codes.device != scales.device:
+            raise ValueError("the MX4 planes do not fit each other or their columns")
+        self.codes, self.scales, self.cols, self.shape = codes, scales, cols, codes.shape[:-1] + (cols,)
+        self.c_ptr, self.s_ptr, self.c_pitch, self.s_pitch = codes.data_ptr(), scales.data_ptr(), None, None
+
+    def pitches(self):
+        if self.c_pitch is None:
+            self.c_pitch, self.s_pitch = _rows(self.codes)[1], _rows(self.scales)[1]
+        return self.c_pitch, self.s_pitch
 
 
 def lib():
@@ -446,9 +457,14 @@ def launch_status(o: Op, scratch) -> int:
 F32 = 2
 
 
+_dtypes = {}
+
+
 def _dt(t):
-    import torch
-    return {torch.float32: F32, torch.float16: 0, torch.bfloat16: 1}[t.dtype]
+    if not _dtypes:
+        import torch
+        _dtypes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return _dtypes[t.dtype]
 
 
 def router_topk(logits, top_k: int, renorm: bool = True, ids=None, w=None, stream=None) -> int:
@@ -486,13 +502,13 @@ def moe_gather(y, y_bf16: bool, w, row_of, out, stream=None) -> int:
 
 
 # ------------------------------------------------------------------------------------------ 16-bit and MX4 experts
-def _launch_on(t, stream, call) -> int:
-    """call(stream) with t's device current and, by default, on that device's current stream."""
+def _launch_on(device, stream, fn, *args) -> int:
+    """fn(*args, stream) with `device` current and, by default, on that device's current stream."""
     import torch
-    if t.device.index == torch.cuda.current_device():
-        return int(call(_stream(stream)))
-    with torch.cuda.device(t.device):
-        return int(call(_stream(stream)))
+    if device.index == torch.cuda.current_device():
+        return fn(*args, (torch.cuda.current_stream() if stream is None else stream).cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, (torch.cuda.current_stream() if stream is None else stream).cuda_stream)
 
 
 def _rows(t):
@@ -514,13 +530,6 @@ def _rows(t):
     return rows, cols if pitch is None else pitch
 
 
-def _check_mx4(q: Mx4, lead, cols: int):
-    nb = (cols + 31) // 32
-    if q.cols != cols or q.codes.shape[:-1] != lead or q.scales.shape[:-1] != lead or \
-            q.codes.shape[-1] < 16 * nb or q.scales.shape[-1] < nb:
-        raise ValueError("the MX4 planes do not fit the values' shape")
-
-
 def mx4_empty(shape, device="cuda") -> Mx4:
     """Uninitialised MX4 rows for values of `shape` ([..., rows, cols])."""
     import torch
@@ -532,18 +541,22 @@ def mx4_empty(shape, device="cuda") -> Mx4:
 
 def mx4_quant(x, q: Mx4, stream=None) -> int:
     """exl3c4_mx4_quant of x [..., cols] (f32 / f16 / bf16) into q; returns the status."""
-    _check_mx4(q, x.shape[:-1], x.shape[-1])
-    (n, pitch), cp, sp = _rows(x), _rows(q.codes)[1], _rows(q.scales)[1]
-    return _launch_on(x, stream, lambda st: lib().exl3c4_mx4_quant(_ptr(x), _dt(x), n, q.cols, pitch, _ptr(q.codes), cp,
-                                                                   _ptr(q.scales), sp, st))
+    if x.shape != q.shape or x.device != q.codes.device:
+        raise ValueError("x and q have other shapes or devices")
+    n, pitch = _rows(x)
+    cp, sp = q.pitches()
+    return _launch_on(x.device, stream, lib().exl3c4_mx4_quant, x.data_ptr(), _dt(x), n, q.cols, pitch, q.c_ptr, cp,
+                      q.s_ptr, sp)
 
 
 def mx4_dequant(q: Mx4, out, stream=None) -> int:
     """exl3c4_mx4_dequant of q into out [..., cols] (f32 / f16 / bf16); returns the status."""
-    _check_mx4(q, out.shape[:-1], out.shape[-1])
-    (n, pitch), cp, sp = _rows(out), _rows(q.codes)[1], _rows(q.scales)[1]
-    return _launch_on(out, stream, lambda st: lib().exl3c4_mx4_dequant(_ptr(q.codes), cp, _ptr(q.scales), sp, n, q.cols,
-                                                                       _ptr(out), _dt(out), pitch, st))
+    if out.shape != q.shape or out.device != q.codes.device:
+        raise ValueError("q and out have other shapes or devices")
+    n, pitch = _rows(out)
+    cp, sp = q.pitches()
+    return _launch_on(out.device, stream, lib().exl3c4_mx4_dequant, q.c_ptr, cp, q.s_ptr, sp, n, q.cols, out.data_ptr(),
+                      _dt(out), pitch)
 
 
 def _planes(t):
@@ -565,9 +578,6 @@ def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT
     if Kw != K or y.shape[1] != (N // 2 if act == ACT_SWIGLU else N) or \
             expert_offset.numel() < E + 1:
         raise ValueError("x, w, expert_offset and y do not fit together")
-    for t, q in ((xv, x), (wv, w)):
-        if isinstance(q, Mx4):
-            _check_mx4(q, t.shape[:-1], K)
     for t, n in ((sorted_tok, g.T), (expert_offset, E + 1)):
         if t is not None and (t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous() or t.numel() < n):
             raise ValueError("sorted_tok and expert_offset are contiguous int32, of T and n_expert + 1 values at least")
@@ -600,7 +610,7 @@ def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT
 
 def moe_gemm(g: Gemm, stream=None) -> int:
     """exl3c4_moe_gemm on the device of g's tensors; returns the status."""
-    return _launch_on(g, stream, lambda st: lib().exl3c4_moe_gemm(C.byref(g), st))
+    return _launch_on(g.device, stream, lib().exl3c4_moe_gemm, C.byref(g))
 
 
 def alloc_scratch(o: Op, device="cuda"):
