@@ -304,7 +304,7 @@ int exl3c4_mx4_dequant(const void* codes, int64_t codes_pitch, const void* scale
  * 16-bit operands: K % 8 == 0, base, pitch and stride in multiples of 16 bytes; with an MX4 operand K % 32 == 0; scale bases, pitches
  * and strides in multiples of 4 bytes. N is any. Refusals: INVAL (an unknown act, a required operand absent), DTYPE (another pair of
  * types), SHAPE (extents below one, K or N as above, fewer x rows than read, extents past 2^31 - 1 or more tiles than a launch holds),
- * STRIDE (a pitch or a stride below what it steps over), ALIGN. */
+ * STRIDE (a pitch or a stride below what it steps over, a weight's pitch past 2^27 bytes), ALIGN. */
 typedef struct Exl3c4Gemm {
     int32_t        x_type, w_type, y_type, act;
     int64_t        N, K, n_expert, top_k, T;

@@ -8,8 +8,9 @@
 
 /* extents that the kernels hold in 32 bits, with room for a tile's rounding up */
 #define MAX_EXTENT (INT32_MAX - 65536)
-/* byte pitches: a tile's offsets inside an operand stay far from 64 bits */
+/* byte pitches: offsets inside an operand stay far from 64 bits, and those of a weight's 16 rows in 32 */
 #define MAX_PITCH ((int64_t)1 << 40)
+#define MAX_W_PITCH ((int64_t)1 << 27)
 
 static int size_of(int32_t type) { return type == EXL3C4_F32 ? 4 : 2; }
 static int is_float(int32_t type) { return type == EXL3C4_F16 || type == EXL3C4_BF16 || type == EXL3C4_F32; }
@@ -84,6 +85,7 @@ int exl3c4_moe_gemm(const Exl3c4Gemm* g, void* stream) {
     if (rc) return rc;
     rc = operand_check(g->w_type, g->w, g->w_scales, g->w_pitch, g->ws_pitch, g->K, &w_bytes);
     if (rc) return rc;
+    if (w_bytes > MAX_W_PITCH || g->ws_pitch > MAX_W_PITCH) return EXL3C4_E_STRIDE;
     /* an entry's last row ends with its last column */
     const int64_t w_row = g->w_type == EXL3C4_MX4 ? g->K / 2 : 2 * g->K;
     if (g->w_stride != 0 && g->w_stride < (g->N - 1) * w_bytes + w_row) return EXL3C4_E_STRIDE;

@@ -8,9 +8,11 @@
 // operand (columns of D): lane l ends with D[m = 4 g + r][n = l % 16], r = 0 .. 3.
 //
 // MX4 WEIGHTS AGAINST 16-BIT x. bf16 holds e2m1 x 2^s exactly, so with bf16 x a lane's block is converted with its scale
-// (v_cvt_scalef32_pk_bf16_fp4) and multiplied as bf16. f16 does not hold the scales' range: with f16 x the codes alone are
-// converted, the four lane groups' words are exchanged so that one instruction's 32 columns are one block, and its sums
-// are scaled in f32 as they are added. Either way every product is exact.
+// (v_cvt_scalef32_pk_bf16_fp4) and multiplied as bf16. f16 does not hold the scales' range: with f16 x a row's blocks are converted
+// relative to the largest scale among some hundred columns (its level), where those within 2^-13 of it are exact in f16, and the
+// sums are scaled in f32 as they are added; blocks further down, if any of them is not all zeros, have passes of their own. Either
+// way every product is exact. (Scaling each block's sums by itself, one matrix instruction a block, took 125 us where this
+// takes 64: 32 tokens, top-10 of 512 experts, gate and up 2048 -> 2 x 512.)
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -160,8 +162,15 @@ __device__ __forceinline__ int x_row(const Exl3c4DevGemm& a, int i) {
     return r < a.x_rows ? r : -1;
 }
 
-__device__ __forceinline__ const char* entry(const char* base, int64_t stride, int e) {
-    return stride ? base + (int64_t)e * stride : ((const char* const*)base)[e];
+// Weights by addresses known to be global memory: a pointer out of a table is a flat one otherwise, whose loads also hold up LDS.
+typedef const __attribute__((address_space(1))) char* gaddr;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load16(gaddr p) {
+    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)p);
+}
+__device__ __forceinline__ uint32_t load4(gaddr p) { return *(const __attribute__((address_space(1))) uint32_t*)p; }
+__device__ __forceinline__ gaddr entry(const void* base, int64_t stride, int e) {
+    return stride ? (gaddr)base + (int64_t)e * stride : ((const gaddr*)base)[e];
 }
 
 // silu(g) u in f32: g / (1 + exp(-g)) by the hardware's exp2 and reciprocal (a few f32 steps from the exact value,
@@ -214,26 +223,18 @@ __device__ __forceinline__ f32x4 mma_mx4(const uint4& a, int sa, const uint4& b,
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, BYTE, sa, BYTE, sb);
 }
 
-// 8 codes (a word) as 8 bf16 with their scale, or 8 f16 without.
-__device__ __forceinline__ uint4 to_bf16(uint32_t q, float scale) {
-    return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0)),
-             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1)),
-             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 2)),
-             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3)) };
-}
-__device__ __forceinline__ uint4 to_f16(uint32_t q) {
-    return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, 1.f, 0)),
-             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, 1.f, 1)),
-             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, 1.f, 2)),
-             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, 1.f, 3)) };
-}
-// A 4 x 4 transpose of words over the lane groups: group g's word j to group j's word g.
-__device__ __forceinline__ uint4 exchange(const uint4& q) {
-    const auto p = __builtin_amdgcn_permlane32_swap(q.x, q.z, false, false);
-    const auto r = __builtin_amdgcn_permlane32_swap(q.y, q.w, false, false);
-    const auto s = __builtin_amdgcn_permlane16_swap(p[0], r[0], false, false);
-    const auto t = __builtin_amdgcn_permlane16_swap(p[1], r[1], false, false);
-    return { s[0], s[1], t[0], t[1] };
+// 8 codes (a word) times a scale as 8 bf16 or 8 f16.
+template <int XT> __device__ __forceinline__ uint4 widen(uint32_t q, float scale) {
+    if constexpr (XT == BF16)
+        return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3)) };
+    else
+        return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 3)) };
 }
 // 2^(byte - 127) as an operand of the conversions (they read the exponent field), and as an f32 (255: NaN).
 __device__ __forceinline__ float scale_arg(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -242,141 +243,250 @@ __device__ __forceinline__ float scale_f32(uint32_t byte) {
     return v[0];
 }
 
-// ------------------------------------------------------------------------------------------ few rows an expert
-// A workgroup: a chunk of up to 16 rows against 32 weight rows (with SwiGLU 16 gate rows and their 16 up rows), the four
-// waves each a quarter of k; the weights go from memory straight to the matrix units' operands, each byte read once, and
-// the quarters' sums meet in LDS in a fixed order.
-constexpr int ROWS_LOG2 = 4;
-constexpr int WAVES = 4;
+// The levels of f16's passes: the largest scale byte of a word (of four), and the largest below `below` (-1: none).
+__device__ __forceinline__ int top_byte(uint32_t w) {
+    const uint32_t e = w & 0x00FF00FFu, o = (w >> 8) & 0x00FF00FFu;
+    return (int)max(max(e & 0xFFFFu, o & 0xFFFFu), max(e >> 16, o >> 16));
+}
+__device__ __forceinline__ int top_byte_below(uint32_t w, int below) {
+    int m = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int b = (int)((w >> (8 * i)) & 255u);
+        m = b < below ? max(m, b) : m;
+    }
+    return m;
+}
+constexpr int LEVEL = 13;                                       // e2m1 x 2^-13 is a normal f16: 2^-14 at least
+// A block's scale in a pass over the blocks within LEVEL of `level` and below `below`; the others as 2^-127, which f16 rounds to 0.
+__device__ __forceinline__ float pass_scale(int byte, int level, int below) {
+    return byte >= level - LEVEL && byte < below ? __uint_as_float((uint32_t)(byte - level + 127) << 23) : 0.f;
+}
+__device__ __forceinline__ bool any_code(const uint4& q) { return ((q.x | q.y | q.z | q.w) & 0x77777777u) != 0; }
 
-// What one matrix step reads of the two weight strips and of x, and its products. FULL: every lane's bytes are inside
+// ------------------------------------------------------------------------------------------ few rows an expert
+// A workgroup: a chunk of up to 16 rows against NS strips of 16 weight rows (with SwiGLU half of them gate rows and half their up
+// rows), each wave a part of k; the weights go from memory straight to the matrix units' operands, each byte read
+// once, and the parts' sums meet in LDS in a fixed order.
+constexpr int ROWS_LOG2 = 4;
+
+// What one matrix step reads of the NS weight strips and of x, and its products. FULL: every lane's bytes are inside
 // the rows; else what lies past K reads as zeros (and their scales as 2^-127, never as a NaN).
-template <int XT, int WT> struct Step {
+template <int XT, int WT, int NS> struct Step {
     static constexpr int KB = WT == MX4 ? 128 : 32;             // columns of a weight row's 64 bytes
     static constexpr int NX = WT == MX4 && XT != MX4 ? 4 : 1;
-    uint4 q[2], x[NX];
-    uint32_t sc[2], xsc;
+    uint4 x[NX];
+    uint32_t xsc;
 
+    // w: the strips' first rows (uniform); at: the lane's row and bytes in a strip
     template <bool FULL>
-    __device__ __forceinline__ void load(int t, int K, int g, const char* xp, const uint8_t* xs, const char* const* w,
-                                         const uint8_t* const* ws) {
-        const int64_t k = (int64_t)t * KB;
-        const uint4 none = { 0, 0, 0, 0 };
-        const bool in = FULL || k + (KB / 4) * g < K;
+    static __device__ __forceinline__ void load_w(uint4* q, int t, int K, int g, const gaddr* w, uint32_t at) {
+        const bool in = FULL || (int64_t)t * KB + (KB / 4) * g < K;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            q[s] = in ? *(const uint4*)(w[s] + (int64_t)t * 64) : none;
-            if constexpr (WT == MX4) sc[s] = *(const uint32_t*)(ws[s] + 4 * (int64_t)t);
-            if constexpr (WT == MX4) if (!FULL) sc[s] &= live_bytes(K, k);
-        }
+        for (int s = 0; s < NS; ++s) q[s] = in ? load16(w[s] + (at + 64u * (uint32_t)t)) : uint4{ 0, 0, 0, 0 };
+    }
+    // has_x: the lane's row holds one (the others load nothing: what the products of their rows are is not used)
+    template <bool FULL>
+    __device__ __forceinline__ void load_x(int t, int K, int g, const char* xp, const uint8_t* xs, bool has_x) {
+        const int64_t k = (int64_t)t * KB;
+        const bool in = has_x && (FULL || k + (KB / 4) * g < K);
+#pragma unroll
+        for (int j = 0; j < NX; ++j) x[j] = uint4{ 0, 0, 0, 0 };
+        xsc = 0;
         if constexpr (XT == MX4) {
-            x[0] = in ? *(const uint4*)(xp + (int64_t)t * 64) : none;
-            xsc = *(const uint32_t*)(xs + 4 * (int64_t)t);
+            if (in) x[0] = *(const uint4*)(xp + (int64_t)t * 64);
+            if (in) xsc = *(const uint32_t*)(xs + 4 * (int64_t)t);
             if (!FULL) xsc &= live_bytes(K, k);
         } else if constexpr (WT != MX4) {
-            x[0] = in ? *(const uint4*)(xp + 2 * (k + 8 * g)) : none;
+            if (in) x[0] = *(const uint4*)(xp + 2 * (k + 8 * g));
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                // bf16: the lane's own block, word j; f16: block j, the lane group's word
-                const int64_t c = k + (XT == BF16 ? 32 * g + 8 * j : 32 * j + 8 * g);
-                x[j] = FULL || c < K ? *(const uint4*)(xp + 2 * c) : none;
+                if (in) x[j] = *(const uint4*)(xp + 2 * (k + 32 * g + 8 * j));   // of the lane's block, word j
             }
         }
     }
-    // the scale bytes of the step's blocks before column K
+    // the scale bytes of a step's blocks before column K
     static __device__ __forceinline__ uint32_t live_bytes(int K, int64_t k) {
         const int n = (int)min((int64_t)(K - k) / 32, (int64_t)4);
         return n >= 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
     }
-    __device__ __forceinline__ void multiply(int g, f32x4* acc) const {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            if constexpr (WT != MX4) {
-                acc[s] = mma<XT>(x[0], q[s], acc[s]);
-            } else if constexpr (XT == MX4) {
-                acc[s] = mma_mx4(x[0], (xsc >> (8 * g)) & 255, q[s], (sc[s] >> (8 * g)) & 255, acc[s]);
-            } else if constexpr (XT == BF16) {
-                const float f = scale_arg((sc[s] >> (8 * g)) & 255);
-                const uint32_t word[4] = { q[s].x, q[s].y, q[s].z, q[s].w };
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[s] = mma<BF16>(x[j], to_bf16(word[j], f), acc[s]);
-            } else {
-                const uint4 e = exchange(q[s]);
-                const uint32_t word[4] = { e.x, e.y, e.z, e.w };
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float f = scale_f32((sc[s] >> (8 * j)) & 255);
-                    const f32x4 p = mma<F16>(x[j], to_f16(word[j]), f32x4{ 0, 0, 0, 0 });
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[r], f, acc[s][r]);
-                }
-            }
+    // a strip's 16 bytes and their scale: MX4 x the scale's byte, else as an operand of the conversion
+    __device__ __forceinline__ f32x4 multiply(int g, const uint4& q, uint32_t sc, f32x4 acc) const {
+        if constexpr (WT != MX4) {
+            return mma<XT>(x[0], q, acc);
+        } else if constexpr (XT == MX4) {
+            return mma_mx4(x[0], (xsc >> (8 * g)) & 255, q, (sc >> (8 * g)) & 255, acc);
+        } else {
+            return multiply_by(q, scale_arg((sc >> (8 * g)) & 255), acc);
         }
+    }
+    __device__ __forceinline__ f32x4 multiply_by(const uint4& q, float f, f32x4 acc) const {
+        const uint32_t word[4] = { q.x, q.y, q.z, q.w };
+#pragma unroll
+        for (int j = 0; j < NX; ++j) acc = mma<XT>(x[j], widen<XT>(word[j], f), acc);
+        return acc;
     }
 };
 
-template <int XT, int WT, bool SW>
-__global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
-    typedef Step<XT, WT> S;
-    constexpr int AHEAD = S::NX == 4 ? 2 : 4;                   // steps whose loads are out together
-    __shared__ f32x4 part[WAVES][2][64];
+template <int XT, int WT, bool SW, int NS, int WV, int AHEAD>
+__global__ __launch_bounds__(64 * WV) void k_mg_rows(Exl3c4DevGemm a) {
+    typedef Step<XT, WT, NS> S;
+    constexpr int OUT = SW ? NS / 2 : NS;                        // strips of y
+    __shared__ f32x4 part[WV][NS][64];
     __shared__ int alive[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const Chunk ch = my_unit<ROWS_LOG2, false>(a, lane, wave);
     if (ch.rows == 0) return;
-    const int n0 = ch.tile * (SW ? 16 : 32);
+    const int n0 = ch.tile * (16 * OUT);
+    // where strip s of y starts: at the last 16 columns if it would pass them (what it repeats is not stored)
+    auto start_of = [&](int s) { return max(min(n0 + 16 * s, a.n_out - 16), 0); };
     const int ysz = a.y_type == EXL3C4_F32 ? 4 : 2;
     if (ch.expert >= 0) {
+        const gaddr we = entry(a.w, a.w_stride, ch.expert);
+        const gaddr wse = WT == MX4 ? entry(a.ws, a.ws_stride, ch.expert) : nullptr;
+        gaddr w[NS], ws[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int64_t n = start_of(s % OUT) + (s / OUT) * a.n_out;
+            w[s] = we + n * a.w_pitch;
+            ws[s] = WT == MX4 ? wse + n * a.ws_pitch : nullptr;
+        }
+        const uint32_t row = (uint32_t)min(l16, a.n_out - 1), at = row * (uint32_t)a.w_pitch + 16 * g;
+        const uint32_t s_at = WT == MX4 ? row * (uint32_t)a.ws_pitch : 0;
+        const int steps = (a.K + S::KB - 1) / S::KB;
+        const int to = (int)((int64_t)steps * (wave + 1) / WV), full = min(to, a.K / S::KB);
         const int xr = l16 < ch.rows ? x_row(a, ch.row0 + l16) : -1;
         if (threadIdx.x < 16) alive[threadIdx.x] = xr >= 0;
         const char* x = a.x + (int64_t)max(xr, 0) * a.x_pitch + (XT == MX4 ? 16 * g : 0);
         const uint8_t* xs = XT == MX4 ? a.xs + (int64_t)max(xr, 0) * a.xs_pitch : nullptr;
-        const char* we = entry(a.w, a.w_stride, ch.expert);
-        const uint8_t* wse = WT == MX4 ? (const uint8_t*)entry((const char*)a.ws, a.ws_stride, ch.expert) : nullptr;
-        const char* w[2];
-        const uint8_t* ws[2];
+        const bool has_x = xr >= 0;
+        f32x4 acc[NS] = {};
+        uint4 q[AHEAD][NS];
+        int t = (int)((int64_t)steps * wave / WV);
+        constexpr bool LEVELS = XT == F16 && WT == MX4;
+        // f16 x, MX4 weights: the passes behind the first over steps t .. t + n - 1, each strip's rows from their own level on
+        auto more_passes = [&](int t, int n, int* level) {
+            bool more;
+            do {
+                int below[NS], next[NS];
+                f32x4 p[NS] = {};
+                more = false;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {                            // rows past the last one repeat it and are not stored
-            const int n = SW ? min(n0 + l16, a.n_out - 1) + s * a.n_out : min(n0 + 16 * s + l16, a.N - 1);
-            w[s] = we + (int64_t)n * a.w_pitch + 16 * g;
-            ws[s] = WT == MX4 ? wse + (int64_t)n * a.ws_pitch : nullptr;
-        }
-        const int steps = (a.K + S::KB - 1) / S::KB;
-        const int to = (int)((int64_t)steps * (wave + 1) / WAVES), full = min(to, a.K / S::KB);
-        int t = (int)((int64_t)steps * wave / WAVES);
-        f32x4 acc[2] = {};
-        for (; t + AHEAD <= full; t += AHEAD) {
-            S st[AHEAD];
+                for (int s = 0; s < NS; ++s) {
+                    below[s] = level[s] - LEVEL;
+                    next[s] = -1;
+                    for (int u = 0; u < n; ++u)
+                        next[s] = max(next[s], top_byte_below(load4(ws[s] + (s_at + 4u * (uint32_t)(t + u))) &
+                                                              S::live_bytes(a.K, (int64_t)(t + u) * S::KB), below[s]));
+                }
+                for (int u = 0; u < n; ++u) {
+                    S st;
+                    uint4 v[NS];
+                    S::template load_w<false>(v, t + u, a.K, g, w, at);
+                    st.template load_x<false>(t + u, a.K, g, x, xs, has_x);
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) st[u].template load<true>(t + u, a.K, g, x, xs, w, ws);
+                    for (int s = 0; s < NS; ++s) {
+                        const int b = ((load4(ws[s] + (s_at + 4u * (uint32_t)(t + u))) &
+                                        S::live_bytes(a.K, (int64_t)(t + u) * S::KB)) >> (8 * g)) & 255;
+                        p[s] = st.multiply_by(v[s], next[s] < 0 ? 0.f : pass_scale(b, next[s], below[s]), p[s]);
+                        more |= next[s] >= 0 && b < next[s] - LEVEL && any_code(v[s]);
+                    }
+                }
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) st[u].multiply(g, acc);
+                for (int s = 0; s < NS; ++s) {
+                    const float f = next[s] < 0 ? 0.f : scale_f32(next[s]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[s][r], f, acc[s][r]);
+                    level[s] = next[s] < 0 ? -1000 : next[s];
+                }
+            } while (__any(more));
+        };
+        for (; t + 4 <= full; t += 4) {                          // (the scale words of four steps are one load a strip)
+            uint4 sc[NS];
+            f32x4 p[NS] = {};
+            int level[NS];
+            bool more = false;
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                if constexpr (WT == MX4) sc[s] = load16(ws[s] + (s_at + 4u * (uint32_t)t));
+#pragma unroll
+            for (int h = 0; h < 4; h += AHEAD) {
+                S st[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) S::template load_w<true>(q[u], t + h + u, a.K, g, w, at);
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) st[u].template load_x<true>(t + h + u, a.K, g, x, xs, has_x);
+                if (LEVELS && h == 0)
+#pragma unroll
+                    for (int s = 0; s < NS; ++s)
+                        level[s] = max(max(top_byte(sc[s].x), top_byte(sc[s].y)), max(top_byte(sc[s].z), top_byte(sc[s].w)));
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) {
+                        const uint32_t word = h + u == 0 ? sc[s].x : h + u == 1 ? sc[s].y : h + u == 2 ? sc[s].z : sc[s].w;
+                        if constexpr (LEVELS) {
+                            const int b = (word >> (8 * g)) & 255;
+                            p[s] = st[u].multiply_by(q[u][s], pass_scale(b, level[s], 256), p[s]);
+                            more |= b < level[s] - LEVEL && any_code(q[u][s]);
+                        } else {
+                            acc[s] = st[u].multiply(g, q[u][s], word, acc[s]);
+                        }
+                    }
+            }
+            if constexpr (LEVELS) {
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const float f = scale_f32(level[s]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[s][r], f, acc[s][r]);
+                }
+                if (__any(more)) more_passes(t, 4, level);
+            }
         }
         for (; t < to; ++t) {
-            S st;
-            st.template load<false>(t, a.K, g, x, xs, w, ws);
-            st.multiply(g, acc);
+            if constexpr (LEVELS) {
+                int level[NS];
+#pragma unroll
+                for (int s = 0; s < NS; ++s) level[s] = 256 + LEVEL;
+                more_passes(t, 1, level);
+            } else {
+                S st;
+                S::template load_w<false>(q[0], t, a.K, g, w, at);
+                st.template load_x<false>(t, a.K, g, x, xs, has_x);
+                const uint32_t live = WT == MX4 ? S::live_bytes(a.K, (int64_t)t * S::KB) : 0;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    uint32_t word = 0;
+                    if constexpr (WT == MX4) word = load4(ws[s] + (s_at + 4u * (uint32_t)t)) & live;
+                    acc[s] = st.multiply(g, q[0][s], word, acc[s]);
+                }
+            }
         }
-        part[wave][0][lane] = acc[0];
-        part[wave][1][lane] = acc[1];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) part[wave][s][lane] = acc[s];
     }
     __syncthreads();
-    // thread -> (row m, column j of the strip), and both strips: their sums at [strip][16 (m / 4) + j][m % 4]
-    const int m = threadIdx.x >> 4, j = threadIdx.x & 15;
+    // thread -> row m, column j of each of its strips: the sums at [strip][16 (m / 4) + j][m % 4]
+    const int j = threadIdx.x & 15, m = (threadIdx.x >> 4) & 15;
     if (m >= ch.rows) return;
-    float v[2] = { 0.f, 0.f };
-    if (ch.expert >= 0 && alive[m]) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int u = 0; u < WAVES; ++u) v[s] += part[u][s][16 * (m >> 2) + j][m & 3];
-        if (SW) v[0] = swiglu(v[0], v[1]);
-    }
+    const bool live = ch.expert >= 0 && alive[m];
     char* y = a.y + (int64_t)(ch.row0 + m) * a.y_pitch;
-    if (n0 + j < a.n_out) store(y + (int64_t)(n0 + j) * ysz, a.y_type, v[0]);
-    if (!SW && n0 + 16 + j < a.n_out) store(y + (int64_t)(n0 + 16 + j) * ysz, a.y_type, v[1]);
+    for (int s = threadIdx.x >> 8; s < OUT; s += WV / 4) {
+        const int col = start_of(s) + j;
+        if (col < n0 + 16 * s || col >= a.n_out) continue;
+        float v[2] = { 0.f, 0.f };
+        if (live) {
+#pragma unroll
+            for (int h = 0; h < (SW ? 2 : 1); ++h)
+#pragma unroll
+                for (int u = 0; u < WV; ++u) v[h] += part[u][s + h * OUT][16 * (m >> 2) + j][m & 3];
+            if (SW) v[0] = swiglu(v[0], v[1]);
+        }
+        store(y + (int64_t)col * ysz, a.y_type, v[0]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------ many rows an expert
@@ -398,10 +508,10 @@ __device__ const uint4 k_zero = { 0, 0, 0, 0 };                 // what loads re
 // them. No register is written; the address is read at issue, and s_nop keeps m0's wait state.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"                   // that m0 is reserved: nothing holds a value in it here
-__device__ __forceinline__ void dma16(const void* from, uint32_t lds) {
+__device__ __forceinline__ void dma16(gaddr from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
-__device__ __forceinline__ void dma4(const void* from, uint32_t lds) {
+__device__ __forceinline__ void dma4(gaddr from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -447,13 +557,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
     for (int r = threadIdx.x; r < MT; r += 64 * WV) rows_x[r] = ch.expert >= 0 && r < ch.rows ? x_row(a, ch.row0 + r) : -1;
     __syncthreads();
     if (ch.expert >= 0) {
-        const char* we = entry(a.w, a.w_stride, ch.expert);
-        const char* wse = WT == MX4 ? entry((const char*)a.ws, a.ws_stride, ch.expert) : nullptr;
+        const gaddr we = entry(a.w, a.w_stride, ch.expert);
+        const gaddr wse = WT == MX4 ? entry(a.ws, a.ws_stride, ch.expert) : nullptr;
         // where each of the wave's loads starts, for this lane: in 128-byte rows lane l takes place l % 8 of row l / 8
         const char* xp[G::XL];
-        const char* wp[G::WL];
+        gaddr wp[G::WL];
         const char* xsp[G::XSL + 1];
-        const char* wsp[G::WSL + 1];
+        gaddr wsp[G::WSL + 1];
 #pragma unroll
         for (int i = 0; i < G::XL; ++i) {
             const int q = wave + i * WV, r = 8 * (G::MIXED ? q >> 1 : q) + (lane >> 3);
@@ -488,26 +598,26 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                 const int col = XT == MX4 ? 32 * ((lane & 7) ^ (r & 7)) : 8 * ((lane & 7) ^ (r & 7)) + (G::MIXED ? 64 * (q & 1) : 0);
                 const char* p = xp[i] + (int64_t)t * G::XROW;
                 if (!full && k + col >= a.K) p = (const char*)&k_zero;
-                dma16(p, to + q * 1024);
+                dma16((gaddr)p, to + q * 1024);
             }
 #pragma unroll
             for (int i = 0; i < G::WL; ++i) {
                 const int q = wave + i * WV, r = G::MIXED ? 16 * q + (lane >> 2) : 8 * q + (lane >> 3);
                 const int col = G::MIXED ? 32 * ((lane & 3) ^ ((r >> 1) & 3)) : (WT == MX4 ? 32 : 8) * ((lane & 7) ^ (r & 7));
-                const char* p = wp[i] + (int64_t)t * G::WROW;
-                if (!full && k + col >= a.K) p = (const char*)&k_zero;
+                gaddr p = wp[i] + (int64_t)t * G::WROW;
+                if (!full && k + col >= a.K) p = (gaddr)&k_zero;
                 dma16(p, to + G::AT_W + q * 1024);
             }
 #pragma unroll
             for (int i = 0; i < G::XSL; ++i) {
                 const char* p = xsp[i] + (int64_t)t * 8;
                 if (!full && k + 128 * (lane & 1) >= a.K) p = (const char*)&k_zero;
-                dma4(p, to + G::AT_XS + ((wave + i * WV) % max(G::XS, 1)) * 256);
+                dma4((gaddr)p, to + G::AT_XS + ((wave + i * WV) % max(G::XS, 1)) * 256);
             }
 #pragma unroll
             for (int i = 0; i < G::WSL; ++i) {
-                const char* p = wsp[i] + (int64_t)t * (KS / 32);
-                if (!full && k + (G::MIXED ? 0 : 128 * (lane & 1)) >= a.K) p = (const char*)&k_zero;
+                gaddr p = wsp[i] + (int64_t)t * (KS / 32);
+                if (!full && k + (G::MIXED ? 0 : 128 * (lane & 1)) >= a.K) p = (gaddr)&k_zero;
                 dma4(p, to + G::AT_WS + ((wave + i * WV) % max(G::WS, 1)) * 256);
             }
         };
@@ -570,11 +680,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                 auto x_at = [&](int m, int u) {
                     return *(const uint4*)(X + ((xr >> 3) + 2 * m) * 2048 + (u >> 3) * 1024 + (l16 & 7) * 128 + 16 * ((u & 7) ^ (l16 & 7)));
                 };
-                if constexpr (XT == BF16) {
-                    float f[TN];
+                int byte[TN];
 #pragma unroll
-                    for (int i = 0; i < TN; ++i)
-                        f[i] = scale_arg(((*(const uint32_t*)(WS + (wr + 16 * i) * 4) & live) >> (8 * g)) & 255);
+                for (int i = 0; i < TN; ++i) byte[i] = ((*(const uint32_t*)(WS + (wr + 16 * i) * 4) & live) >> (8 * g)) & 255;
+                // the products with the weights' blocks scaled by f, added to `to`
+                auto pass = [&](const float* f, f32x4 (*to)[TM]) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint4 xv[TM];
@@ -583,39 +693,54 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
 #pragma unroll
                         for (int n = 0; n < TN; ++n) {
                             const uint32_t word[4] = { q[n].x, q[n].y, q[n].z, q[n].w };
-                            const uint4 wv = to_bf16(word[j], f[n]);
+                            const uint4 wv = widen<XT>(word[j], f[n]);
 #pragma unroll
-                            for (int m = 0; m < TM; ++m) acc[n][m] = mma<BF16>(wv, xv[m], acc[n][m]);
+                            for (int m = 0; m < TM; ++m) to[n][m] = mma<XT>(wv, xv[m], to[n][m]);
                         }
                     }
+                };
+                float f[TN];
+                if constexpr (XT == BF16) {
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) f[n] = scale_arg(byte[n]);
+                    pass(f, acc);
                 } else {
-                    // D's rows are the weights': lane group g's are 4 g + r, whose scale words are 16 bytes in LDS
-                    uint4 sw[TN];
+                    // The rows of D are the weights': lane group g's are 4 g + r, whose scale words are 16 bytes in LDS. Each row's level
+                    // follows from its word alone, so that the lanes that convert a row and those that hold its sums agree on it.
+                    int at[TN], sums_at[TN][4];
+                    bool more = true;
 #pragma unroll
                     for (int n = 0; n < TN; ++n) {
-                        q[n] = exchange(q[n]);
-                        sw[n] = *(const uint4*)(WS + (wr - l16 + 16 * n + 4 * g) * 4);
+                        at[n] = 256 + LEVEL;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sums_at[n][r] = 256 + LEVEL;
                     }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint4 xv[TM];
-#pragma unroll
-                        for (int m = 0; m < TM; ++m) xv[m] = x_at(m, 4 * j + g);
+                    while (more) {
+                        f32x4 p[TN][TM] = {};
+                        more = false;
 #pragma unroll
                         for (int n = 0; n < TN; ++n) {
-                            const uint32_t word[4] = { q[n].x, q[n].y, q[n].z, q[n].w };
-                            const uint32_t sc[4] = { sw[n].x, sw[n].y, sw[n].z, sw[n].w };
-                            float f[4];
+                            const int below = at[n] - LEVEL;
+                            at[n] = top_byte_below(*(const uint32_t*)(WS + (wr + 16 * n) * 4) & live, below);
+                            f[n] = at[n] < 0 ? 0.f : pass_scale(byte[n], at[n], below);
+                            more |= byte[n] < at[n] - LEVEL && any_code(q[n]);
+                            if (at[n] < 0) at[n] = -1000;
+                        }
+                        pass(f, p);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) f[r] = scale_f32(((sc[r] & live) >> (8 * j)) & 255);
-                            const uint4 wv = to_f16(word[j]);
+                        for (int n = 0; n < TN; ++n) {
+                            const uint4 w = *(const uint4*)(WS + (wr - l16 + 16 * n + 4 * g) * 4);
+                            const uint32_t sc[4] = { w.x, w.y, w.z, w.w };
 #pragma unroll
-                            for (int m = 0; m < TM; ++m) {
-                                const f32x4 p = mma<F16>(wv, xv[m], f32x4{ 0, 0, 0, 0 });
+                            for (int r = 0; r < 4; ++r) {
+                                const int l = top_byte_below(sc[r] & live, sums_at[n][r] - LEVEL);
+                                const float s = l < 0 ? 0.f : scale_f32(l);
+                                sums_at[n][r] = l < 0 ? -1000 : l;
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) acc[n][m][r] = __builtin_fmaf(p[r], f[r], acc[n][m][r]);
+                                for (int m = 0; m < TM; ++m) acc[n][m][r] = __builtin_fmaf(p[n][m][r], s, acc[n][m][r]);
                             }
                         }
+                        more = __any(more);
                     }
                 }
             }
@@ -661,6 +786,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
 
 int launched() { return hipGetLastError() == hipSuccess ? 0 : EXL3C4_E_DEVICE; }
 
+#ifndef WIDE_NS
+#define WIDE_NS 4
+#endif
+#ifndef WIDE_AHEAD
+#define WIDE_AHEAD 2
+#endif
+#ifndef NARROW_AHEAD
+#define NARROW_AHEAD 2
+#endif
+#ifndef WIDE_MIN
+#define WIDE_MIN 1024
+#endif
 #ifndef ROWS_MAX
 #define ROWS_MAX 8
 #endif
@@ -673,12 +810,13 @@ int64_t chunk_bound(const Exl3c4DevGemm& a, int rows) {
     return a.T / rows + (seg < a.T ? seg : a.T);
 }
 
-template <int XT, int WT, bool SW>
+template <int XT, int WT, bool SW, int NS, int WV, int AHEAD>
 int launch_rows(Exl3c4DevGemm& a, hipStream_t st) {
-    a.tiles = (a.n_out + (SW ? 15 : 31)) / (SW ? 16 : 32);
-    const int64_t grid = (chunk_bound(a, 1 << ROWS_LOG2) * a.tiles + 7) / 8 * 8;
+    constexpr int cols = 16 * (SW ? NS / 2 : NS);
+    a.tiles = (a.n_out + cols - 1) / cols;
+    const int64_t grid = chunk_bound(a, 1 << ROWS_LOG2) * a.tiles;
     if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
-    hipLaunchKernelGGL((k_mg_rows<XT, WT, SW>), dim3((unsigned)grid), dim3(64 * WAVES), 0, st, a);
+    hipLaunchKernelGGL((k_mg_rows<XT, WT, SW, NS, WV, AHEAD>), dim3((unsigned)grid), dim3(64 * WV), 0, st, a);
     return launched();
 }
 
@@ -692,15 +830,27 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     return launched();
 }
 
+#ifndef T64_BUFS
+#define T64_BUFS 2
+#endif
+#ifndef BIG
+#define BIG 8, 256, 2, 4, 2
+#endif
 template <int XT, int WT, bool SW>
 int launch(Exl3c4DevGemm& a, hipStream_t st) {
     const int64_t T = a.T, live = a.n_expert < T ? a.n_expert : T;
-    if (T <= ROWS_MAX * live) return launch_rows<XT, WT, SW>(a, st);
-    if constexpr (WT == MX4 && XT != MX4) {
-        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
+    constexpr bool mixed = WT == MX4 && XT != MX4;
+    if (T <= ROWS_MAX * live) {
+        constexpr int cols = SW ? 8 * WIDE_NS : 16 * WIDE_NS;
+        if (chunk_bound(a, 1 << ROWS_LOG2) * ((a.n_out + cols - 1) / cols) >= WIDE_MIN)
+            return launch_rows<XT, WT, SW, WIDE_NS, 4, WIDE_AHEAD>(a, st);
+        return launch_rows<XT, WT, SW, 2, 4, NARROW_AHEAD>(a, st);
+    }
+    if constexpr (mixed) {
+        return launch_tile<XT, WT, SW, 6, 128, 1, 4, T64_BUFS>(a, st);
     } else {
-        if (T <= TILE_MAX * live) return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
-        return launch_tile<XT, WT, SW, 8, 256, 2, 4, 2>(a, st);
+        if (T <= TILE_MAX * live) return launch_tile<XT, WT, SW, 6, 128, 1, 4, T64_BUFS>(a, st);
+        return launch_tile<XT, WT, SW, BIG>(a, st);
     }
 }
 

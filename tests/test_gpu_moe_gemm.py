@@ -176,14 +176,21 @@ def test_pointer_tables_give_the_stacked_buffers_bits(ex, pair):
 
 @pytest.mark.parametrize("pair", [p for p in PAIRS if p[1] == "mx4"], ids="-".join)
 @pytest.mark.parametrize("tokens", [3, 150])
-def test_extreme_scales(ex, pair, tokens):
-    """Scales over the format's whole range: a row's blocks from 2^-120 to 2^20, where f16 could not hold the weights; and a
-    NaN block, which makes its own rows' outputs NaN and no others."""
+@pytest.mark.parametrize("K", [256, 2304])
+def test_extreme_scales(ex, pair, tokens, K):
+    """Scales over the format's whole range: a row's blocks from 2^-120 to 2^20, where f16 could not hold the weights; x zero
+    where the largest are, so that the small ones make the sums; and a NaN block, which makes its own rows' outputs
+    NaN and no others."""
     g = torch.Generator().manual_seed(3)
-    K, N, E = 256, 40, 2
-    w = torch.randn((E, N, K // 32, 32), generator=g) * torch.exp2(torch.randint(-118, 18, (E, N, K // 32, 1), generator=g).float())
-    w = w.reshape(E, N, K)
+    N, E = 40, 2
+    e = torch.randint(-118, 18, (E, N, K // 32, 1), generator=g)
+    e[:, :, 1::2] = torch.randint(-118, -30, (E, N, K // 32, 1), generator=g)[:, :, 1::2]
+    e[:, ::3] = torch.randint(-3, 4, (E, N, K // 32, 1), generator=g)[:, ::3]
+    w = (torch.randn((E, N, K // 32, 32), generator=g) * torch.exp2(e.float())).reshape(E, N, K)
     check(ex, pair, "f32", False, tokens, 1, E, N, K, w=w)
+    x = torch.randn((tokens, K // 64, 2, 32), generator=g)
+    x[:, :, 0] = 0
+    check(ex, pair, "f32", False, tokens, 1, E, N, K, w=w, x=x.reshape(tokens, K))
     w[1, 7, 40] = float("nan")
     check(ex, pair, "f32", False, tokens, 1, E, N, K, w=w, seed=4)
 

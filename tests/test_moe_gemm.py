@@ -43,7 +43,7 @@ def rc(g):
     ({"x_rows": 0}, SHAPE), ({"x_rows": 15, "sorted_tok": None}, SHAPE), ({"T": 1 << 31}, SHAPE), ({"K": 1 << 32}, SHAPE),
     ({"act": 1, "N": 47, "w_stride": 1 << 20}, SHAPE),
     ({"x_pitch": 56}, STRIDE), ({"w_pitch": 56}, STRIDE), ({"w_stride": 47 * 128}, STRIDE), ({"w_stride": -16}, STRIDE), ({"y_pitch": 47}, STRIDE),
-    ({"x_pitch": -64}, STRIDE), ({"x_pitch": 1 << 62}, STRIDE),
+    ({"w_pitch": (1 << 26) + 8, "w_stride": 1 << 34}, STRIDE), ({"x_pitch": -64}, STRIDE), ({"x_pitch": 1 << 62}, STRIDE),
     ({"x": P + 8}, ALIGN), ({"w": P + 2}, ALIGN), ({"x_pitch": 68}, ALIGN), ({"w_pitch": 68, "w_stride": 1 << 20}, ALIGN),
     ({"w_stride": 48 * 128 + 8}, ALIGN), ({"y": P + 1}, ALIGN), ({"y_type": 2, "y": P + 2}, ALIGN), ({"sorted_tok": P + 2}, ALIGN),
     ({"expert_offset": P + 1}, ALIGN),
