@@ -169,6 +169,7 @@ typedef struct Exl3c4DevGemm {
     int32_t        n_out;          /* y's columns: N, or N / 2 with SwiGLU */
     int32_t        y_type;
     int32_t        tiles;          /* column tiles of y */
+    int32_t        grid;           /* workgroups, where they take several units each */
 } Exl3c4DevGemm;
 int exl3c4_dev_gemm(const Exl3c4DevGemm* g, int32_t x_type, int32_t w_type, int32_t act, void* stream);
 int exl3c4_dev_mx4_quant(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t pitch, uint8_t* codes,

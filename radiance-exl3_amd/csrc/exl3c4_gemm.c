@@ -121,6 +121,6 @@ int exl3c4_moe_gemm(const Exl3c4Gemm* g, void* stream) {
     d.K = (int32_t)g->K;
     d.n_out = (int32_t)n_out;
     d.y_type = g->y_type;
-    d.tiles = 0;
+    d.tiles = d.grid = 0;                                     /* the launcher's */
     return exl3c4_dev_gemm(&d, g->x_type, g->w_type, g->act, stream);
 }

@@ -95,9 +95,8 @@ template <int MT_LOG2> struct Runs {
 // experts', then those of the rows before the first run and behind the last one -- each with its column tiles in turn. One wave of the workgroup
 // finds its unit from the offsets (one read and one scan for 512 experts), so a launch needs no plan before it.
 // XCD: the units are cut into eight ranges, one an XCD (workgroups go to the XCDs in turn), whose L2 then holds a chunk's rows for all its
-// tiles and an expert's weights for all its chunks. Else neighbouring units go to different XCDs, which read one stretch
-// of weights together: faster where each weight is read about once (512 experts of about 12 rows in bf16: 579 us against 597; of 40 in MX4 154
-// against 174).
+// tiles and an expert's weights for all its chunks (bf16, 400 tokens of top-10 over 512 experts: 437 us in plain order, 362 so). The rows
+// kernel reads every weight once and its few rows of x from anywhere: the same either way, and plain.
 template <int MT_LOG2, bool XCD>
 __device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
     typedef Runs<MT_LOG2> R;
@@ -269,6 +268,7 @@ __device__ __forceinline__ bool any_code(const uint4& q) { return ((q.x | q.y | 
 // rows), each wave a part of k; the weights go from memory straight to the matrix units' operands, each byte read
 // once, and the parts' sums meet in LDS in a fixed order.
 constexpr int ROWS_LOG2 = 4;
+constexpr int WAVES = 4;
 
 // What one matrix step reads of the NS weight strips and of x, and its products. FULL: every lane's bytes are inside
 // the rows; else what lies past K reads as zeros (and their scales as 2^-127, never as a NaN).
@@ -329,8 +329,9 @@ template <int XT, int WT, int NS> struct Step {
     }
 };
 
-template <int XT, int WT, bool SW, int NS, int WV, int AHEAD>
-__global__ __launch_bounds__(64 * WV) void k_mg_rows(Exl3c4DevGemm a) {
+template <int XT, int WT, bool SW, int NS>
+__global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
+    constexpr int WV = WAVES, AHEAD = 2;                         // steps whose loads are out together
     typedef Step<XT, WT, NS> S;
     constexpr int OUT = SW ? NS / 2 : NS;                        // strips of y
     __shared__ f32x4 part[WV][NS][64];
@@ -544,7 +545,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
-    const Chunk ch = my_unit<MT_LOG2, (MT_LOG2 >= 7)>(a, lane, wave);
+    const Chunk ch = my_unit<MT_LOG2, true>(a, lane, wave);
     if (ch.rows == 0) return;
     const int n0 = ch.tile * (SW ? NT / 2 : NT);                    // the tile's first column of y
     // row r of the tile -> a row of the weight (past the last one: it again, not stored)
@@ -708,15 +709,31 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                     // The rows of D are the weights': lane group g's are 4 g + r, whose scale words are 16 bytes in LDS. Each row's level
                     // follows from its word alone, so that the lanes that convert a row and those that hold its sums agree on it.
                     int at[TN], sums_at[TN][4];
-                    bool more = true;
+                    bool more = false;
+                    f32x4 p[TN][TM] = {};
+                    auto add = [&](int n, int r, int level) {    // the pass's sums of row r, scaled
+                        const float f = level < 0 ? 0.f : scale_f32(level);
+                        sums_at[n][r] = level;
+#pragma unroll
+                        for (int m = 0; m < TM; ++m) acc[n][m][r] = __builtin_fmaf(p[n][m][r], f, acc[n][m][r]);
+                    };
+                    uint4 words[TN];
 #pragma unroll
                     for (int n = 0; n < TN; ++n) {
-                        at[n] = 256 + LEVEL;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) sums_at[n][r] = 256 + LEVEL;
+                        at[n] = top_byte(*(const uint32_t*)(WS + (wr + 16 * n) * 4) & live);
+                        f[n] = pass_scale(byte[n], at[n], 256);
+                        more |= byte[n] < at[n] - LEVEL && any_code(q[n]);
+                        words[n] = *(const uint4*)(WS + (wr - l16 + 16 * n + 4 * g) * 4);
                     }
-                    while (more) {
-                        f32x4 p[TN][TM] = {};
+                    pass(f, p);
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) {
+                        add(n, 0, top_byte(words[n].x & live));
+                        add(n, 1, top_byte(words[n].y & live));
+                        add(n, 2, top_byte(words[n].z & live));
+                        add(n, 3, top_byte(words[n].w & live));
+                    }
+                    while (__any(more)) {
                         more = false;
 #pragma unroll
                         for (int n = 0; n < TN; ++n) {
@@ -724,23 +741,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                             at[n] = top_byte_below(*(const uint32_t*)(WS + (wr + 16 * n) * 4) & live, below);
                             f[n] = at[n] < 0 ? 0.f : pass_scale(byte[n], at[n], below);
                             more |= byte[n] < at[n] - LEVEL && any_code(q[n]);
-                            if (at[n] < 0) at[n] = -1000;
+#pragma unroll
+                            for (int m = 0; m < TM; ++m) p[n][m] = f32x4{ 0, 0, 0, 0 };
                         }
                         pass(f, p);
 #pragma unroll
                         for (int n = 0; n < TN; ++n) {
-                            const uint4 w = *(const uint4*)(WS + (wr - l16 + 16 * n + 4 * g) * 4);
-                            const uint32_t sc[4] = { w.x, w.y, w.z, w.w };
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const int l = top_byte_below(sc[r] & live, sums_at[n][r] - LEVEL);
-                                const float s = l < 0 ? 0.f : scale_f32(l);
-                                sums_at[n][r] = l < 0 ? -1000 : l;
-#pragma unroll
-                                for (int m = 0; m < TM; ++m) acc[n][m][r] = __builtin_fmaf(p[n][m][r], s, acc[n][m][r]);
-                            }
+                            add(n, 0, top_byte_below(words[n].x & live, sums_at[n][0] - LEVEL));
+                            add(n, 1, top_byte_below(words[n].y & live, sums_at[n][1] - LEVEL));
+                            add(n, 2, top_byte_below(words[n].z & live, sums_at[n][2] - LEVEL));
+                            add(n, 3, top_byte_below(words[n].w & live, sums_at[n][3] - LEVEL));
                         }
-                        more = __any(more);
                     }
                 }
             }
@@ -761,62 +772,52 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
             buf = buf + 1 == BUFS ? 0 : buf + 1;
         }
     }
-    // lane: row 16 m + l16 of the wave's rows, columns 16 n + 4 g .. + 3 (SwiGLU: of gate tile 2 n and up tile 2 n + 1)
+    // A lane holds columns 16 n + 4 g .. + 3 of row 16 m + l16 of the wave's (SwiGLU: of gate tile 2 n and up tile 2 n + 1). 16 rows at a
+    // time cross LDS, in the wave's own part of it, so that a row's columns go out together -- and so that what differs by type
+    // and edge is code for one store and not for all of a lane's (unrolled over 32 tiles it took 12 us to fetch).
+    constexpr int TO = SW ? TN / 2 : TN, LANES = 4 * TO, PITCH = 16 * TO + 4;
+    static_assert(WV * 16 * PITCH * 4 <= (int)sizeof(lds), "the rows fit the stages' buffers");
+    __syncthreads();
+    float* rows = (float*)lds + wave * (16 * PITCH);
     const int ysz = a.y_type == EXL3C4_F32 ? 4 : 2;
     const bool whole = ((uintptr_t)a.y | (uintptr_t)a.y_pitch) % (4 * ysz) == 0;      // four columns are one aligned store
+    const int col = n0 + wn * TO * 16 + 4 * (lane % LANES);
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
-        const int r = (wm * TM + m) * 16 + l16;
-        if (r >= ch.rows) continue;
-        const bool alive = rows_x[r] >= 0;
-        char* y = a.y + (int64_t)(ch.row0 + r) * a.y_pitch;
 #pragma unroll
-        for (int n = 0; n < (SW ? TN / 2 : TN); ++n) {
-            const int col = n0 + (wn * (SW ? TN / 2 : TN) + n) * 16 + 4 * g;
+        for (int n = 0; n < TO; ++n) {
             f32x4 v = SW ? acc[2 * n][m] : acc[n][m];
+            if (SW)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (SW) v[i] = swiglu(v[i], acc[(SW ? 2 * n + 1 : n)][m][i]);
-                if (!alive) v[i] = 0.f;
-            }
-            store4(y + (int64_t)col * ysz, a.y_type, v, a.n_out - col, whole);
+                for (int i = 0; i < 4; ++i) v[i] = swiglu(v[i], acc[SW ? 2 * n + 1 : n][m][i]);
+            *(f32x4*)(rows + l16 * PITCH + 16 * n + 4 * g) = v;
+        }
+#pragma unroll 1
+        for (int i = 0; i < TO; ++i) {
+            const int q = i * (64 / LANES) + lane / LANES, r = (wm * TM + m) * 16 + q;
+            f32x4 v = *(const f32x4*)(rows + q * PITCH + 4 * (lane % LANES));
+            if (r >= ch.rows) continue;
+            if (rows_x[r] < 0) v = f32x4{ 0, 0, 0, 0 };
+            store4(a.y + (int64_t)(ch.row0 + r) * a.y_pitch + (int64_t)col * ysz, a.y_type, v, a.n_out - col, whole);
         }
     }
 }
 
 int launched() { return hipGetLastError() == hipSuccess ? 0 : EXL3C4_E_DEVICE; }
 
-#ifndef WIDE_NS
-#define WIDE_NS 4
-#endif
-#ifndef WIDE_AHEAD
-#define WIDE_AHEAD 2
-#endif
-#ifndef NARROW_AHEAD
-#define NARROW_AHEAD 2
-#endif
-#ifndef WIDE_MIN
-#define WIDE_MIN 1024
-#endif
-#ifndef ROWS_MAX
-#define ROWS_MAX 8
-#endif
-#ifndef TILE_MAX
-#define TILE_MAX 128
-#endif
 // Chunks of at most `rows` that the launch's segments (the runs, and the rows before and behind them) can make.
 int64_t chunk_bound(const Exl3c4DevGemm& a, int rows) {
     const int64_t seg = (int64_t)a.n_expert + 2;
     return a.T / rows + (seg < a.T ? seg : a.T);
 }
 
-template <int XT, int WT, bool SW, int NS, int WV, int AHEAD>
+template <int XT, int WT, bool SW, int NS>
 int launch_rows(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr int cols = 16 * (SW ? NS / 2 : NS);
     a.tiles = (a.n_out + cols - 1) / cols;
     const int64_t grid = chunk_bound(a, 1 << ROWS_LOG2) * a.tiles;
     if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
-    hipLaunchKernelGGL((k_mg_rows<XT, WT, SW, NS, WV, AHEAD>), dim3((unsigned)grid), dim3(64 * WV), 0, st, a);
+    hipLaunchKernelGGL((k_mg_rows<XT, WT, SW, NS>), dim3((unsigned)grid), dim3(64 * WAVES), 0, st, a);
     return launched();
 }
 
@@ -830,27 +831,41 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     return launched();
 }
 
-#ifndef T64_BUFS
-#define T64_BUFS 2
-#endif
-#ifndef BIG
-#define BIG 8, 256, 2, 4, 2
-#endif
+// Which kernel, and how large a tile: by the types, the sizes and the rows that an expert has at least on average, r = T / min(E, T)
+// -- never by the routing, which is on the device. Larger tiles read weights and rows less often; smaller ones waste
+// less of a chunk, make more workgroups and start sooner. Measured, us (E / top-k, N x K, tokens; SwiGLU where E > 1):
+//   rows against tiles     bf16 512/10 1024x2048: 32 tokens 179 / 248, 64 261 / 249, 200 373 / 338. MX4 64: 89 / 79, 200: 125 / 105.
+//                          bf16 x, MX4 w 64: 85 / 98, 200 118 / 133; 64/6 at 400 49 / 24. One expert, 77 rows 512x2048: 9.1 / 16.
+//   32 rows against 64     8/2 at 400 tokens: bf16 17.5 / 20.0, MX4 12.1 / 14.6; MX4 512/10 at 200 105 / 117, at 2048 Zipf 171 / 152.
+//   64 against 128         bf16 512/10 at 4096 522 / 409, 64/6 at 2000 113 / 95; MX4 193 / 175, 46 / 41; bf16 x, MX4 w 339 / 379.
+//   128 against 256        bf16 64/6 at 2000 95 / 85, 8/2 2816x2048 at 8192 225 / 190; MX4 64/6 at 2000 41 / 33, but K = 1408 at
+//                          8192 76 / 82 (few stages, and the larger tile's start and stores stand alone on its CU).
 template <int XT, int WT, bool SW>
 int launch(Exl3c4DevGemm& a, hipStream_t st) {
-    const int64_t T = a.T, live = a.n_expert < T ? a.n_expert : T;
     constexpr bool mixed = WT == MX4 && XT != MX4;
-    if (T <= ROWS_MAX * live) {
-        constexpr int cols = SW ? 8 * WIDE_NS : 16 * WIDE_NS;
-        if (chunk_bound(a, 1 << ROWS_LOG2) * ((a.n_out + cols - 1) / cols) >= WIDE_MIN)
-            return launch_rows<XT, WT, SW, WIDE_NS, 4, WIDE_AHEAD>(a, st);
-        return launch_rows<XT, WT, SW, 2, 4, NARROW_AHEAD>(a, st);
+    const int64_t T = a.T, live = a.n_expert < T ? a.n_expert : T;
+    // workgroups of tiles of `rows` x `cols` (SwiGLU: half as many columns of y)
+    auto units = [&](int rows, int cols) {
+        if (SW) cols /= 2;
+        return chunk_bound(a, rows) * ((a.n_out + cols - 1) / cols);
+    };
+    if (T <= (mixed ? 8 : 1) * live || units(32, 128) < 64 || (T <= 4 * live && units(32, 128) < 256)) {
+        if (units(16, 64) >= 1024) return launch_rows<XT, WT, SW, 4>(a, st);
+        return launch_rows<XT, WT, SW, 2>(a, st);
     }
     if constexpr (mixed) {
-        return launch_tile<XT, WT, SW, 6, 128, 1, 4, T64_BUFS>(a, st);
+        if (units(64, 128) < 256) return launch_tile<XT, WT, SW, 5, 128, 1, 4, 3>(a, st);
+        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
+    } else if constexpr (WT == MX4) {
+        if (T > 160 * live && units(256, 256) >= 256 && a.K >= 2048) return launch_tile<XT, WT, SW, 8, 256, 2, 4, 2>(a, st);
+        if (T > 64 * live && units(128, 128) >= 256) return launch_tile<XT, WT, SW, 7, 128, 2, 2, 2>(a, st);
+        if (T <= 16 * live || units(64, 128) < 256) return launch_tile<XT, WT, SW, 5, 128, 1, 4, 3>(a, st);
+        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
     } else {
-        if (T <= TILE_MAX * live) return launch_tile<XT, WT, SW, 6, 128, 1, 4, T64_BUFS>(a, st);
-        return launch_tile<XT, WT, SW, BIG>(a, st);
+        if (T > 160 * live && units(256, 256) >= 256) return launch_tile<XT, WT, SW, 8, 256, 2, 4, 2>(a, st);
+        if (T > 64 * live && units(128, 128) >= 256) return launch_tile<XT, WT, SW, 7, 128, 2, 4, 2>(a, st);
+        if (units(64, 128) < 256) return launch_tile<XT, WT, SW, 5, 128, 1, 4, 3>(a, st);
+        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 3>(a, st);
     }
 }
 

@@ -45,18 +45,19 @@ def gemm(x, w, sorted_tok, offset, T, top_k, swiglu):
     y, tol = torch.zeros(T, n_out, dtype=torch.float64), torch.zeros(T, n_out, dtype=torch.float64)
     off = [min(max(int(o), 0), T) for o in offset]
     for e in range(E):
-        for i in range(off[e], off[e + 1]):
-            r = i if sorted_tok is None else int(sorted_tok[i]) // top_k if int(sorted_tok[i]) >= 0 else -1
-            if r < 0 or r >= x.shape[0]:
-                continue
-            p = w[e] @ x[r]
-            t = K * 2.0 ** -23 * (w[e].abs() @ x[r].abs())
-            if swiglu:
-                g, u, tg, tu = p[:n_out], p[n_out:], t[:n_out], t[n_out:]
-                s = torch.nn.functional.silu(g)
-                p = s * u
-                t = 1.1 * tg * (u.abs() + tu) + s.abs() * tu + (8 + g.abs()) * 2.0 ** -24 * p.abs()
-            y[i], tol[i] = p, t
+        i = torch.arange(off[e], max(off[e], off[e + 1]))
+        st = i * top_k if sorted_tok is None else torch.as_tensor(sorted_tok)[i].long()
+        r = torch.div(st, top_k, rounding_mode="floor")
+        ok = (st >= 0) & (r < x.shape[0])
+        i, r = i[ok], r[ok]
+        p = x[r] @ w[e].T
+        t = K * 2.0 ** -23 * (x[r].abs() @ w[e].abs().T)
+        if swiglu:
+            g, u, tg, tu = p[:, :n_out], p[:, n_out:], t[:, :n_out], t[:, n_out:]
+            s = torch.nn.functional.silu(g)
+            p = s * u
+            t = 1.1 * tg * (u.abs() + tu) + s.abs() * tu + (8 + g.abs()) * 2.0 ** -24 * p.abs()
+        y[i], tol[i] = p, t
     return y, tol
 
 

@@ -88,6 +88,41 @@ def test_products(ex, pair, tokens, top_k, E, N, K):
     check(ex, pair, "f32", False, tokens, top_k, E, N - 1, K, gather=False, seed=1)
 
 
+# (T, E, N) that take each kernel and tile: few rows an expert in narrow and wide workgroups, 32, 64, 128 and 256 rows a tile
+PATHS = {"rows": (40, 3, 200), "rows wide": (60, 4, 11000), "32": (150, 2, 1450), "64": (250, 4, 3700), "128": (260, 2, 5510), "256": (700, 2, 13320)}
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("path", list(PATHS))
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_each_tile(ex, pair, path, swiglu):
+    """Sizes that take each kernel and tile, their last tiles partly past the rows and columns, k ending inside a stage (MX4's
+    largest tile is taken from K = 2048 on)."""
+    T, E, N = PATHS[path]
+    K = 2080 if path == "256" and pair[0] == "mx4" else 160 if pair[1] == "mx4" else 136
+    N *= 2 if swiglu else 1
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn((T, K), generator=g)
+    if pair[1] == "mx4":                                            # random codes at once: rounding so many is slow here
+        codes = torch.randint(0, 256, (E, N, K // 2), dtype=torch.uint8, generator=g)
+        scales = torch.randint(118, 122, (E, N, (K // 32 + 3) // 4 * 4), dtype=torch.uint8, generator=g)
+        scales[..., K // 32:] = 255
+        w = ex.Mx4(codes.cuda(), scales.cuda(), K), mx4ref.dequant(codes, scales, K)
+    else:
+        w = operand(ex, torch.randn((E, N, K), generator=g) / K ** 0.5, pair[1])
+    xd, xv = operand(ex, x, pair[0])
+    off = torch.tensor([0] + [T * (e + 1) // E - (e == 0) for e in range(E)], dtype=torch.int32)
+    off[-1] = T - 2
+    st = torch.randperm(T, generator=g).to(torch.int32)
+    n_out = N // 2 if swiglu else N
+    y = torch.full((T + 1, n_out + 3), float("nan"), dtype=torch.float32, device="cuda")
+    assert ex.moe_gemm(ex.make_gemm(xd, w[0], st.cuda(), off.cuda(), y[:T, :n_out], act=ex.ACT_SWIGLU if swiglu else ex.ACT_NONE)) == 0
+    torch.cuda.synchronize()
+    want, tol = mx4ref.gemm(xv, w[1], st, off, T, 1, swiglu)
+    assert mx4ref.close(y[:T, :n_out].cpu(), want, tol)
+    assert torch.isnan(y[T]).all() and torch.isnan(y[:, n_out:]).all()
+
+
 @pytest.mark.parametrize("pair", [("f16", "f16"), ("bf16", "bf16")], ids="-".join)
 @pytest.mark.parametrize("K", [8, 24, 40, 72, 1000, 1544])
 def test_columns_that_end_inside_a_step(ex, pair, K):
