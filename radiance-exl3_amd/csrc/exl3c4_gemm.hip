@@ -261,6 +261,15 @@ constexpr int LEVEL = 13;                                       // e2m1 x 2^-13 
 __device__ __forceinline__ float pass_scale(int byte, int level, int below) {
     return byte >= level - LEVEL && byte < below ? __uint_as_float((uint32_t)(byte - level + 127) << 23) : 0.f;
 }
+// The level of a word's pass k, and what it is below.
+__device__ __forceinline__ int level_of(uint32_t w, int k, int& below) {
+    int l = top_byte(w);
+    for (int i = 0; i < k; ++i) {                                // (k is uniform)
+        below = l < 0 ? -1 : l - LEVEL;
+        l = top_byte_below(w, below);
+    }
+    return l;
+}
 __device__ __forceinline__ bool any_code(const uint4& q) { return ((q.x | q.y | q.z | q.w) & 0x77777777u) != 0; }
 
 // ------------------------------------------------------------------------------------------ few rows an expert
@@ -708,51 +717,35 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                 } else {
                     // The rows of D are the weights': lane group g's are 4 g + r, whose scale words are 16 bytes in LDS. Each row's level
                     // follows from its word alone, so that the lanes that convert a row and those that hold its sums agree on it.
-                    int at[TN], sums_at[TN][4];
-                    bool more = false;
-                    f32x4 p[TN][TM] = {};
-                    auto add = [&](int n, int r, int level) {    // the pass's sums of row r, scaled
-                        const float f = level < 0 ? 0.f : scale_f32(level);
-                        sums_at[n][r] = level;
-#pragma unroll
-                        for (int m = 0; m < TM; ++m) acc[n][m][r] = __builtin_fmaf(p[n][m][r], f, acc[n][m][r]);
-                    };
-                    uint4 words[TN];
-#pragma unroll
-                    for (int n = 0; n < TN; ++n) {
-                        at[n] = top_byte(*(const uint32_t*)(WS + (wr + 16 * n) * 4) & live);
-                        f[n] = pass_scale(byte[n], at[n], 256);
-                        more |= byte[n] < at[n] - LEVEL && any_code(q[n]);
-                        words[n] = *(const uint4*)(WS + (wr - l16 + 16 * n + 4 * g) * 4);
-                    }
-                    pass(f, p);
-#pragma unroll
-                    for (int n = 0; n < TN; ++n) {
-                        add(n, 0, top_byte(words[n].x & live));
-                        add(n, 1, top_byte(words[n].y & live));
-                        add(n, 2, top_byte(words[n].z & live));
-                        add(n, 3, top_byte(words[n].w & live));
-                    }
-                    while (__any(more)) {
+                    // (Everything but the sums is read again in the rare passes behind the first, for registers.)
+                    bool more;
+                    auto level_pass = [&](int k) {
+                        f32x4 p[TN][TM] = {};
                         more = false;
 #pragma unroll
                         for (int n = 0; n < TN; ++n) {
-                            const int below = at[n] - LEVEL;
-                            at[n] = top_byte_below(*(const uint32_t*)(WS + (wr + 16 * n) * 4) & live, below);
-                            f[n] = at[n] < 0 ? 0.f : pass_scale(byte[n], at[n], below);
-                            more |= byte[n] < at[n] - LEVEL && any_code(q[n]);
-#pragma unroll
-                            for (int m = 0; m < TM; ++m) p[n][m] = f32x4{ 0, 0, 0, 0 };
+                            int below = 256;
+                            const int l = level_of(*(const uint32_t*)(WS + (wr + 16 * n) * 4) & live, k, below);
+                            f[n] = l < 0 ? 0.f : pass_scale(byte[n], l, below);
+                            more |= byte[n] < l - LEVEL && any_code(q[n]);
                         }
                         pass(f, p);
 #pragma unroll
                         for (int n = 0; n < TN; ++n) {
-                            add(n, 0, top_byte_below(words[n].x & live, sums_at[n][0] - LEVEL));
-                            add(n, 1, top_byte_below(words[n].y & live, sums_at[n][1] - LEVEL));
-                            add(n, 2, top_byte_below(words[n].z & live, sums_at[n][2] - LEVEL));
-                            add(n, 3, top_byte_below(words[n].w & live, sums_at[n][3] - LEVEL));
+                            const uint4 w = *(const uint4*)(WS + (wr - l16 + 16 * n + 4 * g) * 4);
+                            const uint32_t word[4] = { w.x, w.y, w.z, w.w };
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                int below = 256;
+                                const int l = level_of(word[r] & live, k, below);
+                                const float s = l < 0 ? 0.f : scale_f32(l);
+#pragma unroll
+                                for (int m = 0; m < TM; ++m) acc[n][m][r] = __builtin_fmaf(p[n][m][r], s, acc[n][m][r]);
+                            }
                         }
-                    }
+                    };
+                    level_pass(0);
+                    for (int k = 1; __any(more); ++k) level_pass(k);
                 }
             }
         };
