@@ -127,7 +127,7 @@ __device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
     } else if (a.n_expert <= 512) {
         s.find(0, lane, c, out);
     } else {
-        for (int base = 0;; base += 512) {
+        for (int base = 0; base < a.n_expert; base += 512) {
             s.read(a, base, lane);
             if (c < s.total()) {
                 s.find(base, lane, c, out);
@@ -136,6 +136,7 @@ __device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
             c -= s.total();
         }
     }
+    out.rows = max(out.rows, 0);                                 // (a table that is no routing: more chunks than 32 bits count)
     return out;
 }
 // The same for the whole workgroup, by its first wave.
@@ -166,6 +167,10 @@ typedef const __attribute__((address_space(1))) char* gaddr;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint4 load16(gaddr p) {
     return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)p);
+}
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));            // scale rows start at any word
+__device__ __forceinline__ uint4 load_words(gaddr p) {
+    return __builtin_bit_cast(uint4, (u32x4)*(const __attribute__((address_space(1))) u32x4_at4*)p);
 }
 __device__ __forceinline__ uint32_t load4(gaddr p) { return *(const __attribute__((address_space(1))) uint32_t*)p; }
 __device__ __forceinline__ gaddr entry(const void* base, int64_t stride, int e) {
@@ -420,7 +425,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
             bool more = false;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
-                if constexpr (WT == MX4) sc[s] = load16(ws[s] + (s_at + 4u * (uint32_t)t));
+                if constexpr (WT == MX4) sc[s] = load_words(ws[s] + (s_at + 4u * (uint32_t)t));
 #pragma unroll
             for (int h = 0; h < 4; h += AHEAD) {
                 S st[AHEAD];
@@ -510,7 +515,16 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 // source: the chunk at place p of row r is p ^ (r & 7) (of 64-byte rows p ^ ((r >> 1) & 3)), and the 16 rows that a matrix
 // operand reads at one column fall on all the banks evenly.
 //
-// Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, one store.
+// Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y.
+//
+// What bounds it, measured. Where experts have up to some 60 rows, memory: bf16, 200 and 400 tokens of top-10 over 512 experts 5.9 to 6.1 TB/s
+// of weights, the card's reading rate. Beyond, the stages' latency: a CU takes about 88 bytes a ns from its L2, and with
+// 256 x 256 tiles two stages (128 KB) are all that LDS holds, so that a stage's loads (64 KB, 0.74 us) and its products (1.05 us at 2.05
+// PFLOP/s) only partly cover each other: 8192 tokens over 8 experts bf16 at 1.0 PFLOP/s, where a plain library product of 8192^3
+// reaches 1.44. Tried without gain: the next step's operands read ahead into registers (188 -> 185 us bf16, MX4 spilled), loads spread between
+// the products (188 -> 198), four stages of half the columns (64-byte rows fetch each line twice: 188 -> 204), one workgroup
+// a CU taking unit after unit with the next one's loads under the last one's stores (188 -> 199), weights asked for before the rows of x
+// are known (the same), scales in 16-byte loads (MX4 4096 tokens 181 -> 172, but a workgroup less a CU: 2048 Zipf 153 -> 163).
 __device__ const uint4 k_zero = { 0, 0, 0, 0 };                 // what loads read past the end of a row
 
 // 16 or 4 bytes a lane from memory to LDS at `lds` (uniform; lane after lane). As asm, so that the compiler does not hold every
@@ -766,8 +780,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
         }
     }
     // A lane holds columns 16 n + 4 g .. + 3 of row 16 m + l16 of the wave's (SwiGLU: of gate tile 2 n and up tile 2 n + 1). 16 rows at a
-    // time cross LDS, in the wave's own part of it, so that a row's columns go out together -- and so that what differs by type
-    // and edge is code for one store and not for all of a lane's (unrolled over 32 tiles it took 12 us to fetch).
+    // time cross LDS, in the wave's own part of it, so that a row's columns go out together, and what differs by type and edge is code
+    // for one store (stores straight from the lanes, 8 bytes a row each, took the same time and 30 times the code).
     constexpr int TO = SW ? TN / 2 : TN, LANES = 4 * TO, PITCH = 16 * TO + 4;
     static_assert(WV * 16 * PITCH * 4 <= (int)sizeof(lds), "the rows fit the stages' buffers");
     __syncthreads();
