@@ -512,8 +512,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 //
 // LDS. A row of a stage is 128 bytes (64 columns in 16 bits, 256 in MX4; x beside MX4 weights: two such halves, and the
 // weights' rows 64 bytes). The loads write lane after lane, 16 bytes each, so the order within a row is chosen at the
-// source: the chunk at place p of row r is p ^ (r & 7) (of 64-byte rows p ^ ((r >> 1) & 3)), and the 16 rows that a matrix
-// operand reads at one column fall on all the banks evenly.
+// source: the chunk at place p of row r is number p ^ (r & 7) (of 64-byte rows p ^ ((r >> 1) & 3)), and the 16 rows and four lane
+// groups that read a matrix operand fall on all the banks evenly.
 //
 // Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y.
 //
@@ -556,6 +556,9 @@ template <int XT, int WT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS
     static constexpr int LOADS = XL + WL + XSL + WSL;                        // a wave's, every stage
     static constexpr int AT_W = XG * 1024, AT_XS = AT_W + WG * 1024, AT_WS = AT_XS + XS * 256, STAGE = AT_WS + WS * 256;
     static constexpr int TM = MT / WM / 16, TN = NT / WN / 16;               // matrix tiles a wave
+    // the chunk that place 4 h + g (before the rows' permutation) holds, for step h and lane group g: MX4 x's chunk 2 g + h, so that
+    // a lane group's two blocks have neighbouring scale bytes
+    static __device__ __forceinline__ int chunk(int place) { return XT == MX4 ? (place & 3) * 2 + (place >> 2) : place; }
     static_assert(XG % WAVES_ == 0 && WG % WAVES_ == 0 && LOADS * (BUFS - 1) < 64 && TN % 2 == 0, "tile");
 };
 
@@ -591,14 +594,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
 #pragma unroll
         for (int i = 0; i < G::XL; ++i) {
             const int q = wave + i * WV, r = 8 * (G::MIXED ? q >> 1 : q) + (lane >> 3);
-            xp[i] = a.x + (int64_t)max(rows_x[r], 0) * a.x_pitch + 16 * ((lane & 7) ^ (r & 7)) + (G::MIXED ? 128 * (q & 1) : 0);
+            xp[i] = a.x + (int64_t)max(rows_x[r], 0) * a.x_pitch + 16 * G::chunk((lane & 7) ^ (r & 7)) + (G::MIXED ? 128 * (q & 1) : 0);
         }
 #pragma unroll
         for (int i = 0; i < G::WL; ++i) {
             const int q = wave + i * WV;
             const int r = G::MIXED ? 16 * q + (lane >> 2) : 8 * q + (lane >> 3);
             wp[i] = we + (int64_t)w_row(r) * a.w_pitch +
-                    16 * (G::MIXED ? (lane & 3) ^ ((r >> 1) & 3) : (lane & 7) ^ (r & 7));
+                    16 * (G::MIXED ? (lane & 3) ^ ((r >> 1) & 3) : G::chunk((lane & 7) ^ (r & 7)));
         }
 #pragma unroll
         for (int i = 0; i < G::XSL; ++i) {
@@ -619,7 +622,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
 #pragma unroll
             for (int i = 0; i < G::XL; ++i) {
                 const int q = wave + i * WV, r = 8 * (G::MIXED ? q >> 1 : q) + (lane >> 3);
-                const int col = XT == MX4 ? 32 * ((lane & 7) ^ (r & 7)) : 8 * ((lane & 7) ^ (r & 7)) + (G::MIXED ? 64 * (q & 1) : 0);
+                const int col = (XT == MX4 ? 32 : 8) * G::chunk((lane & 7) ^ (r & 7)) + (G::MIXED ? 64 * (q & 1) : 0);
                 const char* p = xp[i] + (int64_t)t * G::XROW;
                 if (!full && k + col >= a.K) p = (const char*)&k_zero;
                 dma16((gaddr)p, to + q * 1024);
@@ -627,7 +630,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
 #pragma unroll
             for (int i = 0; i < G::WL; ++i) {
                 const int q = wave + i * WV, r = G::MIXED ? 16 * q + (lane >> 2) : 8 * q + (lane >> 3);
-                const int col = G::MIXED ? 32 * ((lane & 3) ^ ((r >> 1) & 3)) : (WT == MX4 ? 32 : 8) * ((lane & 7) ^ (r & 7));
+                const int col = G::MIXED ? 32 * ((lane & 3) ^ ((r >> 1) & 3)) : (WT == MX4 ? 32 : 8) * G::chunk((lane & 7) ^ (r & 7));
                 gaddr p = wp[i] + (int64_t)t * G::WROW;
                 if (!full && k + col >= a.K) p = (gaddr)&k_zero;
                 dma16(p, to + G::AT_W + q * 1024);
@@ -680,9 +683,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                 for (int h = 0; h < 2; ++h) {
                     uint4 xv[TM], wv[TN];
 #pragma unroll
-                    for (int i = 0; i < TN; ++i) wv[i] = *(const uint4*)(W + (wr + 16 * i) * 128 + 16 * ((2 * g + h) ^ (l16 & 7)));
+                    for (int i = 0; i < TN; ++i) wv[i] = *(const uint4*)(W + (wr + 16 * i) * 128 + 16 * ((4 * h + g) ^ (l16 & 7)));
 #pragma unroll
-                    for (int i = 0; i < TM; ++i) xv[i] = *(const uint4*)(X + (xr + 16 * i) * 128 + 16 * ((2 * g + h) ^ (l16 & 7)));
+                    for (int i = 0; i < TM; ++i) xv[i] = *(const uint4*)(X + (xr + 16 * i) * 128 + 16 * ((4 * h + g) ^ (l16 & 7)));
 #pragma unroll
                     for (int n = 0; n < TN; ++n)
 #pragma unroll
