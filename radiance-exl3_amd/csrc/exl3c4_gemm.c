@@ -47,16 +47,17 @@ int exl3c4_mx4_dequant(const void* codes, int64_t codes_pitch, const void* scale
                                   out, out_dtype, out_pitch, stream);
 }
 
-/* One operand of the product: rows of K columns, pitch as the caller gives it; *bytes: the pitch in bytes. */
-static int operand_check(int32_t type, const void* p, const void* scales, int64_t pitch, int64_t s_pitch, int64_t K,
+/* One operand of the product: rows of K columns, pitch as the caller gives it; *bytes: the pitch in bytes. table: p and scales are
+ * device arrays of pointers. */
+static int operand_check(int32_t type, const void* p, const void* scales, int table, int64_t pitch, int64_t s_pitch, int64_t K,
                          int64_t* bytes) {
     const int mx4 = type == EXL3C4_MX4;
     if (!p || (mx4 && !scales)) return EXL3C4_E_INVAL;
     if (pitch < (mx4 ? K / 2 : K) || (mx4 && s_pitch < K / 32)) return EXL3C4_E_STRIDE;      /* K in whole blocks */
     if (pitch > MAX_PITCH || s_pitch > MAX_PITCH) return EXL3C4_E_STRIDE;
     *bytes = mx4 ? pitch : 2 * pitch;
-    if ((uintptr_t)p % 16 || *bytes % 16) return EXL3C4_E_ALIGN;
-    if (mx4 && ((uintptr_t)scales % 4 || s_pitch % 4)) return EXL3C4_E_ALIGN;
+    if ((uintptr_t)p % (table ? 8 : 16) || *bytes % 16) return EXL3C4_E_ALIGN;
+    if (mx4 && ((uintptr_t)scales % (table ? 8 : 4) || s_pitch % 4)) return EXL3C4_E_ALIGN;
     return EXL3C4_OK;
 }
 
@@ -81,9 +82,9 @@ int exl3c4_moe_gemm(const Exl3c4Gemm* g, void* stream) {
     if (g->T == 0) return EXL3C4_OK;
     if (!g->y) return EXL3C4_E_INVAL;
     if (g->x_rows < (g->sorted_tok ? 1 : g->T)) return EXL3C4_E_SHAPE;
-    rc = operand_check(g->x_type, g->x, g->x_scales, g->x_pitch, g->xs_pitch, g->K, &x_bytes);
+    rc = operand_check(g->x_type, g->x, g->x_scales, 0, g->x_pitch, g->xs_pitch, g->K, &x_bytes);
     if (rc) return rc;
-    rc = operand_check(g->w_type, g->w, g->w_scales, g->w_pitch, g->ws_pitch, g->K, &w_bytes);
+    rc = operand_check(g->w_type, g->w, g->w_scales, g->w_stride == 0, g->w_pitch, g->ws_pitch, g->K, &w_bytes);
     if (rc) return rc;
     if (w_bytes > MAX_W_PITCH || g->ws_pitch > MAX_W_PITCH) return EXL3C4_E_STRIDE;
     /* an entry's last row ends with its last column */
@@ -95,7 +96,6 @@ int exl3c4_moe_gemm(const Exl3c4Gemm* g, void* stream) {
         if (g->ws_stride % 4) return EXL3C4_E_ALIGN;
         if ((g->ws_stride == 0) != (g->w_stride == 0)) return EXL3C4_E_INVAL;      /* one form for both tables */
     }
-    if (g->w_stride == 0 && ((uintptr_t)g->w % 8 || (uintptr_t)g->w_scales % 8)) return EXL3C4_E_ALIGN;
     if ((uintptr_t)g->y % (uintptr_t)size_of(g->y_type) || (uintptr_t)g->sorted_tok % 4 ||
         (uintptr_t)g->expert_offset % 4)
         return EXL3C4_E_ALIGN;

@@ -209,6 +209,23 @@ def test_pointer_tables_give_the_stacked_buffers_bits(ex, pair):
     assert torch.equal(yd[:40, :32].cpu(), got)
 
 
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+@pytest.mark.parametrize("tokens", [20, 600])
+def test_a_pointer_table_that_starts_between_16_bytes(ex, pair, tokens):
+    got, y, tol, gm = run(ex, pair, "f32", False, tokens, 2, 5, 640, 128)
+    _, wd, _, yd = gm.keep
+    table = lambda t: torch.tensor([0] + [t[e].data_ptr() for e in range(t.shape[0])], dtype=torch.int64, device="cuda")
+    tw = table(wd.codes if pair[1] == "mx4" else wd)
+    gm.w, gm.w_stride = tw.data_ptr() + 8, 0
+    if pair[1] == "mx4":
+        ts = table(wd.scales)
+        gm.w_scales, gm.ws_stride = ts.data_ptr() + 8, 0
+    yd.fill_(7)
+    assert ex.moe_gemm(gm) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(yd[:2 * tokens, :640].cpu(), got)
+
+
 @pytest.mark.parametrize("pair", [p for p in PAIRS if p[1] == "mx4"], ids="-".join)
 @pytest.mark.parametrize("tokens", [3, 150])
 @pytest.mark.parametrize("K", [256, 2304])

@@ -64,6 +64,14 @@ def test_moe_gemm_refuses_mx4(change, want):
     assert rc(mx4(**change)) == want
 
 
+def test_a_pointer_table_needs_a_pointers_alignment():
+    """A row of a layers x experts table may start at any pointer: what is refused is what comes behind (here the pitch), not it."""
+    far = {"w_stride": 0, "w": P + 8, "w_pitch": (1 << 26) + 8}
+    assert rc(gemm(**far)) == STRIDE and rc(gemm(**dict(far, w=P + 4))) == ALIGN
+    far = {"w_stride": 0, "ws_stride": 0, "w": P + 8, "w_scales": P + 8, "w_pitch": (1 << 27) + 16}
+    assert rc(mx4(**far)) == STRIDE and rc(mx4(**dict(far, w=P + 4))) == ALIGN
+
+
 def test_no_rows_launch_nothing():
     assert rc(gemm(T=0, x=None, w=None, y=None)) == 0
     assert rc(mx4(T=0, x=None, w=None, y=None)) == 0
