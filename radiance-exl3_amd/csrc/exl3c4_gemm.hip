@@ -813,6 +813,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
     }
 }
 
+// Threads a launch may have in all: what it holds in 32 bits.
+constexpr int64_t THREADS = UINT32_MAX;
 int launched() { return hipGetLastError() == hipSuccess ? 0 : EXL3C4_E_DEVICE; }
 
 // Chunks of at most `rows` that the launch's segments (the runs, and the rows before and behind them) can make.
@@ -826,7 +828,7 @@ int launch_rows(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr int cols = 16 * (SW ? NS / 2 : NS);
     a.tiles = (a.n_out + cols - 1) / cols;
     const int64_t grid = chunk_bound(a, 1 << ROWS_LOG2) * a.tiles;
-    if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
+    if (grid > THREADS / (64 * WAVES)) return EXL3C4_E_SHAPE;
     hipLaunchKernelGGL((k_mg_rows<XT, WT, SW, NS>), dim3((unsigned)grid), dim3(64 * WAVES), 0, st, a);
     return launched();
 }
@@ -836,7 +838,7 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr int cols = SW ? NT / 2 : NT;
     a.tiles = (a.n_out + cols - 1) / cols;
     const int64_t grid = (chunk_bound(a, 1 << MT_LOG2) * a.tiles + 7) / 8 * 8;
-    if (grid > INT32_MAX) return EXL3C4_E_SHAPE;
+    if (grid > THREADS / (64 * WM * WN)) return EXL3C4_E_SHAPE;
     hipLaunchKernelGGL((k_mg_tile<XT, WT, SW, MT_LOG2, NT, WM, WN, BUFS>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
     return launched();
 }

@@ -72,6 +72,14 @@ def test_a_pointer_table_needs_a_pointers_alignment():
     assert rc(mx4(**far)) == STRIDE and rc(mx4(**dict(far, w=P + 4))) == ALIGN
 
 
+@pytest.mark.parametrize("change", [{"T": 1 << 20, "x_rows": 1 << 20, "n_expert": 1 << 20}, {"T": 1 << 30, "x_rows": 1 << 30, "n_expert": 1}],
+                         ids=["rows", "tiles"])
+def test_more_threads_than_a_launch_holds_are_refused(change):
+    """17.8 M workgroups of 256 threads and 2^29 of 512: past 2^32 threads, before anything is launched."""
+    n = 1024 if change["n_expert"] > 1 else 1 << 15
+    assert rc(gemm(N=n, y_pitch=n, w_stride=n * 128, **change)) == SHAPE
+
+
 def test_no_rows_launch_nothing():
     assert rc(gemm(T=0, x=None, w=None, y=None)) == 0
     assert rc(mx4(T=0, x=None, w=None, y=None)) == 0
