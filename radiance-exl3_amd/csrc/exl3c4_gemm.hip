@@ -518,13 +518,17 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 // Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y.
 //
 // What bounds it, measured. Where experts have up to some 60 rows, memory: bf16, 200 and 400 tokens of top-10 over 512 experts 5.9 to 6.1 TB/s
-// of weights, the card's reading rate. Beyond, the stages' latency: a CU takes about 88 bytes a ns from its L2, and with
-// 256 x 256 tiles two stages (128 KB) are all that LDS holds, so that a stage's loads (64 KB, 0.74 us) and its products (1.05 us at 2.05
-// PFLOP/s) only partly cover each other: 8192 tokens over 8 experts bf16 at 1.0 PFLOP/s, where a plain library product of 8192^3
-// reaches 1.44. Tried without gain: the next step's operands read ahead into registers (188 -> 185 us bf16, MX4 spilled), loads spread between
-// the products (188 -> 198), four stages of half the columns (64-byte rows fetch each line twice: 188 -> 204), one workgroup
-// a CU taking unit after unit with the next one's loads under the last one's stores (188 -> 199), weights asked for before the rows of x
-// are known (the same), scales in 16-byte loads (MX4 4096 tokens 181 -> 172, but a workgroup less a CU: 2048 Zipf 153 -> 163).
+// of weights, the card's reading rate. Beyond, the two sides of a stage, which only partly cover each other: bf16, 8192 tokens over 8
+// experts (2816 x 2048) 192 us, 1.0 PFLOP/s; without its loads 149 (at the clock that the power then leaves, 1.27 PFLOP/s with starts and
+// stores; a plain library product of 8192^3 reaches 1.44 in all), without its products 160: with 256 x 256 tiles two stages
+// (128 KB) are all that LDS holds, so that one stage's loads are out at a time. MX4 (the same sizes) 88, 75 and 72.
+// Tried without gain (us there): the waves in two halves that take turns with reads and products 211, products of 32 x 32 209, a line
+// of each row of later stages asked for ahead 211, stages in another order by workgroup 197 to 202, the next step's operands read ahead
+// into registers (188 -> 185, MX4 spilled), loads spread between the products (188 -> 198), four stages of half the columns (64-byte rows
+// fetch each line twice: 188 -> 204), one workgroup a CU taking unit after unit with the next one's loads under the last one's
+// stores (188 -> 199), weights asked for before the rows of x are known (the same), scales in 16-byte loads (MX4 4096 tokens
+// 181 -> 172, but a workgroup less a CU: 2048 Zipf 153 -> 163). Neither the rows' pitch (K = 2048 against 2112) nor the order within
+// a line changes the loads' rate.
 __device__ const uint4 k_zero = { 0, 0, 0, 0 };                 // what loads read past the end of a row
 
 // 16 or 4 bytes a lane from memory to LDS at `lds` (uniform; lane after lane). As asm, so that the compiler does not hold every
