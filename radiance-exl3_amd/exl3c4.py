@@ -60,7 +60,7 @@ class Mx4:
     """MX4 rows (include/exl3c4.h) of values [..., rows, cols]: codes uint8 [..., rows, >= 16 ceil(cols / 32)], scales uint8
     [..., rows, >= ceil(cols / 32)], the columns they stand for. The conversions take a row's pitches from the tensors once,
     here; leading dimensions have to step evenly as one for them (for moe_gemm they need not)."""
-    __slots__ = ("codes", "scales", "cols", "shape", "c_ptr", "s_ptr", "c_pitch", "s_pitch")
+    __slots__ = ("codes", "scales", "cols", "shape", "rows", "device", "c_ptr", "s_ptr", "c_pitch", "s_pitch")
 
     def __init__(self, codes, scales, cols: int):
         nb = (cols + 31) // 32
@@ -68,6 +68,7 @@ class Mx4:
                 codes.element_size() != 1 or scales.element_size() != 1 or codes.device != scales.device:
             raise ValueError("the MX4 planes do not fit each other or their columns")
         self.codes, self.scales, self.cols, self.shape = codes, scales, cols, codes.shape[:-1] + (cols,)
+        self.rows, self.device = codes.shape[:-1].numel(), codes.get_device()
         self.c_ptr, self.s_ptr, self.c_pitch, self.s_pitch = codes.data_ptr(), scales.data_ptr(), None, None
 
     def pitches(self):
@@ -539,24 +540,30 @@ def mx4_empty(shape, device="cuda") -> Mx4:
                torch.empty((*lead, (nb + 3) // 4 * 4), dtype=torch.uint8, device=device), cols)
 
 
+def _convert(fn, v, q: Mx4, stream, quant: bool) -> int:
+    """One of the conversions between the rows of v and q (a small one is bound by what happens here: rows that follow each
+    other need no look at the strides)."""
+    import torch
+    dev = v.get_device()
+    if v.shape != q.shape or dev != q.device:
+        raise ValueError("the values and q have other shapes or devices")
+    n, pitch = (q.rows, q.cols) if v.is_contiguous() else _rows(v)
+    cp, sp = q.pitches() if q.c_pitch is None else (q.c_pitch, q.s_pitch)
+    args = (v.data_ptr(), _dt(v), n, q.cols, pitch, q.c_ptr, cp, q.s_ptr, sp) if quant else \
+        (q.c_ptr, cp, q.s_ptr, sp, n, q.cols, v.data_ptr(), _dt(v), pitch)
+    if stream is not None and dev == torch.cuda.current_device():
+        return fn(*args, stream.cuda_stream)
+    return _launch_on(v.device, stream, fn, *args)
+
+
 def mx4_quant(x, q: Mx4, stream=None) -> int:
     """exl3c4_mx4_quant of x [..., cols] (f32 / f16 / bf16) into q; returns the status."""
-    if x.shape != q.shape or x.device != q.codes.device:
-        raise ValueError("x and q have other shapes or devices")
-    n, pitch = _rows(x)
-    cp, sp = q.pitches()
-    return _launch_on(x.device, stream, lib().exl3c4_mx4_quant, x.data_ptr(), _dt(x), n, q.cols, pitch, q.c_ptr, cp,
-                      q.s_ptr, sp)
+    return _convert(lib().exl3c4_mx4_quant, x, q, stream, True)
 
 
 def mx4_dequant(q: Mx4, out, stream=None) -> int:
     """exl3c4_mx4_dequant of q into out [..., cols] (f32 / f16 / bf16); returns the status."""
-    if out.shape != q.shape or out.device != q.codes.device:
-        raise ValueError("q and out have other shapes or devices")
-    n, pitch = _rows(out)
-    cp, sp = q.pitches()
-    return _launch_on(out.device, stream, lib().exl3c4_mx4_dequant, q.c_ptr, cp, q.s_ptr, sp, n, q.cols, out.data_ptr(),
-                      _dt(out), pitch)
+    return _convert(lib().exl3c4_mx4_dequant, out, q, stream, False)
 
 
 def _planes(t):
