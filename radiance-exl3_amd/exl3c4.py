@@ -578,6 +578,8 @@ def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT
     sorted rows), expert_offset i32 [n_expert + 1], y [T, N] ([T, N / 2] with ACT_SWIGLU) f16, bf16 or f32."""
     xv, xs, K, xt = _planes(x)
     wv, ws, Kw, wt = _planes(w)
+    if xv.dim() != 2 or wv.dim() != 3 or y.dim() != 2:
+        raise ValueError("x and y are rows, w one [N, K] an expert")
     g = Gemm()
     g.x_type, g.w_type, g.y_type, g.act = xt, wt, _dt(y), act
     E, N = wv.shape[0], wv.shape[1]

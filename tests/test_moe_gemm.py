@@ -130,6 +130,20 @@ def test_the_binding_refuses_what_does_not_fit():
             bad()
 
 
+def test_the_binding_refuses_operands_of_another_rank():
+    """x of a batch and a sequence, weights of one expert as they are, y by head: their strides are not a row's, and the call would
+    have read every other sequence's first token."""
+    i = torch.zeros(4, dtype=torch.int32)
+    x, w, y = torch.zeros(4, 64).half(), torch.zeros(3, 8, 64).half(), torch.zeros(4, 8)
+    m = exl3c4.mx4_empty((2, 2, 64), device="cpu")
+    for bad in (lambda: exl3c4.make_gemm(x.reshape(2, 2, 64), w, i, i, y),
+                lambda: exl3c4.make_gemm(x, w[0], i, i, torch.zeros(4, 64)),
+                lambda: exl3c4.make_gemm(x, w, i, i, torch.zeros(4, 8, 2)),
+                lambda: exl3c4.make_gemm(m, exl3c4.mx4_empty((3, 8, 64), device="cpu"), i, i, y)):
+        with pytest.raises(ValueError):
+            bad()
+
+
 def test_the_reference_rounds_to_the_nearest_code():
     """mx4ref.quant on every tie and neighbour of a tie, against the format's list."""
     x = torch.zeros(1, 32)
