@@ -280,7 +280,9 @@ __device__ __forceinline__ bool any_code(const uint4& q) { return ((q.x | q.y | 
 // ------------------------------------------------------------------------------------------ few rows an expert
 // A workgroup: a chunk of up to 16 rows against NS strips of 16 weight rows (with SwiGLU half of them gate rows and half their up
 // rows), each wave a part of k; the weights go from memory straight to the matrix units' operands, each byte read
-// once, and the parts' sums meet in LDS in a fixed order.
+// once, and the parts' sums meet in LDS in a fixed order. Bound by latency for one token (512 experts, bf16 1024 x 2048: 13.2 us, of
+// which the 42 MB ask 6.7) and by memory beyond (f16 2048 x 512 at 8 tokens 32 us, 4.9 TB/s). Four waves and two steps' loads out
+// together: with four steps these take 14.4 and 36.8 us, with eight waves 13.7 and 42.5 (MX4 w, bf16 x, 32 tokens 60, 85 and 92).
 constexpr int ROWS_LOG2 = 4;
 constexpr int WAVES = 4;
 
