@@ -524,7 +524,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 // experts (2816 x 2048) 192 us, 1.0 PFLOP/s; without its loads 149 (at the clock that the power then leaves, 1.27 PFLOP/s with starts and
 // stores; a plain library product of 8192^3 reaches 1.44 in all), without its products 160: with 256 x 256 tiles two stages
 // (128 KB) are all that LDS holds, so that one stage's loads are out at a time. MX4 (the same sizes) 88, 75 and 72.
-// Tried without gain (us there): the waves in two halves that take turns with reads and products 211, products of 32 x 32 209, a line
+// Tried without gain (us there): the waves in two halves that take turns with reads and products 211, products of 32 x 32 209, 128 x 256 tiles three stages deep 223, a line
 // of each row of later stages asked for ahead 211, stages in another order by workgroup 197 to 202, the next step's operands read ahead
 // into registers (188 -> 185, MX4 spilled), loads spread between the products (188 -> 198), four stages of half the columns (64-byte rows
 // fetch each line twice: 188 -> 204), one workgroup a CU taking unit after unit with the next one's loads under the last one's

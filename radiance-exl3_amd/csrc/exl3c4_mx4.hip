@@ -7,7 +7,7 @@
 // nearest even and saturates (checked for every tie and every exponent against that rule), and its inverse is exact.
 //
 // Both are bound by memory: 131072 x 2048 f32 quantised in 261 us (1.07 GB in, 0.14 out: 4.6 TB/s) and read back in 291
-// (4.2 TB/s; a large copy on this card 4.7); 20480 x 650 f16 in 9.8 and 7.5 us; 8 x 2048 in 2.5 and 2.2, a launch's least.
+// (4.2 TB/s; a large copy on this card 4.7); 20480 x 650 f16 in 9.5 and 7.4 us; 8 x 2048 in 2.5 and 1.9, a launch's least.
 // Four slots a lane, 256 lanes: the loads of four are out together.
 #include <hip/hip_runtime.h>
 
