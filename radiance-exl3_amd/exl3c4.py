@@ -58,23 +58,37 @@ class Gemm(C.Structure):
 
 class Mx4:
     """MX4 rows (include/exl3c4.h) of values [..., rows, cols]: codes uint8 [..., rows, >= 16 ceil(cols / 32)], scales uint8
-    [..., rows, >= ceil(cols / 32)], the columns they stand for. The conversions take a row's pitches from the tensors once,
-    here; leading dimensions have to step evenly as one for them (for moe_gemm they need not)."""
-    __slots__ = ("codes", "scales", "cols", "shape", "rows", "device", "c_ptr", "s_ptr", "c_pitch", "s_pitch")
+    [..., rows, >= ceil(cols / 32)], the columns they stand for. Its attributes are fixed, and the planes keep their sizes and
+    strides (the conversions take a row's pitches from them once); where their memory is, is read at each call. Leading
+    dimensions have to step evenly as one for the conversions (for moe_gemm they need not)."""
+    __slots__ = ("codes", "scales", "cols", "shape", "rows", "device", "_pitches")
 
     def __init__(self, codes, scales, cols: int):
         nb = (cols + 31) // 32
         if codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] < 16 * nb or scales.shape[-1] < nb or \
                 codes.element_size() != 1 or scales.element_size() != 1 or codes.device != scales.device:
             raise ValueError("the MX4 planes do not fit each other or their columns")
-        self.codes, self.scales, self.cols, self.shape = codes, scales, cols, codes.shape[:-1] + (cols,)
-        self.rows, self.device = codes.shape[:-1].numel(), codes.get_device()
-        self.c_ptr, self.s_ptr, self.c_pitch, self.s_pitch = codes.data_ptr(), scales.data_ptr(), None, None
+        put = super().__setattr__
+        put("codes", codes)
+        put("scales", scales)
+        put("cols", cols)
+        put("shape", codes.shape[:-1] + (cols,))
+        put("rows", codes.shape[:-1].numel())
+        put("device", codes.get_device())
+        put("_pitches", None)
+
+    def __setattr__(self, name, *value):
+        raise AttributeError(f"{name} of an Mx4 is fixed: make another one")
+
+    __delattr__ = __setattr__
+
+    def __reduce__(self):                                      # copies and pickles: made of their own planes
+        return Mx4, (self.codes, self.scales, self.cols)
 
     def pitches(self):
-        if self.c_pitch is None:
-            self.c_pitch, self.s_pitch = _rows(self.codes)[1], _rows(self.scales)[1]
-        return self.c_pitch, self.s_pitch
+        if self._pitches is None:
+            super().__setattr__("_pitches", (_rows(self.codes)[1], _rows(self.scales)[1]))
+        return self._pitches
 
 
 def lib():
@@ -548,9 +562,10 @@ def _convert(fn, v, q: Mx4, stream, quant: bool) -> int:
     if v.shape != q.shape or dev != q.device:
         raise ValueError("the values and q have other shapes or devices")
     n, pitch = (q.rows, q.cols) if v.is_contiguous() else _rows(v)
-    cp, sp = q.pitches() if q.c_pitch is None else (q.c_pitch, q.s_pitch)
-    args = (v.data_ptr(), _dt(v), n, q.cols, pitch, q.c_ptr, cp, q.s_ptr, sp) if quant else \
-        (q.c_ptr, cp, q.s_ptr, sp, n, q.cols, v.data_ptr(), _dt(v), pitch)
+    cp, sp = q._pitches or q.pitches()
+    c, s = q.codes.data_ptr(), q.scales.data_ptr()
+    args = (v.data_ptr(), _dt(v), n, q.cols, pitch, c, cp, s, sp) if quant else \
+        (c, cp, s, sp, n, q.cols, v.data_ptr(), _dt(v), pitch)
     if stream is not None and dev == torch.cuda.current_device():
         return fn(*args, stream.cuda_stream)
     return _launch_on(v.device, stream, fn, *args)
