@@ -294,7 +294,8 @@ int exl3c4_mx4_dequant(const void* codes, int64_t codes_pitch, const void* scale
  *     act SWIGLU   y[i][n] = silu(g) u, g = W_e[n] . x[r], u = W_e[N / 2 + n] . x[r],  n = 0 .. N / 2 - 1
  * with r = sorted_tok[i] / top_k, or r = i where sorted_tok is null (down: x holds sorted rows). Sums and the activation in f32, rounded
  * once. Rows outside the runs, and rows whose sorted_tok is negative or names no row of x, are written as zeros, as the EXL3 ops write
- * them; runs are clamped to [0, T). The same bits on every launch. (f16 x, MX4 w: where the scales of a weight row lie more than 2^13
+ * them; offsets are clamped to [0, T], and one below an earlier offset counts as that one, so that every row belongs to one run at most
+ * whatever the table holds. The same bits on every launch. (f16 x, MX4 w: where the scales of a weight row lie more than 2^13
  * apart, an infinity in x may give NaN where the sum is infinite.)
  *   x_type, w_type   F16, F16 | BF16, BF16 | F16, MX4 | BF16, MX4 | MX4, MX4
  *   y_type           F16, BF16 or F32

@@ -29,6 +29,17 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int F16 = EXL3C4_F16, BF16 = EXL3C4_BF16, MX4 = EXL3C4_MX4;
 
+// Memory by addresses known to be global: a pointer out of a table is a flat one otherwise, whose loads also hold up LDS.
+typedef const __attribute__((address_space(1))) char* gaddr;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load16(gaddr p) {
+    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)p);
+}
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));            // scale rows and offsets start at any word
+__device__ __forceinline__ uint4 load_words(gaddr p) {
+    return __builtin_bit_cast(uint4, (u32x4)*(const __attribute__((address_space(1))) u32x4_at4*)p);
+}
+
 // ------------------------------------------------------------------------------------------ the rows of a workgroup
 // The inclusive sum of v over lanes 0 .. lane, by DPP (row shifts, then the rows' totals by row broadcasts).
 __device__ __forceinline__ int wave_scan_incl(int v) {
@@ -41,28 +52,52 @@ __device__ __forceinline__ int wave_scan_incl(int v) {
     return v;
 }
 
+// The largest v of lanes 0 .. lane - 1 (0 for lane 0; no v is below 0).
+__device__ __forceinline__ int wave_max_before(int v, int lane) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    const int up = __shfl_up(v, 1);
+    return lane == 0 ? 0 : up;
+}
+
 struct Chunk { int expert, row0, rows, tile; };                 // expert -1: rows that no run holds (zeros)
 
 // 512 experts from `base` on, eight a lane: where each run starts, and the wave's inclusive sum of their chunks. The offsets are
-// clamped to [0, T] and a run that ends before it starts is empty: whatever the table holds, every chunk's rows are in [0, T).
+// clamped to [0, T], and one below an earlier one counts as that one (`reach`: the largest so far). So whatever the table holds, the runs, the
+// rows before the first and the rows behind the last are disjoint and make up [0, T): every row is written once.
 template <int MT_LOG2> struct Runs {
     int v[9], own, incl;
-    static __device__ __forceinline__ int chunks(int len) { return (max(len, 0) + (1 << MT_LOG2) - 1) >> MT_LOG2; }
-    __device__ __forceinline__ void read(const Exl3c4DevGemm& a, int base, int lane) {
-        struct __attribute__((packed, aligned(4))) Four { int v[4]; };
+    static __device__ __forceinline__ int chunks(int len) { return (len + (1 << MT_LOG2) - 1) >> MT_LOG2; }
+    __device__ __forceinline__ void read(const Exl3c4DevGemm& a, int base, int lane, int& reach) {
         const int i = base + 8 * lane;
         if (i + 8 <= a.n_expert) {                               // (16-byte loads: a load a value costs nine times the requests)
-            const Four p = *(const Four*)(a.off + i), q = *(const Four*)(a.off + i + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = p.v[j], v[4 + j] = q.v[j];
+            const uint4 p = load_words((gaddr)(a.off + i)), q = load_words((gaddr)(a.off + i + 4));
+            v[0] = (int)p.x, v[1] = (int)p.y, v[2] = (int)p.z, v[3] = (int)p.w;
+            v[4] = (int)q.x, v[5] = (int)q.y, v[6] = (int)q.z, v[7] = (int)q.w;
             v[8] = a.off[i + 8];
         } else {
 #pragma unroll
             for (int j = 0; j < 9; ++j) v[j] = a.off[min(i + j, a.n_expert)];
         }
-        own = 0;
 #pragma unroll
         for (int j = 0; j < 9; ++j) v[j] = min(max(v[j], 0), a.T);
+        int fall = v[0] - reach;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) fall |= v[j + 1] - v[j];
+        if (__any(fall < 0)) {                                   // a table that is no routing
+            v[0] = max(v[0], reach);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j + 1] = max(v[j + 1], v[j]);
+            const int before = wave_max_before(v[8], lane);
+#pragma unroll
+            for (int j = 0; j < 9; ++j) v[j] = max(v[j], before);
+        }
+        reach = __builtin_amdgcn_readlane(v[8], 63);
+        own = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) own += chunks(v[j + 1] - v[j]);
         incl = wave_scan_incl(own);
@@ -75,7 +110,7 @@ template <int MT_LOG2> struct Runs {
         bool found = false;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int len = max(v[j + 1] - v[j], 0), n = chunks(len);
+            const int len = v[j + 1] - v[j], n = chunks(len);
             if (!found && r < n) {
                 found = true;
                 e = base + 8 * lane + j;
@@ -102,12 +137,12 @@ __device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
     typedef Runs<MT_LOG2> R;
     Chunk out = { -1, 0, 0, 0 };
     R s;
-    int live = 0;
+    int live = 0, head = 0, tail = 0;
     for (int base = 0; base < a.n_expert; base += 512) {
-        s.read(a, base, lane);
+        s.read(a, base, lane, tail);
         live += s.total();
+        if (base == 0) head = __builtin_amdgcn_readlane(s.v[0], 0);
     }
-    const int head = min(max(a.off[0], 0), a.T), tail = min(max(a.off[a.n_expert], 0), a.T);
     const int n_head = R::chunks(head), total = live + n_head + R::chunks(a.T - tail);
     const uint32_t units = (uint32_t)total * (uint32_t)a.tiles, x = blockIdx.x & 7u, i = blockIdx.x >> 3;
     uint32_t unit = blockIdx.x;
@@ -127,8 +162,9 @@ __device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
     } else if (a.n_expert <= 512) {
         s.find(0, lane, c, out);
     } else {
+        int reach = 0;
         for (int base = 0; base < a.n_expert; base += 512) {
-            s.read(a, base, lane);
+            s.read(a, base, lane, reach);
             if (c < s.total()) {
                 s.find(base, lane, c, out);
                 break;
@@ -136,7 +172,6 @@ __device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
             c -= s.total();
         }
     }
-    out.rows = max(out.rows, 0);                                 // (a table that is no routing: more chunks than 32 bits count)
     return out;
 }
 // The same for the whole workgroup, by its first wave.
@@ -162,16 +197,7 @@ __device__ __forceinline__ int x_row(const Exl3c4DevGemm& a, int i) {
     return r < a.x_rows ? r : -1;
 }
 
-// Weights by addresses known to be global memory: a pointer out of a table is a flat one otherwise, whose loads also hold up LDS.
-typedef const __attribute__((address_space(1))) char* gaddr;
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ uint4 load16(gaddr p) {
-    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)p);
-}
-typedef u32x4 u32x4_at4 __attribute__((aligned(4)));            // scale rows start at any word
-__device__ __forceinline__ uint4 load_words(gaddr p) {
-    return __builtin_bit_cast(uint4, (u32x4)*(const __attribute__((address_space(1))) u32x4_at4*)p);
-}
+// A weight's words and an expert's weights.
 __device__ __forceinline__ uint32_t load4(gaddr p) { return *(const __attribute__((address_space(1))) uint32_t*)p; }
 __device__ __forceinline__ gaddr entry(const void* base, int64_t stride, int e) {
     return stride ? (gaddr)base + (int64_t)e * stride : ((const gaddr*)base)[e];
