@@ -7,8 +7,9 @@
 // row l % 16 -- in MX4 exactly one block, whose scale byte is the lane's own. x is the A operand (rows of D), W the B
 // operand (columns of D): lane l ends with D[m = 4 g + r][n = l % 16], r = 0 .. 3.
 //
-// MX4 WEIGHTS AGAINST 16-BIT x. bf16 holds e2m1 x 2^s exactly, so with bf16 x a lane's block is converted with its scale
-// (v_cvt_scalef32_pk_bf16_fp4) and multiplied as bf16. f16 does not hold the scales' range: with f16 x a row's blocks are converted
+// MX4 WEIGHTS AGAINST 16-BIT x. bf16 holds e2m1 x 2^s exactly for all but the two largest scales, so with bf16 x a lane's block is
+// converted with its scale (v_cvt_scalef32_pk_bf16_fp4) and multiplied as bf16; a wave (few rows) or a tile (many) that has met one of
+// those two, whose larger elements pass 2^128, sums again, with a quarter of every weight, and takes four times that. f16 does not hold the scales' range: with f16 x a row's blocks are converted
 // relative to the largest scale among some hundred columns (its level), where those within 2^-13 of it are exact in f16, and the
 // sums are scaled in f32 as they are added; blocks further down, if any of them is not all zeros, have passes of their own. Either
 // way every product is exact. (Scaling each block's sums by itself, one matrix instruction a block, took 125 us where this
@@ -267,10 +268,23 @@ template <int XT> __device__ __forceinline__ uint4 widen(uint32_t q, float scale
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 3)) };
 }
 // 2^(byte - 127) as an operand of the conversions (they read the exponent field), and as an f32 (255: NaN).
+constexpr uint32_t FAR = 253;                                   // scale bytes from here on: bf16 does not hold 4 or 6 times them
 __device__ __forceinline__ float scale_arg(uint32_t byte) { return __uint_as_float(byte << 23); }
 __device__ __forceinline__ float scale_f32(uint32_t byte) {
     const f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(2u, scale_arg(byte), 0);      // code 2 is 1
     return v[0];
+}
+
+// 8 codes times a quarter of the scale `byte` as 8 bf16, exact whatever the scale: from 2^-130 to 6 x 2^125. (Through f32, which holds the least of
+// them after the division; their low halves are zeros.)
+__device__ __forceinline__ uint4 widen_quarter(uint32_t q, uint32_t byte) {
+    const float scale = scale_arg(byte >= 2 && byte < 255 ? byte - 2 : byte), by = byte < 2 ? 0.25f : 1.f;
+    uint32_t w[4];
+#define PAIR(i) { const f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, i); \
+                  w[i] = __float_as_uint(v[0] * by) >> 16 | (__float_as_uint(v[1] * by) & 0xFFFF0000u); }
+    PAIR(0) PAIR(1) PAIR(2) PAIR(3)
+#undef PAIR
+    return { w[0], w[1], w[2], w[3] };
 }
 
 // The levels of f16's passes: the largest scale byte of a word (of four), and the largest below `below` (-1: none).
@@ -353,15 +367,17 @@ template <int XT, int WT, int NS> struct Step {
         const int n = (int)min((int64_t)(K - k) / 32, (int64_t)4);
         return n >= 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
     }
-    // a strip's 16 bytes and their scale: MX4 x the scale's byte, else as an operand of the conversion
+    // the products of a strip's 16 bytes: 16-bit weights, or MX4 with the word of their scales
     __device__ __forceinline__ f32x4 multiply(int g, const uint4& q, uint32_t sc, f32x4 acc) const {
-        if constexpr (WT != MX4) {
-            return mma<XT>(x[0], q, acc);
-        } else if constexpr (XT == MX4) {
-            return mma_mx4(x[0], (xsc >> (8 * g)) & 255, q, (sc >> (8 * g)) & 255, acc);
-        } else {
-            return multiply_by(q, scale_arg((sc >> (8 * g)) & 255), acc);
-        }
+        if constexpr (WT != MX4) return mma<XT>(x[0], q, acc);
+        else return mma_mx4(x[0], (xsc >> (8 * g)) & 255, q, (sc >> (8 * g)) & 255, acc);
+    }
+    // MX4 against 16 bits: by a scale as the conversions take it, or by a quarter of a scale's byte
+    __device__ __forceinline__ f32x4 multiply_quarter(const uint4& q, uint32_t byte, f32x4 acc) const {
+        const uint32_t word[4] = { q.x, q.y, q.z, q.w };
+#pragma unroll
+        for (int j = 0; j < NX; ++j) acc = mma<XT>(x[j], widen_quarter(word[j], byte), acc);
+        return acc;
     }
     __device__ __forceinline__ f32x4 multiply_by(const uint4& q, float f, f32x4 acc) const {
         const uint32_t word[4] = { q.x, q.y, q.z, q.w };
@@ -407,8 +423,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
         const bool has_x = xr >= 0;
         f32x4 acc[NS] = {};
         uint4 q[AHEAD][NS];
-        int t = (int)((int64_t)steps * wave / WV);
-        constexpr bool LEVELS = XT == F16 && WT == MX4;
+        const int from = (int)((int64_t)steps * wave / WV);
+        int t = from;
+        uint32_t top = 0;                                        // the largest scale that the lane has multiplied by
+        constexpr bool LEVELS = XT == F16 && WT == MX4, QUARTERS = XT == BF16 && WT == MX4;
         // f16 x, MX4 weights: the passes behind the first over steps t .. t + n - 1, each strip's rows from their own level on
         auto more_passes = [&](int t, int n, int* level) {
             bool more;
@@ -474,6 +492,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
                             const int b = (word >> (8 * g)) & 255;
                             p[s] = st[u].multiply_by(q[u][s], pass_scale(b, level[s], 256), p[s]);
                             more |= b < level[s] - LEVEL && any_code(q[u][s]);
+                        } else if constexpr (QUARTERS) {
+                            const uint32_t byte = (word >> (8 * g)) & 255;
+                            top = max(top, byte);
+                            acc[s] = st[u].multiply_by(q[u][s], scale_arg(byte), acc[s]);
                         } else {
                             acc[s] = st[u].multiply(g, q[u][s], word, acc[s]);
                         }
@@ -495,6 +517,17 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 #pragma unroll
                 for (int s = 0; s < NS; ++s) level[s] = 256 + LEVEL;
                 more_passes(t, 1, level);
+            } else if constexpr (QUARTERS) {
+                S st;
+                S::template load_w<false>(q[0], t, a.K, g, w, at);
+                st.template load_x<false>(t, a.K, g, x, xs, has_x);
+                const uint32_t live = S::live_bytes(a.K, (int64_t)t * S::KB);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const uint32_t byte = ((load4(ws[s] + (s_at + 4u * (uint32_t)t)) & live) >> (8 * g)) & 255;
+                    top = max(top, byte);
+                    acc[s] = st.multiply_by(q[0][s], scale_arg(byte), acc[s]);
+                }
             } else {
                 S st;
                 S::template load_w<false>(q[0], t, a.K, g, w, at);
@@ -506,6 +539,22 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
                     if constexpr (WT == MX4) word = load4(ws[s] + (s_at + 4u * (uint32_t)t)) & live;
                     acc[s] = st.multiply(g, q[0][s], word, acc[s]);
                 }
+            }
+        }
+        if (QUARTERS && __any(top >= FAR)) {                     // the wave's sums again, a strip at a time (for registers)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                f32x4 p = {};
+#pragma unroll 1
+                for (int u = from; u < to; ++u) {
+                    S st;
+                    st.template load_x<false>(u, a.K, g, x, xs, has_x);
+                    const bool in = (int64_t)u * S::KB + (S::KB / 4) * g < a.K;
+                    const uint4 v = in ? load16(w[s] + (at + 64u * (uint32_t)u)) : uint4{ 0, 0, 0, 0 };
+                    const uint32_t word = load4(ws[s] + (s_at + 4u * (uint32_t)u)) & S::live_bytes(a.K, (int64_t)u * S::KB);
+                    p = st.multiply_quarter(v, (word >> (8 * g)) & 255, p);
+                }
+                acc[s] = p * 4.f;
             }
         }
 #pragma unroll
@@ -557,6 +606,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 // stores (188 -> 199), weights asked for before the rows of x are known (the same), scales in 16-byte loads (MX4 4096 tokens
 // 181 -> 172, but a workgroup less a CU: 2048 Zipf 153 -> 163). Neither the rows' pitch (K = 2048 against 2112) nor the order within
 // a line changes the loads' rate.
+template <bool B> struct Is { static constexpr bool value = B; };
 __device__ const uint4 k_zero = { 0, 0, 0, 0 };                 // what loads read past the end of a row
 
 // 16 or 4 bytes a lane from memory to LDS at `lds` (uniform; lane after lane). As asm, so that the compiler does not hold every
@@ -680,8 +730,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                 dma4(p, to + G::AT_WS + ((wave + i * WV) % max(G::WS, 1)) * 256);
             }
         };
-        // the products of one stage; last: scale bytes past K (in a word that begins before it) count as 0
-        auto multiply = [&](int t, int buf, bool last) {
+        int top = 0;                                             // bf16 x, MX4 weights: the largest scale that the lane has multiplied by
+        // the products of one stage, by quarters of the weights or as they are; last: scale bytes past K (in a word that begins before
+        // it) count as 0
+        auto multiply = [&](int t, int buf, bool last, auto quarters) {
             const char* X = lds + buf * G::STAGE;
             const char* W = X + G::AT_W;
             const int xr = wm * TM * 16 + l16, wr = wn * TN * 16 + l16;      // the lane's row in the first tile of each
@@ -759,9 +811,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                     }
                 };
                 float f[TN];
-                if constexpr (XT == BF16) {
+                if constexpr (decltype(quarters)::value) {
+#pragma unroll 1
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int n = 0; n < TN; ++n) f[n] = scale_arg(byte[n]);
+                        for (int n = 0; n < TN; ++n) {
+                            const uint4 wv = widen_quarter(j == 0 ? q[n].x : j == 1 ? q[n].y : j == 2 ? q[n].z : q[n].w, byte[n]);
+#pragma unroll
+                            for (int m = 0; m < TM; ++m) acc[n][m] = mma<XT>(wv, x_at(m, 4 * g + j), acc[n][m]);
+                        }
+                } else if constexpr (XT == BF16) {
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) f[n] = scale_arg(byte[n]), top = max(top, byte[n]);
                     pass(f, acc);
                 } else {
                     // The rows of D are the weights': lane group g's are 4 g + r, whose scale words are 16 bytes in LDS. Each row's level
@@ -798,20 +859,36 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
                 }
             }
         };
+        auto sum = [&](auto quarters) {
 #pragma unroll
-        for (int i = 0; i < BUFS - 1; ++i)
-            if (i < stages) load(i, i);
-        int buf = 0;
-        for (int t = 0; t < stages; ++t) {
-            if (BUFS == 2 || t + 1 >= stages) wait_loads<0>();
-            else wait_loads<G::LOADS>();
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            const int next = buf == 0 ? BUFS - 1 : buf - 1;      // the buffer of stage t - 1, read by all before the barrier
-            if (t + BUFS - 1 < stages) load(t + BUFS - 1, next);
-            multiply(t, buf, t + 1 == stages);
-            asm volatile("" ::: "memory");
-            buf = buf + 1 == BUFS ? 0 : buf + 1;
+            for (int i = 0; i < BUFS - 1; ++i)
+                if (i < stages) load(i, i);
+            int buf = 0;
+            for (int t = 0; t < stages; ++t) {
+                if (BUFS == 2 || t + 1 >= stages) wait_loads<0>();
+                else wait_loads<G::LOADS>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                const int next = buf == 0 ? BUFS - 1 : buf - 1;  // the buffer of stage t - 1, read by all before the barrier
+                if (t + BUFS - 1 < stages) load(t + BUFS - 1, next);
+                multiply(t, buf, t + 1 == stages, quarters);
+                asm volatile("" ::: "memory");
+                buf = buf + 1 == BUFS ? 0 : buf + 1;
+            }
+        };
+        sum(Is<false>());
+        if constexpr (XT == BF16 && WT == MX4) {
+            if (__syncthreads_or(top >= (int)FAR)) {             // the tile's sums again
+#pragma unroll
+                for (int n = 0; n < TN; ++n)
+#pragma unroll
+                    for (int m = 0; m < TM; ++m) acc[n][m] = f32x4{ 0, 0, 0, 0 };
+                sum(Is<true>());
+#pragma unroll
+                for (int n = 0; n < TN; ++n)
+#pragma unroll
+                    for (int m = 0; m < TM; ++m) acc[n][m] *= 4.f;
+            }
         }
     }
     // A lane holds columns 16 n + 4 g .. + 3 of row 16 m + l16 of the wave's (SwiGLU: of gate tile 2 n and up tile 2 n + 1). 16 rows at a
