@@ -204,10 +204,37 @@ __device__ __forceinline__ gaddr entry(const void* base, int64_t stride, int e) 
     return stride ? (gaddr)base + (int64_t)e * stride : ((const gaddr*)base)[e];
 }
 
-// silu(g) u in f32: g / (1 + exp(-g)) by the hardware's exp2 and reciprocal (a few f32 steps from the exact value,
-// below the rounding to 16 bits; 2^-22 or so beside an f32 output's own sums).
-__device__ __forceinline__ float swiglu(float g, float u) {
+// silu(g) u = g u / (1 + e^-g) in f32, by the hardware's exp2 and reciprocal. The exponent's argument is rounded once, an error of e^-g that grows
+// with |g| and that a negative g meets in full: so from -8 up, where it is 9.8 steps of 2^-24 and the whole 16.8 at most. Below,
+// e^g = 2^n e with the argument's fraction exact to a step, silu = g 2^n e / (1 + 2^n e), and u comes in between the two halves of 2^n: 9 steps,
+// also where e^-g passes f32 (from -88.7 down) or silu is below it, and u brings the product back. Each value goes by its own g alone.
+constexpr float SILU_NEAR = -8.f;
+__device__ __forceinline__ float swiglu_near(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f)) * u;
+}
+__device__ __forceinline__ float swiglu_far(float g, float u) {
+    const float a = fmaxf(g, -1024.f);                           // (2^-1477: 0 beside any finite u)
+    const float n = rintf(a * 1.44269502162933349609f);
+    const float r = __builtin_fmaf(a, 1.92596299e-8f, __builtin_fmaf(a, 1.44269502162933349609f, -n));   // a log2 e - n, log2 e in two parts
+    const float e = __builtin_amdgcn_exp2f(r);
+    const int k = (int)n, half = k >> 1;
+    const float v = g * e * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_ldexpf(e, k));
+    const float y = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(v, half) * u, k - half);
+    return g == -__builtin_inff() ? __builtin_nanf("") : y;      // -inf / inf
+}
+__device__ __forceinline__ float swiglu(float g, float u) {
+    float y = swiglu_near(g, u);
+    if (g < SILU_NEAR) y = swiglu_far(g, u);
+    return y;
+}
+__device__ __forceinline__ f32x4 swiglu4(const f32x4& g, const f32x4& u) {
+    f32x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = swiglu_near(g[i], u[i]);
+    if (fminf(fminf(g[0], g[1]), fminf(g[2], g[3])) < SILU_NEAR)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = g[i] < SILU_NEAR ? swiglu_far(g[i], u[i]) : y[i];
+    return y;
 }
 
 __device__ __forceinline__ void store(char* p, int type, float v) {
@@ -906,9 +933,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
 #pragma unroll
         for (int n = 0; n < TO; ++n) {
             f32x4 v = SW ? acc[2 * n][m] : acc[n][m];
-            if (SW)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = swiglu(v[i], acc[SW ? 2 * n + 1 : n][m][i]);
+            if (SW) v = swiglu4(v, acc[SW ? 2 * n + 1 : n][m]);
             *(f32x4*)(rows + l16 * PITCH + 16 * n + 4 * g) = v;
         }
 #pragma unroll 1
