@@ -648,6 +648,13 @@ __device__ __forceinline__ void dma4(gaddr from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
+// Orders the wave's LDS accesses before it and behind it, whichever of its lanes makes them. (The hardware does one wave's in order, so this
+// is no instruction: it holds the compiler, which sees one lane's accesses to places that another lane's do not touch.)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 // Until at most N of the wave's loads are out, and none of its LDS reads.
 template <int N> __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
@@ -936,6 +943,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
             if (SW) v = swiglu4(v, acc[SW ? 2 * n + 1 : n][m]);
             *(f32x4*)(rows + l16 * PITCH + 16 * n + 4 * g) = v;
         }
+        wave_sync();                                             // other lanes read what a lane has written
 #pragma unroll 1
         for (int i = 0; i < TO; ++i) {
             const int q = i * (64 / LANES) + lane / LANES, r = (wm * TM + m) * 16 + q;
@@ -944,6 +952,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
             if (rows_x[r] < 0) v = f32x4{ 0, 0, 0, 0 };
             store4(a.y + (int64_t)(ch.row0 + r) * a.y_pitch + (int64_t)col * ysz, a.y_type, v, a.n_out - col, whole);
         }
+        wave_sync();                                             // and are done before it is written again
     }
 }
 
