@@ -172,6 +172,8 @@ typedef struct Exl3c4DevGemm {
     int32_t        grid;           /* workgroups, where they take several units each */
 } Exl3c4DevGemm;
 int exl3c4_dev_gemm(const Exl3c4DevGemm* g, int32_t x_type, int32_t w_type, int32_t act, void* stream);
+/* which of its kernels such a launch takes (T > 0): a tile's rows, or for few rows an expert the strips of a workgroup (2 or 4) */
+int exl3c4_dev_gemm_path(int32_t x_type, int32_t w_type, int32_t act, int64_t T, int64_t n_expert, int64_t N, int64_t K);
 int exl3c4_dev_mx4_quant(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t pitch, uint8_t* codes,
                          int64_t codes_pitch, uint8_t* scales, int64_t scales_pitch, void* stream);
 int exl3c4_dev_mx4_dequant(const uint8_t* codes, int64_t codes_pitch, const uint8_t* scales, int64_t scales_pitch,

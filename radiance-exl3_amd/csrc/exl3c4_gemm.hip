@@ -968,17 +968,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mg_tile(Exl3c4DevGemm a) {
 constexpr int64_t THREADS = UINT32_MAX;
 int launched() { return hipGetLastError() == hipSuccess ? 0 : EXL3C4_E_DEVICE; }
 
-// Chunks of at most `rows` that the launch's segments (the runs, and the rows before and behind them) can make.
-int64_t chunk_bound(const Exl3c4DevGemm& a, int rows) {
-    const int64_t seg = (int64_t)a.n_expert + 2;
-    return a.T / rows + (seg < a.T ? seg : a.T);
+// Chunks of at most `rows` that the segments of T rows (the runs of n_expert experts, and the rows before and behind them) can make.
+int64_t chunk_bound(int64_t T, int64_t n_expert, int rows) {
+    const int64_t seg = n_expert + 2;
+    return T / rows + (seg < T ? seg : T);
 }
 
 template <int XT, int WT, bool SW, int NS>
 int launch_rows(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr int cols = 16 * (SW ? NS / 2 : NS);
     a.tiles = (a.n_out + cols - 1) / cols;
-    const int64_t grid = chunk_bound(a, 1 << ROWS_LOG2) * a.tiles;
+    const int64_t grid = chunk_bound(a.T, a.n_expert, 1 << ROWS_LOG2) * a.tiles;
     if (grid > THREADS / (64 * WAVES)) return EXL3C4_E_SHAPE;
     hipLaunchKernelGGL((k_mg_rows<XT, WT, SW, NS>), dim3((unsigned)grid), dim3(64 * WAVES), 0, st, a);
     return launched();
@@ -988,7 +988,7 @@ template <int XT, int WT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS
 int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr int cols = SW ? NT / 2 : NT;
     a.tiles = (a.n_out + cols - 1) / cols;
-    const int64_t grid = (chunk_bound(a, 1 << MT_LOG2) * a.tiles + 7) / 8 * 8;
+    const int64_t grid = (chunk_bound(a.T, a.n_expert, 1 << MT_LOG2) * a.tiles + 7) / 8 * 8;
     if (grid > THREADS / (64 * WM * WN)) return EXL3C4_E_SHAPE;
     hipLaunchKernelGGL((k_mg_tile<XT, WT, SW, MT_LOG2, NT, WM, WN, BUFS>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
     return launched();
@@ -1003,33 +1003,36 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
 //   64 against 128         bf16 512/10 at 4096 522 / 409, 64/6 at 2000 113 / 95; MX4 193 / 175, 46 / 41; bf16 x, MX4 w 339 / 379.
 //   128 against 256        bf16 64/6 at 2000 95 / 85, 8/2 2816x2048 at 8192 225 / 190; MX4 64/6 at 2000 41 / 33, but K = 1408 at
 //                          8192 76 / 82 (few stages, and the larger tile's start and stores stand alone on its CU).
+// Returns a tile's rows (32, 64, 128, 256), or for few rows an expert the strips of a workgroup (2, 4).
+int choose(int x_type, int w_type, bool swiglu, int64_t T, int64_t n_expert, int64_t n_out, int64_t K) {
+    const bool mixed = w_type == MX4 && x_type != MX4;
+    const int64_t live = n_expert < T ? n_expert : T;
+    // workgroups of tiles of `rows` x `cols` (SwiGLU: half as many columns of y)
+    auto units = [&](int rows, int cols) {
+        if (swiglu) cols /= 2;
+        return chunk_bound(T, n_expert, rows) * ((n_out + cols - 1) / cols);
+    };
+    if (T <= (mixed ? 8 : 1) * live || units(32, 128) < 64 || (T <= 4 * live && units(32, 128) < 256))
+        return units(16, 64) >= 1024 ? 4 : 2;
+    if (mixed) return units(64, 128) < 256 ? 32 : 64;
+    if (T > 160 * live && units(256, 256) >= 256 && (w_type != MX4 || K >= 2048)) return 256;
+    if (T > 64 * live && units(128, 128) >= 256) return 128;
+    if ((w_type == MX4 && T <= 16 * live) || units(64, 128) < 256) return 32;
+    return 64;
+}
+
 template <int XT, int WT, bool SW>
 int launch(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr bool mixed = WT == MX4 && XT != MX4;
-    const int64_t T = a.T, live = a.n_expert < T ? a.n_expert : T;
-    // workgroups of tiles of `rows` x `cols` (SwiGLU: half as many columns of y)
-    auto units = [&](int rows, int cols) {
-        if (SW) cols /= 2;
-        return chunk_bound(a, rows) * ((a.n_out + cols - 1) / cols);
-    };
-    if (T <= (mixed ? 8 : 1) * live || units(32, 128) < 64 || (T <= 4 * live && units(32, 128) < 256)) {
-        if (units(16, 64) >= 1024) return launch_rows<XT, WT, SW, 4>(a, st);
-        return launch_rows<XT, WT, SW, 2>(a, st);
+    const int path = choose(XT, WT, SW, a.T, a.n_expert, a.n_out, a.K);
+    if (path == 2) return launch_rows<XT, WT, SW, 2>(a, st);
+    if (path == 4) return launch_rows<XT, WT, SW, 4>(a, st);
+    if (path == 32) return launch_tile<XT, WT, SW, 5, 128, 1, 4, 3>(a, st);
+    if constexpr (!mixed) {
+        if (path == 256) return launch_tile<XT, WT, SW, 8, 256, 2, 4, 2>(a, st);
+        if (path == 128) return launch_tile<XT, WT, SW, 7, 128, 2, WT == MX4 ? 2 : 4, 2>(a, st);
     }
-    if constexpr (mixed) {
-        if (units(64, 128) < 256) return launch_tile<XT, WT, SW, 5, 128, 1, 4, 3>(a, st);
-        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
-    } else if constexpr (WT == MX4) {
-        if (T > 160 * live && units(256, 256) >= 256 && a.K >= 2048) return launch_tile<XT, WT, SW, 8, 256, 2, 4, 2>(a, st);
-        if (T > 64 * live && units(128, 128) >= 256) return launch_tile<XT, WT, SW, 7, 128, 2, 2, 2>(a, st);
-        if (T <= 16 * live || units(64, 128) < 256) return launch_tile<XT, WT, SW, 5, 128, 1, 4, 3>(a, st);
-        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 2>(a, st);
-    } else {
-        if (T > 160 * live && units(256, 256) >= 256) return launch_tile<XT, WT, SW, 8, 256, 2, 4, 2>(a, st);
-        if (T > 64 * live && units(128, 128) >= 256) return launch_tile<XT, WT, SW, 7, 128, 2, 4, 2>(a, st);
-        if (units(64, 128) < 256) return launch_tile<XT, WT, SW, 5, 128, 1, 4, 3>(a, st);
-        return launch_tile<XT, WT, SW, 6, 128, 1, 4, 3>(a, st);
-    }
+    return launch_tile<XT, WT, SW, 6, 128, 1, 4, WT == MX4 ? 2 : 3>(a, st);
 }
 
 template <int XT, int WT>
@@ -1047,4 +1050,9 @@ extern "C" int exl3c4_dev_gemm(const Exl3c4DevGemm* g, int32_t x_type, int32_t w
     if (x_type == F16) return launch_act<F16, MX4>(a, act, st);
     if (x_type == BF16) return launch_act<BF16, MX4>(a, act, st);
     return launch_act<MX4, MX4>(a, act, st);
+}
+
+extern "C" int exl3c4_dev_gemm_path(int32_t x_type, int32_t w_type, int32_t act, int64_t T, int64_t n_expert, int64_t N, int64_t K) {
+    const bool swiglu = act == EXL3C4_ACT_SWIGLU;
+    return choose(x_type, w_type, swiglu, T, n_expert, swiglu ? N / 2 : N, K);
 }

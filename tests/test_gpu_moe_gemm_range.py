@@ -3,87 +3,77 @@ every 16- and 32-bit float by themselves) against x so small that the sums are f
 and the conversions at the same bytes."""
 import pytest
 
+import gemmpath
 import mx4ref
 from test_gpu_moe_gemm import ex, operand  # noqa: F401 (ex is a fixture)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-# (T, E, N, K): few rows an expert in narrow and in wide workgroups, and tiles; K with steps of four and a rest for each wave
-SIZES = {"rows": (6, 2, 40, 2592), "rows wide": (33, 33, 1000, 2592), "tile 32": (90, 2, 1450, 416), "tile 64": (270, 3, 3700, 416)}
+PATHS = [2, 4, 32, 64]                                                   # few rows an expert by 2 and 4 strips, tiles of 32 and 64 rows
 
 
-def weights(ex, g, E, N, K, scale):  # noqa: F811
-    """Random codes with the scale bytes that `scale` gives for [E, N, K / 32]: (operand, values in f64)."""
-    codes = torch.randint(0, 256, (E, N, K // 2), dtype=torch.uint8, generator=g)
-    s = torch.full((E, N, (K // 32 + 3) // 4 * 4), 255, dtype=torch.uint8)
-    s[..., :K // 32] = scale
-    return ex.Mx4(codes.cuda(), s.cuda(), K), mx4ref.dequant(codes, s, K)
-
-
-def x_of(ex, v, kind, low):  # noqa: F811
-    """x on the device and in f64: v's values, as MX4 with `low` off every scale byte."""
-    if kind != "mx4":
-        return operand(ex, v, kind)
-    q, _ = operand(ex, v, kind)
-    nb = v.shape[1] // 32
-    s = q.scales.cpu()
-    s[:, :nb] = torch.where(s[:, :nb] > low, s[:, :nb] - low, 0)
-    q.scales.copy_(s)
-    return q, mx4ref.dequant(q.codes.cpu(), s, v.shape[1])
+def size_of(kind, p):
+    """(T, experts, experts with weights of their own, N, K): steps of four and a rest for each wave of few rows."""
+    T, E, N = gemmpath.SIZES[p]
+    K = 2592 if p in (2, 4) else 416
+    assert gemmpath.path((kind, "mx4"), False, T, E, N, K) == p
+    return T, E, min(E, 3), N, K
 
 
 def check(ex, xd, x64, wd, w64, T, E):  # noqa: F811
     N = w64.shape[1]
+    w64 = gemmpath.Shared(w64, E)
     off = torch.tensor([T * e // E for e in range(E + 1)], dtype=torch.int32)
     y = torch.full((T, N), float("nan"), device="cuda")
-    assert ex.moe_gemm(ex.make_gemm(xd, wd, None, off.cuda(), y)) == 0
+    gm = ex.make_gemm(xd, wd, None, off.cuda(), y)
+    assert ex.moe_gemm(gemmpath.share(gm, wd, E) if E > w64.w64.shape[0] else gm) == 0
     got = y.cpu()
     want, tol = mx4ref.gemm(x64, w64, None, off, T, 1, False)
     assert mx4ref.close(got, want, tol)
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "mx4"])
-@pytest.mark.parametrize("size", list(SIZES))
-def test_the_largest_scales(ex, kind, size):  # noqa: F811
+@pytest.mark.parametrize("p", PATHS)
+def test_the_largest_scales(ex, kind, p):  # noqa: F811
     """Scale bytes up to 254 in some rows and blocks, x about 2^-12 (sums below 2^127): finite in 64 bits and in f32."""
-    T, E, N, K = SIZES[size]
-    print(f"moe_gemm {kind} {size}: scales 250 .. 254", flush=True)
+    T, E, n, N, K = size_of(kind, p)
+    print(f"moe_gemm {kind} path {p}: scales 250 .. 254", flush=True)
     g = torch.Generator().manual_seed(1)
-    s = torch.randint(250, 255, (E, N, K // 32), generator=g)
+    s = torch.randint(250, 255, (n, N, K // 32), generator=g)
     s[:, ::3] = torch.randint(118, 123, s[:, ::3].shape, generator=g)           # rows without them
     s[:, 1::3, 1::2] = torch.randint(100, 255, s[:, 1::3, 1::2].shape, generator=g)
-    wd, w64 = weights(ex, g, E, N, K, s)
-    xd, x64 = x_of(ex, torch.randn((T, K), generator=g) * 2.0 ** -12, kind, 0)
+    wd, w64 = gemmpath.mx4_weights(g, n, N, K, s)
+    xd, x64 = operand(ex, torch.randn((T, K), generator=g) * 2.0 ** -12, kind)
     check(ex, xd, x64, wd, w64, T, E)
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "mx4"])
-@pytest.mark.parametrize("size", list(SIZES))
-def test_zeros_of_x_at_the_largest_scales(ex, kind, size):  # noqa: F811
+@pytest.mark.parametrize("p", PATHS)
+def test_zeros_of_x_at_the_largest_scales(ex, kind, p):  # noqa: F811
     """Blocks of x that are zero against scales 252 .. 254: they add nothing, and the other blocks -- of ordinary scales, and of the
     smallest the format has -- make the sums."""
-    T, E, N, K = SIZES[size]
+    T, E, n, N, K = size_of(kind, p)
     g = torch.Generator().manual_seed(2)
     x = torch.randn((T, K // 32, 32), generator=g) * 64
     x[:, ::2] = 0
     for low, high in ((110, 130), (0, 3)):
-        print(f"moe_gemm {kind} {size}: zeros, scales {low} .. {high}", flush=True)
-        s = torch.randint(low, high, (E, N, K // 32), generator=g)
+        print(f"moe_gemm {kind} path {p}: zeros, scales {low} .. {high}", flush=True)
+        s = torch.randint(low, high, (n, N, K // 32), generator=g)
         s[:, :, ::2] = torch.randint(252, 255, s[:, :, ::2].shape, generator=g)
-        wd, w64 = weights(ex, g, E, N, K, s)
-        xd, x64 = x_of(ex, x.view(T, K), kind, 0)
+        wd, w64 = gemmpath.mx4_weights(g, n, N, K, s)
+        xd, x64 = operand(ex, x.view(T, K), kind)
         check(ex, xd, x64, wd, w64, T, E)
 
 
-@pytest.mark.parametrize("size", list(SIZES))
-def test_infinities_beside_the_largest_scales(ex, size):  # noqa: F811
+@pytest.mark.parametrize("p", PATHS)
+def test_infinities_beside_the_largest_scales(ex, p):  # noqa: F811
     """bf16 x with an infinity and a NaN, weights with a NaN block: what the definition gives, and no more."""
-    T, E, N, K = SIZES[size]
+    T, E, n, N, K = size_of("bf16", p)
     g = torch.Generator().manual_seed(3)
-    s = torch.randint(245, 255, (E, N, K // 32), generator=g)
+    s = torch.randint(245, 255, (n, N, K // 32), generator=g)
     s[:, 5, 2] = 255
-    wd, w64 = weights(ex, g, E, N, K, s)
+    wd, w64 = gemmpath.mx4_weights(g, n, N, K, s)
     x = torch.randn((T, K), generator=g) * 2.0 ** -14
     x[1, 7], x[2, K - 1], x[3, 40] = float("inf"), -float("inf"), float("nan")
     xd, x64 = operand(ex, x, "bf16")

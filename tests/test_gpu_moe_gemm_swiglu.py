@@ -6,6 +6,7 @@ most 9.8), exp2 and the reciprocal take 2 each, the sum and the products 1 each:
 output's own rounding, half its least step where it is subnormal."""
 import pytest
 
+import gemmpath
 import mx4ref
 from test_gpu_moe_gemm import PAIRS, TYPES, ex, operand  # noqa: F401 (ex is a fixture)
 
@@ -14,8 +15,16 @@ pytestmark = pytest.mark.gpu
 STEPS = 17 * 2.0 ** -24
 INF, NAN = float("inf"), float("nan")
 
-# (T, E): few rows an expert in narrow and wide workgroups, tiles of 32, 64, 128 and 256 rows (16-bit weights)
-SIZES = {"rows": (6, 2), "rows wide": (33, 33), "32": (90, 2), "64": (1100, 3), "128": (2000, 3), "256": (7200, 3)}
+# (T, experts) that take each kernel with some 1,000 columns of y: few rows by 2 and 4 strips, tiles of 32 to 256 rows
+SIZES = {2: (6, 2), 4: (33, 33), 32: (90, 2), 64: (1100, 3), 128: (2000, 3), 256: (16000, 3)}
+
+
+def takes(pair, p, n):
+    """Whether p is a path of the pair (at 32 columns of k MX4 x has no tiles of 256 rows), which the size then takes."""
+    if p not in gemmpath.paths(pair) or (pair[0] == "mx4" and p == 256):
+        return False
+    assert gemmpath.path(pair, True, *SIZES[p], n, 32) == p
+    return True
 
 
 def gates(pair):
@@ -53,14 +62,16 @@ def layer(ex, pair, T, E, g, u, yt):  # noqa: F811
 
 
 @pytest.mark.parametrize("pair", PAIRS, ids="-".join)
-@pytest.mark.parametrize("size", list(SIZES))
+@pytest.mark.parametrize("p", list(SIZES))
 @pytest.mark.parametrize("yt", ["f32", "bf16"])
-def test_gates_of_every_size(ex, pair, size, yt):  # noqa: F811
+def test_gates_of_every_size(ex, pair, p, yt):  # noqa: F811
     g, u = gates(pair)
     r = -(-1000 // len(g))
     g, u = g.repeat(r), u.repeat(r)                                    # some 1,000 columns, so that the sizes take their kernels
-    print(f"swiglu {pair} {size} {yt}: {len(g)} gates", flush=True)
-    got = layer(ex, pair, *SIZES[size], g, u, yt)
+    if not takes(pair, p, len(g)):
+        return
+    print(f"swiglu {pair} path {p} {yt}: {len(g)} gates", flush=True)
+    got = layer(ex, pair, *SIZES[p], g, u, yt)
     want = torch.nn.functional.silu(g.double()) * u.double()
     over = want.abs() >= 2.0 ** 128
     assert torch.equal(got[over].double(), torch.sign(want[over]) * INF)
@@ -70,15 +81,16 @@ def test_gates_of_every_size(ex, pair, size, yt):  # noqa: F811
 
 
 @pytest.mark.parametrize("pair", [p for p in PAIRS if p[1] != "mx4"], ids="-".join)
-@pytest.mark.parametrize("size", list(SIZES))
-def test_infinite_gates_and_what_is_beside_them(ex, pair, size):  # noqa: F811
+@pytest.mark.parametrize("p", list(SIZES))
+def test_infinite_gates_and_what_is_beside_them(ex, pair, p):  # noqa: F811
     """g / (1 + e^-g) u of infinities and NaNs, by IEEE's rules; the columns beside them as always."""
     g = torch.tensor([INF, INF, -INF, NAN, 2.0, -3.0, -120.0, 1.0, -65504.0, 60000.0]).repeat(100)
     u = torch.tensor([2.0, -3.0, 1.0, 1.0, INF, NAN, -INF, 0.5, 1024.0, 2.0]).repeat(100)
+    assert takes(pair, p, len(g))
     t = TYPES[pair[1]]
     g, u = g.to(t).float(), u.to(t).float()
     # a zero of x times an infinity is a NaN, so x has one column only that is not a weight's zero: K = 32, the others 0 x 0
-    got = layer(ex, pair, *SIZES[size], g, u, "f32")
+    got = layer(ex, pair, *SIZES[p], g, u, "f32")
     want = g.double() / (1 + torch.exp(-g.double())) * u.double()
     assert mx4ref.close(got, want, STEPS * want.abs().nan_to_num(0, 0, 0))
 
@@ -86,7 +98,7 @@ def test_infinite_gates_and_what_is_beside_them(ex, pair, size):  # noqa: F811
 def test_a_row_goes_by_itself(ex):  # noqa: F811
     """A row's bits do not change with the gates of the rows and columns beside it."""
     rng = torch.Generator().manual_seed(1)
-    for size, (T, E) in SIZES.items():
+    for p, (T, E) in SIZES.items():
         n, K = 1000, 32
         w = (torch.randn(1, 2 * n, K, generator=rng) / 4).bfloat16().repeat(E, 1, 1).cuda()
         x = torch.randn(T, K, generator=rng).bfloat16()
@@ -98,4 +110,4 @@ def test_a_row_goes_by_itself(ex):  # noqa: F811
             y = torch.zeros(T, n, device="cuda")
             assert ex.moe_gemm(ex.make_gemm(v.cuda(), w, None, off, y, act=ex.ACT_SWIGLU)) == 0
             got.append(y.cpu())
-        assert torch.equal(got[0][::2], got[1][::2]) and not torch.equal(got[0][1::2], got[1][1::2]), size
+        assert torch.equal(got[0][::2], got[1][::2]) and not torch.equal(got[0][1::2], got[1][1::2]), p
