@@ -3,6 +3,7 @@ every row of y is written once -- by its run's expert, or as zeros -- and every 
 import numpy as np
 import pytest
 
+import gemmpath
 import mx4ref
 from test_gpu_moe_gemm import PAIRS, ex, operand  # noqa: F401 (ex is a fixture)
 
@@ -26,8 +27,10 @@ def disjoint(off, T):
 
 
 @pytest.mark.parametrize("pair", PAIRS, ids="-".join)
-@pytest.mark.parametrize("E,T,N", [(6, 64, 40), (6, 400, 1450), (1500, 90, 36), (520, 4200, 160)], ids=str)
-def test_every_row_is_written_once(ex, pair, E, T, N):  # noqa: F811
+@pytest.mark.parametrize("E,T,N,tile", [(6, 64, 40, False), (6, 400, 1450, True), (1500, 90, 36, False), (520, 4200, 160, True)], ids=str)
+def test_every_row_is_written_once(ex, pair, E, T, N, tile):  # noqa: F811
+    """In few rows and in tiles, with more experts than one step of the search holds (512) as well."""
+    assert (gemmpath.path(pair, False, T, E, N, 64) > 4) == tile
     rng = np.random.default_rng(E + T)
     g = torch.Generator().manual_seed(T)
     K = 64
