@@ -321,10 +321,9 @@ __device__ __forceinline__ half8_t as_half8(uint32_t a, uint32_t b, uint32_t c, 
     return __builtin_bit_cast(half8_t, u32x4_t{ a, b, c, d });
 }
 
-// gfx950's v_mfma_f32_16x16x32_f16 still reads its A and B registers for some cycles after it issues, and the compiler
-// does not hold back a VALU or load that writes them meanwhile (measured: an address computed into a just-issued MFMA's
-// B registers corrupted the product). Every tile's MFMAs end with this guard: the scheduler may move nothing across
-// it, and its inputs keep the tile's operand registers allocated through 16 wait states after the last MFMA.
+// Keeps writes of a tile's A and B registers 16 wait states behind its last MFMA: the scheduler may move nothing across it, and its inputs keep
+// those registers allocated. (A precaution: a build without it, whose B operands were outputs of asm blocks, once gave wrong products where an
+// address was computed into them two instructions behind the MFMAs. The compiler's own MFMAs need none.)
 __device__ __forceinline__ void mfma_guard(const half8_t& a0, const half8_t& a1, const half8_t& b0, const half8_t& b1,
                                            const half8_t& b2, const half8_t& b3) {
     __builtin_amdgcn_sched_barrier(0);
