@@ -169,7 +169,6 @@ typedef struct Exl3c4DevGemm {
     int32_t        n_out;          /* y's columns: N, or N / 2 with SwiGLU */
     int32_t        y_type;
     int32_t        tiles;          /* column tiles of y */
-    int32_t        grid;           /* workgroups, where they take several units each */
 } Exl3c4DevGemm;
 int exl3c4_dev_gemm(const Exl3c4DevGemm* g, int32_t x_type, int32_t w_type, int32_t act, void* stream);
 /* which of its kernels such a launch takes (T > 0): a tile's rows, or for few rows an expert the strips of a workgroup (2 or 4) */

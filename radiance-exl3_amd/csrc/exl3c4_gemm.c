@@ -21,7 +21,7 @@ static int mx4_check(const void* codes, int64_t codes_pitch, const void* scales,
     if (!is_float(dtype)) return EXL3C4_E_DTYPE;
     if (rows < 0 || cols < 1 || rows > MAX_EXTENT || cols > MAX_EXTENT) return EXL3C4_E_SHAPE;
     const int64_t blocks = (cols + 31) / 32;
-    if (rows * blocks > ((int64_t)1 << 36)) return EXL3C4_E_SHAPE;      /* the grid's blocks in 31 bits */
+    if (rows * blocks > ((int64_t)1 << 36)) return EXL3C4_E_SHAPE;      /* 2^41 columns: past any memory */
     if (rows > 0 && (!codes || !scales || !v)) return EXL3C4_E_INVAL;
     if (pitch < cols || codes_pitch < 16 * blocks || scales_pitch < blocks) return EXL3C4_E_STRIDE;
     if (pitch > MAX_PITCH || codes_pitch > MAX_PITCH || scales_pitch > MAX_PITCH) return EXL3C4_E_STRIDE;
@@ -121,6 +121,6 @@ int exl3c4_moe_gemm(const Exl3c4Gemm* g, void* stream) {
     d.K = (int32_t)g->K;
     d.n_out = (int32_t)n_out;
     d.y_type = g->y_type;
-    d.tiles = d.grid = 0;                                     /* the launcher's */
+    d.tiles = 0;                                              /* the launcher's */
     return exl3c4_dev_gemm(&d, g->x_type, g->w_type, g->act, stream);
 }

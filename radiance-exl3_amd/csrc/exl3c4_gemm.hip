@@ -19,6 +19,7 @@
 #include <stdint.h>
 
 #include "exl3c4_dev.h"
+#include "exl3c4_wave.h"
 
 namespace {
 
@@ -42,17 +43,6 @@ __device__ __forceinline__ uint4 load_words(gaddr p) {
 }
 
 // ------------------------------------------------------------------------------------------ the rows of a workgroup
-// The inclusive sum of v over lanes 0 .. lane, by DPP (row shifts, then the rows' totals by row broadcasts).
-__device__ __forceinline__ int wave_scan_incl(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-
 // The largest v of lanes 0 .. lane - 1 (0 for lane 0; no v is below 0).
 __device__ __forceinline__ int wave_max_before(int v, int lane) {
     v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
