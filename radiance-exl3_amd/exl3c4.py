@@ -554,19 +554,26 @@ def mx4_empty(shape, device="cuda") -> Mx4:
                torch.empty((*lead, (nb + 3) // 4 * 4), dtype=torch.uint8, device=device), cols)
 
 
+_cuda = None                       # torch.cuda, from the first conversion on (an import statement a call is 0.1 us of 5)
+
+
 def _convert(fn, v, q: Mx4, stream, quant: bool) -> int:
     """One of the conversions between the rows of v and q (a small one is bound by what happens here: rows that follow each
     other need no look at the strides)."""
-    import torch
+    global _cuda
+    if _cuda is None:
+        import torch
+        _cuda = torch.cuda
     dev = v.get_device()
     if v.shape != q.shape or dev != q.device:
         raise ValueError("the values and q have other shapes or devices")
     n, pitch = (q.rows, q.cols) if v.is_contiguous() else _rows(v)
     cp, sp = q._pitches or q.pitches()
-    c, s = q.codes.data_ptr(), q.scales.data_ptr()
-    args = (v.data_ptr(), _dt(v), n, q.cols, pitch, c, cp, s, sp) if quant else \
-        (c, cp, s, sp, n, q.cols, v.data_ptr(), _dt(v), pitch)
-    if stream is not None and dev == torch.cuda.current_device():
+    c, s, dt = q.codes.data_ptr(), q.scales.data_ptr(), _dtypes.get(v.dtype)
+    if dt is None:
+        dt = _dt(v)
+    args = (v.data_ptr(), dt, n, q.cols, pitch, c, cp, s, sp) if quant else (c, cp, s, sp, n, q.cols, v.data_ptr(), dt, pitch)
+    if stream is not None and dev == _cuda.current_device():
         return fn(*args, stream.cuda_stream)
     return _launch_on(v.device, stream, fn, *args)
 
