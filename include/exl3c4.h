@@ -280,7 +280,8 @@ enum { EXL3C4_ACT_NONE = 0, EXL3C4_ACT_SWIGLU = 1 };
 /* x [rows, cols] (f16, bf16 or f32, rows x_pitch elements apart) to MX4: s = max(floor(log2(max |x| of the block)) - 2, -127)
  * + 127, codes x / 2^(s - 127) rounded to nearest, ties to the even code, magnitudes past 6 to 6. A block of zeros: s = 0. A block that
  * holds an infinity or a NaN: s = 255 and codes 0. Every code byte of a row's blocks and every scale byte of a block is written; pitch
- * bytes past them are left. Any x alignment that its elements have; codes 16-byte aligned, scales 4. */
+ * bytes past them are left. Any x alignment that its elements have; codes 16-byte aligned, scales 4. Values and planes share no memory,
+ * here and in mx4_dequant. */
 int exl3c4_mx4_quant(const void* x, int32_t x_dtype, int64_t rows, int64_t cols, int64_t x_pitch, void* codes,
                      int64_t codes_pitch, void* scales, int64_t scales_pitch, void* stream);
 

@@ -12,8 +12,8 @@
 // those two, whose larger elements pass 2^128, sums again, with a quarter of every weight, and takes four times that. f16 does not hold the scales' range: with f16 x a row's blocks are converted
 // relative to the largest scale among some hundred columns (its level), where those within 2^-13 of it are exact in f16, and the
 // sums are scaled in f32 as they are added; blocks further down, if any of them is not all zeros, have passes of their own. Either
-// way every product is exact. (Scaling each block's sums by itself, one matrix instruction a block, took 125 us where this
-// takes 64: 32 tokens, top-10 of 512 experts, gate and up 2048 -> 2 x 512.)
+// way every product is exact. (Scaling each block's sums by itself, one matrix instruction a block, took twice the time of levels when they were
+// chosen, 125 us against 64. 32 tokens, top-10 of 512 experts, gate and up 2048 -> 2 x 512 now: f16 x 75, bf16 x 57.)
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -345,9 +345,10 @@ __device__ __forceinline__ bool any_code(const uint4& q) { return ((q.x | q.y | 
 // ------------------------------------------------------------------------------------------ few rows an expert
 // A workgroup: a chunk of up to 16 rows against NS strips of 16 weight rows (with SwiGLU half of them gate rows and half their up
 // rows), each wave a part of k; the weights go from memory straight to the matrix units' operands, each byte read
-// once, and the parts' sums meet in LDS in a fixed order. Bound by latency for one token (512 experts, bf16 1024 x 2048: 13.2 us, of
-// which the 42 MB ask 6.7) and by memory beyond (f16 2048 x 512 at 8 tokens 32 us, 4.9 TB/s). Four waves and two steps' loads out
-// together: with four steps these take 14.4 and 36.8 us, with eight waves 13.7 and 42.5 (MX4 w, bf16 x, 32 tokens 60, 85 and 92).
+// once, and the parts' sums meet in LDS in a fixed order. Bound by latency for one token (512 experts, bf16 1024 x 2048: 12.0 us, of
+// which the 42 MB ask 6.7) and by memory beyond (f16 2048 x 512 at 8 tokens 32 us, 4.9 TB/s; MX4 w, bf16 x, 32 tokens 57 us, 4.7 TB/s, where the
+// VALU is busy 30% of the SIMDs' cycles and the matrix units 12%). Four waves and two steps' loads out together, chosen at 13.2, 32 and
+// 60 us for these: with four steps 14.4, 36.8 and 85, with eight waves 13.7, 42.5 and 92.
 constexpr int ROWS_LOG2 = 4;
 constexpr int WAVES = 4;
 
@@ -986,13 +987,17 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
 
 // Which kernel, and how large a tile: by the types, the sizes and the rows that an expert has at least on average, r = T / min(E, T)
 // -- never by the routing, which is on the device. Larger tiles read weights and rows less often; smaller ones waste
-// less of a chunk, make more workgroups and start sooner. Measured, us (E / top-k, N x K, tokens; SwiGLU where E > 1):
-//   rows against tiles     bf16 512/10 1024x2048: 32 tokens 179 / 248, 64 261 / 249, 200 373 / 338. MX4 64: 89 / 79, 200: 125 / 105.
-//                          bf16 x, MX4 w 64: 85 / 98, 200 118 / 133; 64/6 at 400 49 / 24. One expert, 77 rows 512x2048: 9.1 / 16.
-//   32 rows against 64     8/2 at 400 tokens: bf16 17.5 / 20.0, MX4 12.1 / 14.6; MX4 512/10 at 200 105 / 117, at 2048 Zipf 171 / 152.
-//   64 against 128         bf16 512/10 at 4096 522 / 409, 64/6 at 2000 113 / 95; MX4 193 / 175, 46 / 41; bf16 x, MX4 w 339 / 379.
-//   128 against 256        bf16 64/6 at 2000 95 / 85, 8/2 2816x2048 at 8192 225 / 190; MX4 64/6 at 2000 41 / 33, but K = 1408 at
-//                          8192 76 / 82 (few stages, and the larger tile's start and stores stand alone on its CU).
+// less of a chunk, make more workgroups and start sooner. Measured on one card, us with x's quantisation where x is MX4 (E / top-k, N x K, tokens; SwiGLU
+// where E > 1; "down": 2048 columns of y, sorted rows in):
+//   rows against tiles     bf16 512/10 1024x2048: 32 tokens 169 / 168, 64 256 / 248, 200 357 / 337. MX4 64: 84 / 78, 200 117 / 105.
+//                          bf16 x, MX4 w 64: 83 / 97, 200 116 / 131; 64/6 at 400 49 / 22. One expert, 77 rows 512x2048: 8.5 / 15.8.
+//   32 rows against 64     8/2 at 400 tokens: bf16 16.1 / 19.4, MX4 10.8 / 13.6; MX4 512/10 at 200 105 / 110, at 2048 Zipf 163 / 144; MX4 w at 4096:
+//                          bf16 x 317 / 302, f16 x 425 / 444 (its 64-row tiles hold 236 registers, two waves a SIMD).
+//   64 against 128         bf16 512/10 at 4096 518 / 412, 64/6 at 2000 107 / 94; MX4 184 / 167, 46 / 39; bf16 x, MX4 w 302 / 387 (not built).
+//   128 against 256        bf16 64/6 at 2000 94 / 85, 8/2 2816x2048 at 8192 224 / 186; MX4 64/6 at 2000 39 / 31, 8/2 2816x2048 at 8192 94 / 82.
+//                          MX4 by K, 8/2 at 8192: down 1024 60 / 63, 1408 72 / 77, 1792 80 / 83, 2048 91 / 91, 2560 99 / 105; 2816 with SwiGLU
+//                          1024 63 / 54, 1408 78 / 68, 1792 83 / 75, 2560 112 / 95: less the stages of a tile than how full the last of
+//                          the 256 CUs' two or three rounds is. The rule's K >= 2048 keeps a short K's down at 128 and gives up 8 to 10 us of its gate and up.
 // Returns a tile's rows (32, 64, 128, 256), or for few rows an expert the strips of a workgroup (2, 4).
 int choose(int x_type, int w_type, bool swiglu, int64_t T, int64_t n_expert, int64_t n_out, int64_t K) {
     const bool mixed = w_type == MX4 && x_type != MX4;
