@@ -9,11 +9,12 @@
 //
 // MX4 WEIGHTS AGAINST 16-BIT x. bf16 holds e2m1 x 2^s exactly for all but the two largest scales, so with bf16 x a lane's block is
 // converted with its scale (v_cvt_scalef32_pk_bf16_fp4) and multiplied as bf16; a wave (few rows) or a tile (many) that has met one of
-// those two, whose larger elements pass 2^128, sums again, with a quarter of every weight, and takes four times that. f16 does not hold the scales' range: with f16 x a row's blocks are converted
-// relative to the largest scale among some hundred columns (its level), where those within 2^-13 of it are exact in f16, and the
-// sums are scaled in f32 as they are added; blocks further down, if any of them is not all zeros, have passes of their own. Either
-// way every product is exact. (Scaling each block's sums by itself, one matrix instruction a block, took twice the time of levels when they were
-// chosen, 125 us against 64. 32 tokens, top-10 of 512 experts, gate and up 2048 -> 2 x 512 now: f16 x 75, bf16 x 57.)
+// those two, whose larger elements pass 2^128, sums again, with a quarter of every weight, and takes four times that. f16 does not hold
+// the scales' range: with f16 x a row's blocks are converted relative to the largest scale among some hundred columns (its level), where
+// those within 2^-13 of it are exact in f16, and the sums are scaled in f32 as they are added; blocks further down, if any of them is not
+// all zeros, have passes of their own. Either way every product is exact. (Scaling each block's sums by itself, one matrix instruction a
+// block, took twice the time of levels when they were chosen, 125 us against 64. 32 tokens, top-10 of 512 experts, gate and up
+// 2048 -> 2 x 512 now: f16 x 75, bf16 x 57.)
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
