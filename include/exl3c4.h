@@ -290,6 +290,33 @@ int exl3c4_mx4_quant(const void* x, int32_t x_dtype, int64_t rows, int64_t cols,
 int exl3c4_mx4_dequant(const void* codes, int64_t codes_pitch, const void* scales, int64_t scales_pitch, int64_t rows,
                        int64_t cols, void* out, int32_t out_dtype, int64_t out_pitch, void* stream);
 
+/* F8 (8-bit floats with a scale for each block of 128 columns): a matrix of rows x cols values as e4m3 codes, a byte a column (bit 7 the sign,
+ * bits 3..6 the exponent by 7, three bits of mantissa; subnormals of 2^-9; 448 the largest; 0x7F and 0xFF NaN), and one f32 scale for each block
+ * of `block` rows x 128 columns, block 1 (rows that are apart: activations) or 128 (weights): an element is its code's value times the scale. Blocks
+ * begin at row 0 and column 0 of the matrix; the last ones may be partly outside. n matrices, of codes codes_stride and of scales
+ * scales_stride apart. Codes of a row start codes_pitch bytes apart (a multiple of 16, at least cols rounded up to 16); the scales of a row of
+ * blocks start scales_pitch floats apart (at least ceil(cols / 128)); strides are in bytes for codes, in floats for scales. */
+enum { EXL3C4_F8 = 4 };                                       /* beside EXL3C4_MX4 */
+typedef struct Exl3c4F8 {
+    int64_t n, rows, cols;
+    int32_t block;                            /* 1 or 128 */
+    uint8_t* codes;
+    int64_t  codes_pitch, codes_stride;
+    float*   scales;
+    int64_t  scales_pitch, scales_stride;
+} Exl3c4F8;
+
+/* x (n matrices x_stride elements apart, rows x_pitch apart; f16, bf16 or f32) to F8. Of each block, with a = max(largest |x|, 2^-96) in f32:
+ * scale = a / 448, codes = x * (448 / a) to the nearest e4m3, ties to even, each of the two quotients and the product rounded once to f32. A block
+ * that holds an infinity or a NaN: scale NaN, codes 0. The codes of a row up to a multiple of 16 columns are written (zeros behind cols), and each
+ * block's scale; what lies behind them is left. Values and planes share no memory, here and in f8_dequant. Refusals, also f8_dequant's: INVAL (another
+ * block, a null pointer), DTYPE, SHAPE (extents below zero, cols below one, more than 2^31 rows in all, more than a launch holds), STRIDE, ALIGN
+ * (codes and their pitch and stride in 16s, values and scales to their type). */
+int exl3c4_f8_quant(const void* x, int32_t x_dtype, int64_t x_pitch, int64_t x_stride, const Exl3c4F8* q, void* stream);
+
+/* The values of F8 matrices as f16, bf16 or f32: code times scale in f32, rounded to nearest even. */
+int exl3c4_f8_dequant(const Exl3c4F8* q, void* out, int32_t out_dtype, int64_t out_pitch, int64_t out_stride, void* stream);
+
 /* moe_gemm: for each sorted row i of expert e's run [expert_offset[e], expert_offset[e + 1]),
  *     act NONE     y[i][n] = sum over k of W_e[n][k] x[r][k],                       n = 0 .. N - 1
  *     act SWIGLU   y[i][n] = silu(g) u, g = W_e[n] . x[r], u = W_e[N / 2 + n] . x[r],  n = 0 .. N / 2 - 1
@@ -298,13 +325,18 @@ int exl3c4_mx4_dequant(const void* codes, int64_t codes_pitch, const void* scale
  * them; offsets are clamped to [0, T], and one below an earlier offset counts as that one, so that every row belongs to one run at most
  * whatever the table holds. The same bits on every launch. (f16 x, MX4 w: where the scales of a weight row lie more than 2^13
  * apart, an infinity in x may give NaN where the sum is infinite.)
- *   x_type, w_type   F16, F16 | BF16, BF16 | F16, MX4 | BF16, MX4 | MX4, MX4
+ *   x_type, w_type   F16, F16 | BF16, BF16 | F16, MX4 | BF16, MX4 | MX4, MX4 | F16, F8 | BF16, F8 | F8, F8
  *   y_type           F16, BF16 or F32
  *   x   [x_rows, K], rows x_pitch apart: elements (16 bits) or bytes (MX4's codes, with x_scales xs_pitch bytes apart)
  *   w   expert e's [N, K] at w + e * w_stride bytes, or at ((void**)w)[e] where w_stride is 0; rows w_pitch apart, in the units of
  *       x_pitch; MX4: w_scales, ws_stride and ws_pitch likewise (ws_stride 0: a pointer array)
+ *       F8: x by blocks of one row (x_scales f32, xs_pitch bytes apart), w by blocks of 128 (w_scales f32, rows of blocks ws_pitch and experts
+ *       ws_stride bytes apart); with SWIGLU the gate half and the up half of W_e are matrices of their own, whose rows of blocks follow each
+ *       other: ceil(N / 2 / 128) of gate, then as many of up
+ *       F8 x and y of 16 bits: beside sums in f32, experts of many rows take the matrix unit's 8-bit products, which cut each of eight
+ *       neighbouring columns' products below 2^-13 of the largest of the eight (y in f32: every product is exact)
  *   y   [T, N or N / 2], y_pitch elements apart; shares no memory with the operands
- * 16-bit operands: K % 8 == 0, base, pitch and stride in multiples of 16 bytes; with an MX4 operand K % 32 == 0; scale bases, pitches
+ * 16-bit operands: K % 8 == 0, base, pitch and stride in multiples of 16 bytes; with an MX4 operand K % 32 == 0, with F8 K % 16 == 0; scale bases, pitches
  * and strides in multiples of 4 bytes. N is any. Refusals: INVAL (an unknown act, a required operand absent), DTYPE (another pair of
  * types), SHAPE (extents below one, K or N as above, fewer x rows than read, extents past 2^31 - 1 or more tiles than a launch holds),
  * STRIDE (a pitch or a stride below what it steps over, a weight's pitch past 2^27 bytes), ALIGN. */

@@ -173,10 +173,25 @@ typedef struct Exl3c4DevGemm {
 int exl3c4_dev_gemm(const Exl3c4DevGemm* g, int32_t x_type, int32_t w_type, int32_t act, void* stream);
 /* which of its kernels such a launch takes (T > 0): a tile's rows, or for few rows an expert the strips of a workgroup (2 or 4) */
 int exl3c4_dev_gemm_path(int32_t x_type, int32_t w_type, int32_t act, int64_t T, int64_t n_expert, int64_t N, int64_t K);
+/* F8 weights (exl3c4_gemm_f8.hip), and its path likewise */
+int exl3c4_dev_gemm_f8(const Exl3c4DevGemm* g, int32_t x_type, int32_t act, void* stream);
+int exl3c4_dev_gemm_f8_path(int32_t x_type, int32_t y_type, int32_t act, int64_t T, int64_t n_expert, int64_t N, int64_t K);
 int exl3c4_dev_mx4_quant(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t pitch, uint8_t* codes,
                          int64_t codes_pitch, uint8_t* scales, int64_t scales_pitch, void* stream);
 int exl3c4_dev_mx4_dequant(const uint8_t* codes, int64_t codes_pitch, const uint8_t* scales, int64_t scales_pitch,
                            int64_t rows, int64_t cols, void* out, int32_t dtype, int64_t out_pitch, void* stream);
+/* F8's conversions (exl3c4_f8.hip): n matrices of values and their planes; pitches and strides in bytes */
+typedef struct Exl3c4DevF8 {
+    char*    v;
+    uint8_t* codes;
+    float*   scales;
+    int64_t  v_pitch, v_stride, codes_pitch, codes_stride, scales_pitch, scales_stride;
+    uint32_t n, rows, cols;        /* n * rows fits 31 bits */
+    uint32_t code_cols;            /* cols up to a multiple of 16: the codes that a row has */
+    uint32_t block_log2;           /* a block's rows: 0 (one) or 7 (128) */
+} Exl3c4DevF8;
+int exl3c4_dev_f8_quant(const Exl3c4DevF8* a, int32_t dtype, void* stream);
+int exl3c4_dev_f8_dequant(const Exl3c4DevF8* a, int32_t dtype, void* stream);
 int exl3c4_dev_dequant(const void* record, int32_t rows, int32_t cols, int32_t bits, int32_t codebook, void* w_hat,
                        int64_t w_pitch, void* stream);
 

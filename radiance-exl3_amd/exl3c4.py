@@ -19,7 +19,7 @@ K_PREP, K_GATE_UP, K_EPI_GU, K_DOWN, K_GATE_UP_DOWN = 0, 1, 2, 3, 4
 GD_FUSE_MIN_T = 32                  # gate_up_down runs as one kernel at decode from this many sorted rows
 CB = {"3inst": 0, "mcg": 1, "mul1": 2}
 F16, BF16 = 0, 1
-MX4 = 3
+MX4, TYPE_F8 = 3, 4
 ACT_NONE, ACT_SWIGLU = 0, 1
 STATUS = {0: "OK", -1: "RAD_E_SHAPE", -2: "RAD_E_DTYPE", -3: "RAD_E_ALIGN", -4: "RAD_E_STRIDE", -9: "RAD_E_SCHEMA",
           -12: "RAD_E_INVAL", -18: "RAD_E_UNSUPPORTED", -20: "RAD_E_SCRATCH", -21: "RAD_E_DEVICE",
@@ -89,6 +89,60 @@ class Mx4:
         if self._pitches is None:
             super().__setattr__("_pitches", (_rows(self.codes)[1], _rows(self.scales)[1]))
         return self._pitches
+
+
+class F8Planes(C.Structure):
+    _fields_ = [("n", _i64), ("rows", _i64), ("cols", _i64), ("block", _i32), ("codes", _p), ("codes_pitch", _i64), ("codes_stride", _i64),
+                ("scales", _p), ("scales_pitch", _i64), ("scales_stride", _i64)]
+
+
+class F8:
+    """Matrices in 8-bit floats (include/exl3c4.h) of values [..., rows, cols]: codes uint8 or float8_e4m3fn [..., rows, >= cols rounded up to 16],
+    scales f32 [..., ceil(rows / block), >= ceil(cols / 128)], the columns they stand for and a block's rows: 1 (activations) or 128 (weights). The
+    weights of a SwiGLU product hold gate and up as matrices of their own, one behind the other: quantise them as values [..., 2, rows / 2, cols],
+    and view codes as [..., rows, cols] and scales as [..., 2 ceil(rows / 2 / 128), ...]. Its attributes are fixed, and the planes keep their sizes
+    and strides; where their memory is, is read at each call. Leading dimensions have to step evenly as one for the conversions (for moe_gemm they need
+    not)."""
+    __slots__ = ("codes", "scales", "cols", "block", "shape", "rows", "mats", "device", "_planes")
+
+    def __init__(self, codes, scales, cols: int, block: int):
+        if block not in (1, 128):
+            raise ValueError("a block has 1 or 128 rows")
+        rows = codes.shape[-2] if codes.dim() > 1 else 1
+        if codes.dim() < 2 or codes.dim() != scales.dim() or codes.shape[:-2] != scales.shape[:-2] or cols < 1 or codes.shape[-1] < (cols + 15) // 16 * 16 or \
+                scales.shape[-2] < (rows + block - 1) // block or scales.shape[-1] < (cols + 127) // 128 or codes.element_size() != 1 or \
+                scales.element_size() != 4 or not scales.is_floating_point() or codes.device != scales.device:
+            raise ValueError("the F8 planes do not fit each other or their columns")
+        put = super().__setattr__
+        put("codes", codes)
+        put("scales", scales)
+        put("cols", cols)
+        put("block", block)
+        put("shape", codes.shape[:-1] + (cols,))
+        put("rows", rows)
+        put("mats", codes.shape[:-2].numel())
+        put("device", codes.get_device())
+        put("_planes", None)
+
+    def __setattr__(self, name, *value):
+        raise AttributeError(f"{name} of an F8 is fixed: make another one")
+
+    __delattr__ = __setattr__
+
+    def __reduce__(self):                                      # copies and pickles: made of their own planes
+        return F8, (self.codes, self.scales, self.cols, self.block)
+
+    def planes(self):
+        """The C side's view of the planes as they are now."""
+        q = self._planes
+        if q is None:
+            if self.scales.shape[-2] != (self.rows + self.block - 1) // self.block:
+                raise ValueError("the scales have other rows of blocks than these rows: view gate and up as the two matrices that they are")
+            cm, sm = _matrices(self.codes), _matrices(self.scales)
+            q = F8Planes(self.mats, self.rows, self.cols, self.block, None, cm[0], cm[1], None, sm[0], sm[1])
+            super().__setattr__("_planes", q)
+        q.codes, q.scales = self.codes.data_ptr(), self.scales.data_ptr()
+        return q
 
 
 def lib():
@@ -163,6 +217,10 @@ def lib():
         L.exl3c4_mx4_quant.argtypes = [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]
         L.exl3c4_mx4_dequant.restype = C.c_int
         L.exl3c4_mx4_dequant.argtypes = [_p, _i64, _p, _i64, _i64, _i64, _p, _i32, _i64, _p]
+        L.exl3c4_f8_quant.restype = C.c_int
+        L.exl3c4_f8_quant.argtypes = [_p, _i32, _i64, _i64, C.POINTER(F8Planes), _p]
+        L.exl3c4_f8_dequant.restype = C.c_int
+        L.exl3c4_f8_dequant.argtypes = [C.POINTER(F8Planes), _p, _i32, _i64, _i64, _p]
         L.exl3c4_moe_gemm.restype = C.c_int
         L.exl3c4_moe_gemm.argtypes = [C.POINTER(Gemm), _p]
         L.exl3c4_build_target.restype = C.c_char_p
@@ -588,18 +646,72 @@ def mx4_dequant(q: Mx4, out, stream=None) -> int:
     return _convert(lib().exl3c4_mx4_dequant, out, q, stream, False)
 
 
-def _planes(t):
-    """(values or codes, scales or None, columns, type) of an operand of moe_gemm."""
+def _matrices(t):
+    """(pitch, stride) in elements of [..., rows, columns] whose leading dimensions step evenly as one."""
+    rows, cols = t.shape[-2:]
+    if cols > 1 and t.stride(-1) != 1:
+        raise ValueError("rows have to be contiguous")
+    pitch = t.stride(-2) if rows > 1 else max(t.stride(-2), cols)
+    if t.dim() == 2 or t.shape[:-2].numel() == 1:
+        return pitch, rows * pitch
+    return pitch, _rows(t.flatten(-2) if t.is_contiguous() else t[..., 0, :])[1]
+
+
+def f8_empty(shape, block: int, device="cuda") -> F8:
+    """Uninitialised F8 matrices for values of `shape` ([..., rows, cols]) in blocks of `block` (1 or 128) x 128."""
+    import torch
+    *lead, rows, cols = shape
+    return F8(torch.empty((*lead, rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=device),
+              torch.empty((*lead, (rows + block - 1) // block, (cols + 127) // 128), dtype=torch.float32, device=device), cols, block)
+
+
+def _convert_f8(fn, v, q: F8, stream, quant: bool) -> int:
+    """One of the conversions between the matrices of v and q."""
+    global _cuda
+    if _cuda is None:
+        import torch
+        _cuda = torch.cuda
+    dev = v.get_device()
+    if v.shape != q.shape or dev != q.device:
+        raise ValueError("the values and q have other shapes or devices")
+    pitch, stride = (q.cols, q.rows * q.cols) if v.is_contiguous() else _matrices(v)
+    dt = _dtypes.get(v.dtype)
+    if dt is None:
+        dt = _dt(v)
+    planes = C.byref(q.planes())
+    args = (v.data_ptr(), dt, pitch, stride, planes) if quant else (planes, v.data_ptr(), dt, pitch, stride)
+    if stream is not None and dev == _cuda.current_device():
+        return fn(*args, stream.cuda_stream)
+    return _launch_on(v.device, stream, fn, *args)
+
+
+def f8_quant(x, q: F8, stream=None) -> int:
+    """exl3c4_f8_quant of x [..., rows, cols] (f32 / f16 / bf16) into q; returns the status."""
+    return _convert_f8(lib().exl3c4_f8_quant, x, q, stream, True)
+
+
+def f8_dequant(q: F8, out, stream=None) -> int:
+    """exl3c4_f8_dequant of q into out [..., rows, cols] (f32 / f16 / bf16); returns the status."""
+    return _convert_f8(lib().exl3c4_f8_dequant, out, q, stream, False)
+
+
+def _planes(t, block):
+    """(values or codes, scales or None, columns, type) of an operand of moe_gemm, which takes F8 in blocks of `block` rows."""
     if isinstance(t, Mx4):
         return t.codes, t.scales, t.cols, MX4
+    if isinstance(t, F8):
+        if t.block != block:
+            raise ValueError("F8 x has blocks of one row, F8 w of 128")
+        return t.codes, t.scales, t.cols, TYPE_F8
     return t, None, t.shape[-1], _dt(t)
 
 
 def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT_NONE) -> Gemm:
-    """One moe_gemm: x [x_rows, K] and w [n_expert, N, K], each a 16-bit tensor or Mx4, sorted_tok i32 [T] (None: x holds
+    """One moe_gemm: x [x_rows, K] and w [n_expert, N, K], each a 16-bit tensor, Mx4 or F8 (x in blocks of 1, w of 128; with ACT_SWIGLU w's scales
+    are gate's rows of blocks, then up's), sorted_tok i32 [T] (None: x holds
     sorted rows), expert_offset i32 [n_expert + 1], y [T, N] ([T, N / 2] with ACT_SWIGLU) f16, bf16 or f32."""
-    xv, xs, K, xt = _planes(x)
-    wv, ws, Kw, wt = _planes(w)
+    xv, xs, K, xt = _planes(x, 1)
+    wv, ws, Kw, wt = _planes(w, 128)
     if xv.dim() != 2 or wv.dim() != 3 or y.dim() != 2:
         raise ValueError("x and y are rows, w one [N, K] an expert")
     g = Gemm()
@@ -609,6 +721,8 @@ def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT
     if Kw != K or y.shape[1] != (N // 2 if act == ACT_SWIGLU else N) or \
             expert_offset.numel() < E + 1:
         raise ValueError("x, w, expert_offset and y do not fit together")
+    if wt == TYPE_F8 and ws.shape[1] != (2 * ((N // 2 + 127) // 128) if act == ACT_SWIGLU else (N + 127) // 128):
+        raise ValueError("the scales of w have other rows of blocks than its rows (with ACT_SWIGLU: gate's, then up's)")
     for t, n in ((sorted_tok, g.T), (expert_offset, E + 1)):
         if t is not None and (t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous() or t.numel() < n):
             raise ValueError("sorted_tok and expert_offset are contiguous int32, of T and n_expert + 1 values at least")
@@ -626,13 +740,13 @@ def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT
         return t.stride(d) if t.shape[d] > 1 else max(t.stride(d), t.shape[-1])
 
     def stride(t):
-        return (t.stride(0) if E > 1 else N * pitch(t, 1)) * t.element_size()
+        return (t.stride(0) if E > 1 else t.shape[1] * pitch(t, 1)) * t.element_size()
     g.x, g.x_rows, g.x_pitch = xv.data_ptr(), xv.shape[0], pitch(xv, 0)
     g.w, g.w_pitch, g.w_stride = wv.data_ptr(), pitch(wv, 1), stride(wv)
     if xs is not None:
-        g.x_scales, g.xs_pitch = xs.data_ptr(), pitch(xs, 0)
+        g.x_scales, g.xs_pitch = xs.data_ptr(), pitch(xs, 0) * xs.element_size()
     if ws is not None:
-        g.w_scales, g.ws_pitch, g.ws_stride = ws.data_ptr(), pitch(ws, 1), stride(ws)
+        g.w_scales, g.ws_pitch, g.ws_stride = ws.data_ptr(), pitch(ws, 1) * ws.element_size(), stride(ws)
     g.sorted_tok = None if sorted_tok is None else sorted_tok.data_ptr()
     g.expert_offset, g.y, g.y_pitch = expert_offset.data_ptr(), y.data_ptr(), pitch(y, 0)
     g.device, g.tensors = y.device, (xv, xs, wv, ws, sorted_tok, expert_offset, y)     # alive as long as g
