@@ -255,6 +255,42 @@ int exl3c4_router_topk_scatter(const void* logits, int32_t logits_dtype, int64_t
                                int32_t* sorted_tok, int32_t* expert_offset, int32_t* expert_count, int32_t* row_of,
                                void* stream);
 
+/* moe_route: the router of layers that score by sigmoid or softmax, choose with a bias and within groups, and its scatter. Of each of n_tok
+ * tokens, with l its logits (row t at logits + t * pitch elements):
+ *     score      s_e = 1 / (1 + exp(-l_e)) (SIGMOID), or exp(l_e - m) over the sum of these (SOFTMAX; a NaN is left out of m and of the sum; of
+ *                several logits of +infinity each has one part)
+ *     choice     c_e = s_e + bias[e], or l_e where bias is null (the scores' own order). An expert whose logit is NaN or -infinity, or whose bias
+ *                is NaN or -infinity, is out: it is chosen in no case
+ *     groups     n_group runs of n_expert / n_group experts; a group's value is the largest s_e + bias[e] of its experts that are not out
+ *                (GROUP_MAX; by choice) or the sum of the two largest (GROUP_TOP2; of one expert its own). The top_group groups of the largest value
+ *                stay, ties to the lower group, those without an expert last
+ *     expert_ids i32 [n_tok][top_k]: the experts of the largest choice in the groups that stay, ties to the lower id, in that order;
+ *                -1 for each slot behind the last one that is not out
+ *     expert_w   f32 [n_tok][top_k]: their scores (0 of a slot with -1), divided by their sum where renorm is 1 (0 where that is 0), times scale
+ * All of it in 64 bits (the order of two experts as well), the weights rounded once.
+ * Where expert_offset is not null the pairs are scattered as well, as exl3c4_moe_scatter does with expert_base 0 (slots of -1 are dropped;
+ * expert_count and row_of may be null); up to 16 tokens in the same launch. Limits: 1 <= n_expert <= 1024, n_group divides n_expert, n_group <= 64,
+ * top_group <= n_group, top_k <= min(64, top_group * n_expert / n_group). Refusals before anything is written: INVAL (a null pointer, an unknown
+ * score, group_score or renorm, a scale that is not finite, scatter outputs without expert_offset, row_of that is expert_ids), DTYPE, SHAPE, UNSUPPORTED (n_expert > 1024), STRIDE, ALIGN.
+ * The outputs share no memory with the inputs or each other. */
+enum { EXL3C4_SCORE_SOFTMAX = 0, EXL3C4_SCORE_SIGMOID = 1 };
+enum { EXL3C4_GROUP_MAX = 0, EXL3C4_GROUP_TOP2 = 1 };
+typedef struct Exl3c4Route {
+    int32_t      logits_type, score, group_score, renorm;
+    int32_t      top_k, n_group, top_group;
+    float        scale;
+    int64_t      n_tok, n_expert, pitch;
+    const void*  logits;
+    const float* bias;                        /* [n_expert] or null */
+    int32_t*     expert_ids;
+    float*       expert_w;
+    int32_t*     sorted_tok;                  /* the scatter's, or null */
+    int32_t*     expert_offset;
+    int32_t*     expert_count;
+    int32_t*     row_of;
+} Exl3c4Route;
+int exl3c4_moe_route(const Exl3c4Route* r, void* stream);
+
 /* moe_gather: out[t][c] = f16( sum over slots s = 0 .. top_k-1 in ascending order, of the pairs with a row, of
  * expert_w[t][s] * y[row_of[t * top_k + s]][c] ), accumulated in f32 as one product and one add a slot (the north
  * star's layer output: the weighted sum in fp32, cast to fp16, round to nearest even). y: the down op's output rows,

@@ -152,6 +152,24 @@ int exl3c4_dev_scatter(const int32_t* ids, int64_t T, int64_t base, int32_t n_ex
 int exl3c4_dev_route_scatter(const void* logits, int32_t dtype, int32_t n_tok, int32_t n_expert, int64_t pitch,
                              int32_t top_k, int32_t renorm, int32_t* ids, float* w, int32_t* sorted, int32_t* off,
                              int32_t* count, int32_t* row_of, void* stream);
+typedef struct Exl3c4DevRoute {
+    const void*  logits;
+    const float* bias;
+    int32_t*     ids;
+    float*       w;
+    int32_t*     sorted;
+    int32_t*     off;
+    int32_t*     count;
+    int32_t*     row_of;
+    int64_t      n_tok, pitch;
+    int32_t      type, score, group_score, renorm, n_expert, top_k, n_group, top_group;
+    int32_t      group;            /* experts a group; group_inv: e * group_inv >> 20 = e / group for e < 1024 (group > 512 has one group) */
+    uint32_t     group_inv;
+    int32_t      part_log2;        /* the 2^part_log2 lanes that a group has of a wave */
+    float        scale;
+} Exl3c4DevRoute;
+/* moe_route's router; scatter: with the scatter, at most 16 tokens */
+int exl3c4_dev_score(const Exl3c4DevRoute* r, int scatter, void* stream);
 int exl3c4_dev_gather(const void* y, int32_t y_dtype, int64_t y_pitch, const float* w, const int32_t* row_of,
                       int64_t n_tok, int32_t top_k, int64_t cols, void* out, int64_t out_pitch, void* stream);
 /* the products of 16-bit and MX4 experts, and MX4's conversions (exl3c4_gemm.hip, exl3c4_mx4.hip) */

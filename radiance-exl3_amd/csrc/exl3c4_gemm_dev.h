@@ -275,13 +275,6 @@ __device__ __forceinline__ void dma4(gaddr from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
-// Orders the wave's LDS accesses before it and behind it, whichever of its lanes makes them. (The hardware does one wave's in order, so this
-// is no instruction: it holds the compiler, which sees one lane's accesses to places that another lane's do not touch.)
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 // Until at most N of the wave's loads are out, and none of its LDS reads.
 template <int N> __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);

@@ -1,6 +1,8 @@
 /* exl3c4_route.c -- the C-ABI entry points of the routing around the routed-expert ops (router, moe_scatter,
- * moe_gather; include/exl3c4.h): the refusals, before anything is written, then the device launch
+ * moe_route, moe_gather; include/exl3c4.h): the refusals, before anything is written, then the device launch
  * (exl3c4_route.hip). The contract is include/exl3_abi.h:90-158. */
+#include <math.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include "exl3c4.h"
@@ -75,6 +77,37 @@ int exl3c4_router_topk_scatter(const void* logits, int32_t logits_dtype, int64_t
     if (rc) return rc;
     return exl3c4_dev_scatter(expert_ids, n_tok * top_k, 0, (int32_t)n_expert, sorted_tok, expert_offset,
                               expert_count, row_of, stream);
+}
+
+int exl3c4_moe_route(const Exl3c4Route* r, void* stream) {
+    if (!r || (r->score != EXL3C4_SCORE_SOFTMAX && r->score != EXL3C4_SCORE_SIGMOID) ||
+        (r->group_score != EXL3C4_GROUP_MAX && r->group_score != EXL3C4_GROUP_TOP2) || !isfinite(r->scale))
+        return EXL3C4_E_INVAL;
+    int rc = router_check(r->logits, r->logits_type, r->n_tok, r->n_expert, r->pitch, r->top_k, r->renorm, r->expert_ids, r->expert_w);
+    if (rc) return rc;
+    if (r->n_group < 1 || r->n_group > 64 || r->n_expert % r->n_group || r->top_group < 1 || r->top_group > r->n_group ||
+        r->top_k > r->top_group * (r->n_expert / r->n_group))
+        return EXL3C4_E_SHAPE;
+    if ((uintptr_t)r->bias % 4) return EXL3C4_E_ALIGN;
+    const int scatter = r->expert_offset != NULL;
+    if (!scatter && (r->sorted_tok || r->expert_count || r->row_of)) return EXL3C4_E_INVAL;
+    if (scatter) {
+        if (r->row_of && r->row_of == r->expert_ids) return EXL3C4_E_INVAL;
+        rc = scatter_check(r->expert_ids, r->n_tok, r->top_k, r->n_expert, r->sorted_tok, r->expert_offset, r->expert_count, r->row_of, 1);
+        if (rc) return rc;
+    }
+    const int32_t  group = (int32_t)(r->n_expert / r->n_group);
+    Exl3c4DevRoute d = { .logits = r->logits, .bias = r->bias, .ids = r->expert_ids, .w = r->expert_w, .sorted = r->sorted_tok,
+                         .off = r->expert_offset, .count = r->expert_count, .row_of = r->row_of, .n_tok = r->n_tok, .pitch = r->pitch,
+                         .type = r->logits_type, .score = r->score, .group_score = r->group_score, .renorm = r->renorm,
+                         .n_expert = (int32_t)r->n_expert, .top_k = r->top_k, .n_group = r->n_group, .top_group = r->top_group,
+                         .group = group, .group_inv = ((1u << 20) + (uint32_t)group - 1u) / (uint32_t)group, .scale = r->scale };
+    for (int32_t lanes = 64; lanes / 2 >= r->n_group; lanes /= 2) ++d.part_log2;
+    if (scatter && r->n_tok <= FUSED_MAX_TOKENS) return exl3c4_dev_score(&d, 1, stream);
+    rc = exl3c4_dev_score(&d, 0, stream);
+    if (rc || !scatter) return rc;
+    return exl3c4_dev_scatter(r->expert_ids, r->n_tok * r->top_k, 0, (int32_t)r->n_expert, r->sorted_tok, r->expert_offset, r->expert_count,
+                              r->row_of, stream);
 }
 
 int exl3c4_moe_gather(const void* y, int32_t y_dtype, int64_t y_pitch, const float* expert_w, const int32_t* row_of,

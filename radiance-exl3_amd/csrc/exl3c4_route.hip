@@ -1,6 +1,7 @@
 // exl3c4_route.hip -- the routing around the routed-expert ops, on gfx950 (wave64): the router (softmax over all
 // logits, top_k, renormalisation), moe_scatter (a stable counting sort of the flat (token, slot) pairs by expert) and
-// moe_gather (each token's slots weighted and summed in f32, ascending slot order, cast to f16). The contract is
+// moe_gather (each token's slots weighted and summed in f32, ascending slot order, cast to f16); and moe_route, the router by scores, with a bias
+// and groups. The contract of the first three is
 // radiance's (include/exl3_abi.h:90-158; the scatter as tests/ref/exl3_numpy.py:223-242 states it); the reference
 // device library leaves these to its engine.
 #include <hip/hip_runtime.h>
@@ -370,6 +371,261 @@ __global__ __launch_bounds__(1024) void k_route_scatter(const void* logits, int3
     scatter_small(ids_l, n_tok * top_k, top_k, n_expert, sorted, off, count, row_of, cnt);
 }
 
+// ------------------------------------------------------------------------------------------ moe_route
+// The order of experts and of groups is decided in 64 bits: values of two experts that f32 could not tell apart are common among thousands of
+// tokens, and this card's f64 multiply-adds issue as fast as f32's. Every number behind the logits is f64, the weights are rounded once.
+
+// e^x for x <= 0 (below -800: 0): x = n ln 2 + r with ln 2 in two parts, |r| <= ln 2 / 2, and the exponential series up to r^13, whose rest is
+// below 2^-52 of e^r.
+__device__ __forceinline__ double exp64(double x) {
+    x = fmax(x, -800.0);
+    const double n = rint(x * 1.4426950408889634);
+    double r = fma(n, -6.93147180369123816490e-01, x);
+    r = fma(n, -1.90821492927058770002e-10, r);
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+// 1 / d for d in [1, 2^11]: the hardware's estimate (some 26 bits) and two steps of Newton's.
+__device__ __forceinline__ double inverse64(double d) {
+    double q = __builtin_amdgcn_rcp(d);
+    q = fma(fma(-d, q, 1.0), q, q);
+    return fma(fma(-d, q, 1.0), q, q);
+}
+__device__ __forceinline__ double sigmoid64(double l) {
+    const double t = exp64(-fabs(l)), q = inverse64(1.0 + t);
+    return l >= 0.0 ? q : t * q;
+}
+template <int J> __device__ __forceinline__ double xor_laned(double v, int lane) {
+    return __builtin_bit_cast(double, xor_lane64<J>(__builtin_bit_cast(uint64_t, v), lane));
+}
+__device__ __forceinline__ double wave_sum(double v, int lane) {
+    v += xor_laned<32>(v, lane);
+    v += xor_laned<16>(v, lane);
+    v += xor_laned<8>(v, lane);
+    v += xor_laned<4>(v, lane);
+    v += xor_laned<2>(v, lane);
+    return v + xor_laned<1>(v, lane);
+}
+// An order of doubles as unsigned numbers (-0 as +0); 0 stands for none.
+__device__ __forceinline__ uint64_t order64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
+    return u >> 63 ? ~u : u | (uint64_t)1 << 63;
+}
+__device__ __forceinline__ float logit(const Exl3c4DevRoute& a, int64_t at) {
+    if (a.type == EXL3C4_F32) return ((const float*)a.logits)[at];
+    const uint16_t b = ((const uint16_t*)a.logits)[at];
+    return a.type == EXL3C4_BF16 ? __uint_as_float((uint32_t)b << 16) : (float)__builtin_bit_cast(_Float16, b);
+}
+__device__ __forceinline__ bool is_out(float v) { return !(v > -INFINITY); }       // -infinity or NaN
+
+// One token by one wave: the experts e = lane + 64 j in registers. Lane r < top_k ends with the r-th expert and its weight. key, id: the wave's 64
+// places of LDS; value: its 64 RPL places (GROUPS).
+template <int RPL, bool GROUPS>
+__device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row, int lane, uint64_t* key, int* id, double* value) {
+    float l[RPL], b[RPL];
+    const int E = a.n_expert;
+    if (a.type == EXL3C4_F32) {
+        const float* p = (const float*)a.logits + row;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) l[j] = lane + 64 * j < E ? p[lane + 64 * j] : -INFINITY;
+    } else {
+        const uint16_t* p = (const uint16_t*)a.logits + row;
+        uint16_t h[RPL];
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) h[j] = lane + 64 * j < E ? p[lane + 64 * j] : a.type == EXL3C4_BF16 ? (uint16_t)0xFF80u : (uint16_t)0xFC00u;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) l[j] = a.type == EXL3C4_BF16 ? __uint_as_float((uint32_t)h[j] << 16) : (float)__builtin_bit_cast(_Float16, h[j]);
+    }
+    if (a.bias)
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) b[j] = lane + 64 * j < E ? a.bias[lane + 64 * j] : 0.f;
+    // softmax: the largest logit and the sum's inverse
+    const bool soft = a.score == EXL3C4_SCORE_SOFTMAX, top2 = GROUPS && a.group_score == EXL3C4_GROUP_TOP2;
+    double m = 0.0, inv = 1.0, s[RPL];
+    if (soft) {
+        float mf = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) mf = fmaxf(mf, l[j]);        // (a NaN never wins)
+        mf = fmaxf(mf, xor_lanef<32>(mf, lane));
+        mf = fmaxf(mf, xor_lanef<16>(mf, lane));
+        mf = fmaxf(mf, xor_lanef<8>(mf, lane));
+        mf = fmaxf(mf, xor_lanef<4>(mf, lane));
+        mf = fmaxf(mf, xor_lanef<2>(mf, lane));
+        mf = fmaxf(mf, xor_lanef<1>(mf, lane));
+        m = mf;
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) {
+            s[j] = is_out(l[j]) ? 0.0 : exp64(l[j] == mf ? 0.0 : (double)l[j] - m);      // (infinity - infinity is none)
+            sum += s[j];
+        }
+        inv = inverse64(fmax(wave_sum(sum, lane), 1.0));           // (1 at least, but for a row that is out as a whole)
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) s[j] *= inv;
+    } else if (a.bias || top2) {
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) s[j] = sigmoid64(l[j]);
+    }
+    uint64_t k[RPL];
+#pragma unroll
+    for (int j = 0; j < RPL; ++j) {
+        const double c = a.bias ? s[j] + (double)b[j] : (double)l[j];
+        k[j] = is_out(l[j]) || (a.bias && is_out(b[j])) ? 0 : order64(c);
+    }
+    if constexpr (GROUPS) {
+        // the values by expert through LDS; then 2^part_log2 lanes a group find its two largest
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) {
+            const double v = a.bias ? s[j] + (double)b[j] : top2 ? s[j] : (double)l[j];
+            value[lane + 64 * j] = k[j] ? v : -INFINITY;
+        }
+        wave_sync();
+        const int part = 1 << a.part_log2, g = lane >> a.part_log2;
+        double v1 = -INFINITY, v2 = -INFINITY;
+        if (g < a.n_group)
+            for (int i = lane & (part - 1); i < a.group; i += part) {
+                const double v = value[g * a.group + i];
+                v2 = fmax(v2, fmin(v1, v));
+                v1 = fmax(v1, v);
+            }
+        wave_sync();                                             // read before the next token's values
+        for (int d = 1; d < part; d <<= 1) {
+            const double o1 = __shfl_xor(v1, d), o2 = __shfl_xor(v2, d);
+            v2 = fmax(fmax(v2, o2), fmin(v1, o1));
+            v1 = fmax(v1, o1);
+        }
+        const double gv = top2 && v2 > -INFINITY ? v1 + v2 : v1;
+        const uint64_t gk = gv > -INFINITY ? order64(gv) : 0;
+        int ahead = 0;
+        for (int q = 0; q < a.n_group; ++q) {
+            const uint64_t o = readlane64(gk, q << a.part_log2);
+            ahead += o > gk || (o == gk && q < g) ? 1 : 0;
+        }
+        const uint64_t stay = __ballot(g < a.n_group && ahead < a.top_group);
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) {
+            const uint32_t of = (uint32_t)(lane + 64 * j) * a.group_inv >> 20;           // the expert's group (past the last expert: its key is 0)
+            if (!((stay >> ((of << a.part_log2) & 63)) & 1)) k[j] = 0;
+        }
+    }
+    // As in route_token: the top_k keys have a high word of at least thr, the top_k-th largest of the lanes' own largest; those candidates are gathered
+    // one a lane and ranked (equal keys by id), more than 64 of them by top_k rounds of a wave maximum.
+    uint64_t most = 0;
+#pragma unroll
+    for (int j = 0; j < RPL; ++j) most = k[j] > most ? k[j] : most;
+    const uint32_t thr = (uint32_t)__builtin_amdgcn_readlane((int)sort_desc32((uint32_t)(most >> 32), lane), a.top_k - 1);
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < RPL; ++j) {
+        const bool c = k[j] != 0 && (uint32_t)(k[j] >> 32) >= thr;
+        const uint64_t bal = __ballot(c);
+        const int at = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0));
+        if (c && at < 64) {
+            key[at] = k[j];
+            id[at] = lane + 64 * j;
+        }
+        n += __popcll(bal);
+    }
+    wave_sync();
+    int mine = -1;
+    if (n <= 64) {
+        const uint64_t ck = lane < n ? key[lane] : 0;
+        const int ce = lane < n ? id[lane] : 0x7FFFFFFF;
+        int rank = 0;
+        for (int c = 0; c < n; ++c) {
+            const uint64_t o = readlane64(ck, c);
+            const int oe = __builtin_amdgcn_readlane(ce, c);
+            rank += o > ck || (o == ck && oe < ce) ? 1 : 0;
+        }
+        wave_sync();
+        if (lane < n) id[rank] = ce;
+        wave_sync();
+        if (lane < n && lane < a.top_k) mine = id[lane];
+    } else {
+        uint64_t last = ~(uint64_t)0;
+        int last_id = -1;
+        for (int r = 0; r < a.top_k; ++r) {
+            uint64_t best = 0;
+            int at = 0x7FFFFFFF;                                 // (ids ascend with j: the first of equal keys is the lowest)
+#pragma unroll
+            for (int j = 0; j < RPL; ++j) {
+                const int e = lane + 64 * j;
+                if ((k[j] < last || (k[j] == last && e > last_id)) && k[j] > best) best = k[j], at = e;
+            }
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) {
+                const uint64_t o = shfl_xor64(best, d);
+                const int oe = __shfl_xor(at, d);
+                if (o > best || (o == best && oe < at)) best = o, at = oe;
+            }
+            last = best;
+            last_id = at;
+            if (lane == r && best != 0) mine = at;
+        }
+    }
+    wave_sync();                                                 // read before the next token's
+    double w = 0.0;
+    if (mine >= 0) {
+        const float v = logit(a, row + mine);
+        w = soft ? exp64(v == (float)m ? 0.0 : (double)v - m) * inv : sigmoid64(v);
+    }
+    if (a.renorm) {
+        const double sum = wave_sum(w, lane);
+        w = sum > 0.0 ? w / sum : 0.0;
+    }
+    return Pick{ mine, (float)(w * (double)a.scale) };
+}
+
+// A wave a token.
+template <int RPL, bool GROUPS>
+__global__ __launch_bounds__(256) void k_score(Exl3c4DevRoute a) {
+    __shared__ uint64_t key[4][64];
+    __shared__ int id[4][64];
+    __shared__ double value[4][GROUPS ? 64 * RPL : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    if (t >= a.n_tok) return;
+    const Pick p = score_token<RPL, GROUPS>(a, t * a.pitch, lane, key[wave], id[wave], value[wave]);
+    if (lane < a.top_k) {
+        a.ids[t * a.top_k + lane] = p.id;
+        a.w[t * a.top_k + lane] = p.w;
+    }
+}
+
+// With the scatter, for at most 16 tokens, in one workgroup (as k_route_scatter).
+template <int RPL, bool GROUPS>
+__global__ __launch_bounds__(1024) void k_score_scatter(Exl3c4DevRoute a) {
+    __shared__ uint64_t key[16][64];
+    __shared__ int id[16][64];
+    __shared__ double value[16][GROUPS ? 64 * RPL : 1];
+    __shared__ int ids_l[16 * 64], cnt[64 * RPL + 17];
+    const int lane = threadIdx.x & 63, t = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < a.n_expert; i += blockDim.x) cnt[i] = 0;
+    if (t < a.n_tok) {
+        const Pick p = score_token<RPL, GROUPS>(a, (int64_t)t * a.pitch, lane, key[t], id[t], value[t]);
+        if (lane < a.top_k) {
+            a.ids[t * a.top_k + lane] = p.id;
+            a.w[t * a.top_k + lane] = p.w;
+            ids_l[t * a.top_k + lane] = p.id;
+        }
+    }
+    __syncthreads();
+    scatter_small(ids_l, (int)a.n_tok * a.top_k, a.top_k, a.n_expert, a.sorted, a.off, a.count, a.row_of, cnt);
+}
+
 // moe_gather: one thread a run of 8 columns of one token; the slots in ascending order, one f32 product and one add
 // each, then f16. The rows and weights of 8 slots are read together, then their rows' values.
 __global__ __launch_bounds__(256) void k_gather(const void* y, int32_t y_dtype, int64_t y_pitch, const float* w,
@@ -489,6 +745,32 @@ extern "C" int exl3c4_dev_route_scatter(const void* logits, int32_t dtype, int32
         launch_rs_dt<EXL3C4_BF16>(logits, n_tok, n_expert, pitch, top_k, renorm, ids, w, sorted, off, count, row_of, lds, st);
     else
         launch_rs_dt<EXL3C4_F16>(logits, n_tok, n_expert, pitch, top_k, renorm, ids, w, sorted, off, count, row_of, lds, st);
+    return launched();
+}
+
+namespace {
+
+template <int RPL, bool GROUPS>
+void launch_score(const Exl3c4DevRoute& a, bool scatter, hipStream_t st) {
+    if (scatter) hipLaunchKernelGGL((k_score_scatter<RPL, GROUPS>), dim3(1), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((k_score<RPL, GROUPS>), dim3((unsigned)((a.n_tok + 3) / 4)), dim3(256), 0, st, a);
+}
+template <int RPL>
+void launch_score(const Exl3c4DevRoute& a, bool scatter, hipStream_t st) {
+    if (a.n_group > 1 && a.top_group < a.n_group) launch_score<RPL, true>(a, scatter, st);
+    else launch_score<RPL, false>(a, scatter, st);
+}
+
+}  // namespace
+
+extern "C" int exl3c4_dev_score(const Exl3c4DevRoute* r, int scatter, void* stream) {
+    const hipStream_t st = (hipStream_t)stream;
+    if (r->n_tok <= 0 && !scatter) return 0;
+    if (r->n_expert <= 64) launch_score<1>(*r, scatter, st);
+    else if (r->n_expert <= 128) launch_score<2>(*r, scatter, st);
+    else if (r->n_expert <= 256) launch_score<4>(*r, scatter, st);
+    else if (r->n_expert <= 512) launch_score<8>(*r, scatter, st);
+    else launch_score<16>(*r, scatter, st);
     return launched();
 }
 

@@ -21,6 +21,8 @@ CB = {"3inst": 0, "mcg": 1, "mul1": 2}
 F16, BF16 = 0, 1
 MX4, TYPE_F8 = 3, 4
 ACT_NONE, ACT_SWIGLU = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
 STATUS = {0: "OK", -1: "RAD_E_SHAPE", -2: "RAD_E_DTYPE", -3: "RAD_E_ALIGN", -4: "RAD_E_STRIDE", -9: "RAD_E_SCHEMA",
           -12: "RAD_E_INVAL", -18: "RAD_E_UNSUPPORTED", -20: "RAD_E_SCRATCH", -21: "RAD_E_DEVICE",
           -5: "RAD_E_FORMAT", -30: "RAD_E_NOTFOUND", -31: "RAD_E_IO"}
@@ -54,6 +56,12 @@ class Gemm(C.Structure):
                 ("x", _p), ("x_scales", _p), ("x_rows", _i64), ("x_pitch", _i64), ("xs_pitch", _i64),
                 ("w", _p), ("w_scales", _p), ("w_pitch", _i64), ("ws_pitch", _i64), ("w_stride", _i64),
                 ("ws_stride", _i64), ("sorted_tok", _p), ("expert_offset", _p), ("y", _p), ("y_pitch", _i64)]
+
+
+class Route(C.Structure):
+    _fields_ = [("logits_type", _i32), ("score", _i32), ("group_score", _i32), ("renorm", _i32), ("top_k", _i32), ("n_group", _i32),
+                ("top_group", _i32), ("scale", C.c_float), ("n_tok", _i64), ("n_expert", _i64), ("pitch", _i64), ("logits", _p), ("bias", _p),
+                ("expert_ids", _p), ("expert_w", _p), ("sorted_tok", _p), ("expert_offset", _p), ("expert_count", _p), ("row_of", _p)]
 
 
 class Mx4:
@@ -223,6 +231,8 @@ def lib():
         L.exl3c4_f8_dequant.argtypes = [C.POINTER(F8Planes), _p, _i32, _i64, _i64, _p]
         L.exl3c4_moe_gemm.restype = C.c_int
         L.exl3c4_moe_gemm.argtypes = [C.POINTER(Gemm), _p]
+        L.exl3c4_moe_route.restype = C.c_int
+        L.exl3c4_moe_route.argtypes = [C.POINTER(Route), _p]
         L.exl3c4_build_target.restype = C.c_char_p
         L.exl3c4_abi_version.restype = C.c_int
         _lib = L
@@ -756,6 +766,39 @@ def make_gemm(x, w, sorted_tok, expert_offset, y, top_k: int = 1, act: int = ACT
 def moe_gemm(g: Gemm, stream=None) -> int:
     """exl3c4_moe_gemm on the device of g's tensors; returns the status."""
     return _launch_on(g.device, stream, lib().exl3c4_moe_gemm, C.byref(g))
+
+
+# ------------------------------------------------------------------------------------------ routing by scores
+def make_route(logits, top_k: int, ids, w, score: int = SCORE_SOFTMAX, bias=None, n_group: int = 1, top_group: int = 1,
+               group_score: int = GROUP_MAX, renorm: bool = True, scale: float = 1.0, sorted_tok=None, expert_offset=None, expert_count=None,
+               row_of=None) -> Route:
+    """One moe_route: logits [n_tok, n_expert] (f32 / f16 / bf16), ids i32 and w f32 [n_tok, top_k] out, bias f32 [n_expert] or None; with
+    expert_offset i32 [n_expert + 1] the scatter as well (sorted_tok i32 [n_tok top_k]; expert_count i32 [n_expert] and row_of i32
+    [n_tok top_k] or None)."""
+    import torch
+    if logits.dim() != 2:
+        raise ValueError("logits are [n_tok, n_expert]")
+    n_tok, n_expert = logits.shape
+    if n_expert > 1 and logits.stride(1) != 1:
+        raise ValueError("rows have to be contiguous")
+    for t, n, dt in ((ids, n_tok * top_k, torch.int32), (w, n_tok * top_k, torch.float32), (bias, n_expert, torch.float32),
+                     (sorted_tok, n_tok * top_k, torch.int32), (expert_offset, n_expert + 1, torch.int32), (expert_count, n_expert, torch.int32),
+                     (row_of, n_tok * top_k, torch.int32)):
+        if t is not None and (t.dtype != dt or not t.is_contiguous() or t.numel() < n or t.device != logits.device):
+            raise ValueError("ids, sorted_tok, expert_offset, expert_count and row_of are contiguous int32, w and bias float32, of their sizes and on "
+                             "the logits' device")
+    if tuple(ids.shape) != (n_tok, top_k) or tuple(w.shape) != (n_tok, top_k):
+        raise ValueError("ids and w are [n_tok, top_k]")
+    r = Route(_dt(logits), score, group_score, int(renorm), top_k, n_group, top_group, scale, n_tok, n_expert,
+              logits.stride(0) if n_tok > 1 else max(logits.stride(0), n_expert), *(None if t is None else t.data_ptr() for t in (
+                  logits, bias, ids, w, sorted_tok, expert_offset, expert_count, row_of)))
+    r.device, r.tensors = logits.device, (logits, bias, ids, w, sorted_tok, expert_offset, expert_count, row_of)     # alive as long as r
+    return r
+
+
+def moe_route(r: Route, stream=None) -> int:
+    """exl3c4_moe_route on the device of r's tensors; returns the status."""
+    return _launch_on(r.device, stream, lib().exl3c4_moe_route, C.byref(r))
 
 
 def alloc_scratch(o: Op, device="cuda"):

@@ -1,0 +1,184 @@
+"""moe_route on the device against its definition in 64 bits (tests/routeref.py): experts equal, in order and with ties, the scatter equal, weights
+within their one rounding to f32 (what is behind it is in f64, some 2^-45 off at most)."""
+import numpy as np
+import pytest
+
+import routeref
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def ex():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import exl3c4
+    exl3c4.lib()
+    return exl3c4
+
+
+def outputs(n_tok, E, top_k, spare=3):
+    """(ids, w, sorted_tok, offset, count, row_of) as the routing writes them, each with guards behind."""
+    i32 = lambda n: torch.full((n + spare,), -77, dtype=torch.int32, device="cuda")
+    return (i32(n_tok * top_k), torch.full((n_tok * top_k + spare,), -77.0, device="cuda"), i32(n_tok * top_k), i32(E + 1), i32(E), i32(n_tok * top_k))
+
+
+def check(ex, l, top_k, score="sigmoid", bias=None, n_group=1, top_group=1, group="max", renorm=True, scale=1.0, scatter=True, stream=None):
+    """l [n_tok, n_expert] on the device, of any pitch."""
+    n_tok, E = l.shape
+    ids, w, st, off, cnt, row = outputs(n_tok, E, top_k)
+    more = dict(sorted_tok=st, expert_offset=off, expert_count=cnt, row_of=row) if scatter else {}
+    n = n_tok * top_k
+    r = ex.make_route(l, top_k, ids[:n].view(n_tok, top_k), w[:n].view(n_tok, top_k), score=ex.SCORE_SIGMOID if score == "sigmoid" else ex.SCORE_SOFTMAX,
+                      bias=bias, n_group=n_group, top_group=top_group, group_score=ex.GROUP_TOP2 if group == "top2" else ex.GROUP_MAX, renorm=renorm,
+                      scale=scale, **more)
+    assert ex.moe_route(r, stream) == 0
+    torch.cuda.synchronize()
+    wi, ww = routeref.route(l.float().cpu().numpy(), top_k, score, None if bias is None else bias.cpu().numpy(), n_group, top_group, group, renorm, scale)
+    gi, gw = ids[:n].view(n_tok, top_k).cpu().numpy(), w[:n].view(n_tok, top_k).cpu().numpy().astype(np.float64)
+    assert np.array_equal(gi, wi), (np.argwhere(gi != wi)[:5], gi[(gi != wi).any(1)][:2], wi[(gi != wi).any(1)][:2])
+    assert (np.abs(gw - ww) <= 2.0 ** -24 * (1 + 2.0 ** -18) * np.abs(ww) + 2.0 ** -150).all()
+    assert (ids[n:] == -77).all() and (w[n:] == -77).all()
+    if scatter:
+        for got, want in zip((st, off, cnt, row), routeref.scatter(wi, E)):
+            assert np.array_equal(got[:len(want)].cpu().numpy(), want) and (got[len(want):] == -77).all()
+    return gi, gw
+
+
+CASES = [  # n_tok, n_expert, top_k, n_group, top_group
+    (1, 1, 1, 1, 1), (1, 256, 8, 8, 4), (3, 8, 2, 1, 1), (16, 20, 5, 5, 2), (17, 20, 20, 5, 5), (5, 64, 6, 64, 8), (16, 64, 1, 2, 1), (33, 160, 6, 8, 3),
+    (300, 256, 8, 8, 4), (20, 384, 64, 16, 8), (64, 512, 10, 1, 1), (9, 512, 10, 4, 2), (40, 1000, 7, 10, 3), (16, 1024, 64, 2, 1), (70, 1024, 33, 64, 40),
+    (4, 66, 3, 33, 2)]
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_sizes(ex, case, score):
+    n_tok, E, top_k, n_group, top_group = case
+    print(f"route {case} {score}", flush=True)
+    g = torch.Generator().manual_seed(E + n_tok)
+    l = torch.randn((n_tok, E), generator=g) * 2
+    bias = (torch.randn(E, generator=g) * (0.2 if score == "sigmoid" else 1 / E)).cuda()
+    for b in (None, bias):
+        for group in (("max", "top2") if n_group > 1 else ("max",)):
+            check(ex, l.cuda(), top_k, score, b, n_group, top_group, group, renorm=b is None, scale=2.5, scatter=group == "max")
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("n_tok", [1, 16, 50])
+def test_types_pitches_and_alignment(ex, t, n_tok):
+    """Logits of each type from an odd element on, rows apart by an odd pitch; in 16 bits equal ones are common."""
+    buf = (torch.randn(40000, generator=torch.Generator().manual_seed(n_tok)) * 1.5).to(TYPES[t]).cuda()
+    l = buf[1:].as_strided((n_tok, 192), (301, 1))
+    bias = torch.round(torch.randn(192, generator=torch.Generator().manual_seed(2)) * 4).cuda() / 4
+    for score in ("sigmoid", "softmax"):
+        check(ex, l, 8, score)
+        check(ex, l, 8, score, n_group=6, top_group=2, group="top2")
+        check(ex, l, 8, score, bias, 6, 2, "top2")
+
+
+def test_ties_go_to_the_lower_id(ex):
+    """Equal logits (all of them: more candidates than a wave holds), equal biases, equal groups, zeros of both signs."""
+    for n_tok in (2, 30):
+        l = torch.zeros(n_tok, 300, device="cuda")
+        gi, gw = check(ex, l, 40)
+        assert (gi == np.arange(40)).all()
+        check(ex, l, 40, bias=torch.full((300,), 0.3, device="cuda"))
+        check(ex, l, 12, n_group=30, top_group=2, group="top2")
+        l[:, ::2] = -0.0
+        check(ex, l, 64, "softmax")
+        l = torch.randint(-2, 3, (n_tok, 300), generator=torch.Generator().manual_seed(1)).float().cuda()
+        check(ex, l, 64)
+        check(ex, l, 20, bias=(torch.arange(300) % 3).float().cuda() / 8)
+        check(ex, l, 9, "softmax", n_group=20, top_group=3, group="top2")
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_values_that_32_bits_do_not_tell_apart(ex, score):
+    """Biases that bring the choices of all experts within some 2^-28 of each other, and groups' sums too."""
+    g = torch.Generator().manual_seed(5)
+    l = torch.randn((40, 256), generator=g)
+    s = torch.sigmoid(l.double()) if score == "sigmoid" else torch.softmax(l.double(), 1)
+    for n_group, group in ((1, "max"), (8, "max"), (8, "top2")):
+        for t in range(0, 40, 8):
+            check(ex, l[t:t + 1].cuda(), 8, score, (0.75 - s[t]).float().cuda(), n_group, max(1, n_group // 2), group)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("n_tok", [7, 40])
+def test_experts_that_are_out(ex, score, n_tok):
+    """-infinity and NaN in logits and biases: rows without an expert, groups without one, fewer experts than slots, one expert in a group."""
+    g = torch.Generator().manual_seed(n_tok)
+    l = torch.randn((n_tok, 96), generator=g)
+    l[0] = -float("inf")
+    l[1] = float("nan")
+    l[2, 3:] = -float("inf")
+    l[3, :90] = float("nan")
+    l[4][torch.rand(96, generator=g) < 0.9] = -float("inf")
+    l[5, 12:24] = -float("inf")
+    l[6, 0:11] = float("nan")
+    bias = torch.randn(96, generator=g) * 0.1
+    bias[7], bias[8], bias[24:36] = -float("inf"), float("nan"), -float("inf")
+    for b in (None, bias.cuda()):
+        for n_group, top_group, group in ((1, 1, "max"), (8, 3, "max"), (8, 3, "top2"), (8, 8, "top2")):
+            for renorm in (False, True):
+                gi, gw = check(ex, l.cuda(), 6, score, b, n_group, top_group, group, renorm, 1.5)
+                assert (gi[:2] == -1).all() and (gw[gi < 0] == 0).all()
+    check(ex, torch.full((n_tok, 96), -float("inf"), device="cuda"), 6, score)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_infinities_and_far_logits(ex, score):
+    """+infinity (once, several times), logits far beyond where a score leaves f32 and f64, a bias of +infinity."""
+    l = torch.randn((20, 64), generator=torch.Generator().manual_seed(3))
+    l[0, 9] = float("inf")
+    l[1, 5:8] = float("inf")
+    l[2] *= 1e30
+    l[3] -= 200.0
+    l[4] -= 2000.0
+    l[5] += 3e38
+    l[6] *= 30
+    for renorm in (False, True):
+        check(ex, l.cuda(), 5, score, renorm=renorm)
+    b = torch.zeros(64)
+    b[40] = float("inf")
+    check(ex, l[6:].cuda(), 5, score, b.cuda(), 4, 2, "max")
+
+
+def test_no_tokens_and_one_expert(ex):
+    for top in (1, 3):
+        l = torch.zeros(0, 64, device="cuda")
+        off = torch.full((65,), 9, dtype=torch.int32, device="cuda")
+        ids, w = torch.zeros(0, top, dtype=torch.int32, device="cuda"), torch.zeros(0, top, device="cuda")
+        assert ex.moe_route(ex.make_route(l, top, ids, w, expert_offset=off, sorted_tok=ids.view(-1))) == 0
+        assert (off == 0).all()
+    check(ex, torch.tensor([[-3.0]]).cuda(), 1, "softmax")
+
+
+def test_streams_and_a_replayed_graph(ex):
+    """On a stream of the caller's, two routings at once, and captured (16 tokens: one launch, 40: two), replayed on new logits."""
+    st = torch.cuda.Stream()
+    l = torch.randn(40, 256, device="cuda")
+    st.wait_stream(torch.cuda.current_stream())
+    check(ex, l, 8, n_group=8, top_group=4, group="top2", stream=st)
+    for n_tok in (16, 40):
+        ids, w, so, off, cnt, row = outputs(n_tok, 256, 8, 0)
+        r = ex.make_route(l[:n_tok], 8, ids.view(n_tok, 8), w.view(n_tok, 8), score=ex.SCORE_SIGMOID, n_group=8, top_group=4, group_score=ex.GROUP_TOP2,
+                          sorted_tok=so, expert_offset=off, row_of=row)
+        assert ex.moe_route(r) == 0
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            assert ex.moe_route(r) == 0
+        for seed in range(3):
+            l.copy_(torch.randn(l.shape, generator=torch.Generator().manual_seed(seed)))
+            for o in (ids, so, off, row):
+                o.fill_(-5)
+            graph.replay()
+            torch.cuda.synchronize()
+            wi, _ = routeref.route(l[:n_tok].cpu().numpy(), 8, "sigmoid", None, 8, 4, "top2")
+            want = routeref.scatter(wi, 256)
+            assert np.array_equal(ids.view(n_tok, 8).cpu().numpy(), wi)
+            assert np.array_equal(so.cpu().numpy(), want[0]) and np.array_equal(off.cpu().numpy(), want[1]) and np.array_equal(row.cpu().numpy(), want[3])
