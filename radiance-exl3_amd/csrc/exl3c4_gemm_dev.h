@@ -274,6 +274,13 @@ __device__ __forceinline__ void dma16(gaddr from, uint32_t lds) {
 __device__ __forceinline__ void dma4(gaddr from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
+// The same where `all` is -1, and nothing where it is 0 (uniform; the whole wave is active): no lane loads, without a branch.
+__device__ __forceinline__ void dma16_of(gaddr from, uint32_t lds, int all) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dwordx4 %0, off\n\ts_mov_b64 exec, -1" ::"v"(from), "s"(lds), "s"(all) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4_of(gaddr from, uint32_t lds, int all) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1" ::"v"(from), "s"(lds), "s"(all) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 // Until at most N of the wave's loads are out, and none of its LDS reads.
 template <int N> __device__ __forceinline__ void wait_loads() {

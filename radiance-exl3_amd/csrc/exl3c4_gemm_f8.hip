@@ -204,33 +204,36 @@ __global__ __launch_bounds__(64 * WAVES) void k_f8_rows(Exl3c4DevGemm a) {
 
 // ------------------------------------------------------------------------------------------ many rows an expert
 // A workgroup: a tile of MT rows of one expert against NT weight rows (with SwiGLU 16 gate rows and their 16 up rows in turn, so that a lane holds
-// both), k in stages of one block of 128 columns. A stage's rows and scales go from memory to LDS without registers, BUFS - 1 stages ahead of the
-// products; a wave waits for its own loads by count, and one barrier a stage both publishes them and frees the buffer that the next ones fill.
+// both), k in stages of one block of 128 columns. A stage's rows and scales go from memory to LDS without registers. A wave reads its weight rows into
+// registers at the start of a stage and then uses them for all its rows of x, so one place for weights is enough: once every wave has read them
+// (a barrier among the products) the next stage's come in under the rest of the products. x has XB places, XB - 1 stages ahead. So a workgroup's LDS stays
+// small and a CU holds several, one at its start or end under another's products.
 //
 // LDS. A row of a stage is 128 bytes (16-bit x: two such halves). The loads write lane after lane, 16 bytes each, so the order within a row is chosen
 // at the source: place p of row r holds the chunk p ^ (r & 7), and the 16 rows and four lane groups that read a matrix operand fall on all the
-// banks evenly. Behind them the scales: one of each row of x, and those of the tile's blocks of weight rows.
+// banks evenly. Behind x's rows a scale for each; behind the weights' those of the tile's blocks of weight rows.
 //
 // Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, so that a sum's scale is one number of the
 // lane's row of x times one that the wave shares.
-template <int XT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS> struct Tile {
+template <int XT, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB> struct Tile {
     static constexpr int MT = 1 << MT_LOG2, WAVES_ = WM * WN;
     static constexpr int XROW = XT == F8 ? 128 : 256;                        // bytes of a row of x a stage
     static constexpr int XG = MT * XROW / 1024, WG = NT * 128 / 1024;        // 1-KiB loads a stage
     static constexpr int XS = XT == F8 ? (MT + 63) / 64 : 0;                 // of x's scales, 64 each
     static constexpr int XL = XG / WAVES_, WL = WG / WAVES_, XSL = (XS + WAVES_ - 1) / WAVES_;
-    static constexpr int LOADS = XL + WL + XSL + 1;                          // a wave's, every stage
-    static constexpr int AT_W = XG * 1024, AT_XS = AT_W + WG * 1024, AT_WS = AT_XS + XS * 256, STAGE = AT_WS + 256;
+    static constexpr int NX = XL + XSL, NW = WL + 1;                         // a wave's loads of x and of weights, every stage
+    static constexpr int AT_XS = XG * 1024, XSLOT = AT_XS + XS * 256, AT_W = XB * XSLOT, AT_WS = AT_W + WG * 1024, LDS = AT_WS + 256;
     static constexpr int TM = MT / WM / 16, TN = NT / WN / 16;               // matrix tiles a wave
-    static_assert(XG % WAVES_ == 0 && WG % WAVES_ == 0 && LOADS * (BUFS - 1) < 64 && TN % 2 == 0, "tile");
-    static_assert(NT == 128 || NT == 256, "one or two blocks of weight rows");
+    // waves a SIMD, by the workgroups whose LDS a CU holds: what the compiler may use registers for
+    static constexpr int GROUPS = 160 * 1024 / (LDS + 4 * MT + 1024), EU = GROUPS * WAVES_ / 4, WAVES_EU = EU > 8 ? 8 : EU;
+    static_assert(XG % WAVES_ == 0 && WG % WAVES_ == 0 && (NX + NW) * 2 < 64 && TN % 2 == 0, "tile");
+    static_assert((NT == 128 || NT == 256) && (XB == 2 || XB == 3), "one or two blocks of weight rows; places of x");
 };
 
-template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS>
-__global__ __launch_bounds__(64 * WM * WN) void k_f8_tile(Exl3c4DevGemm a) {
-    typedef Tile<XT, SW, MT_LOG2, NT, WM, WN, BUFS> G;
+template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB, class G = Tile<XT, SW, MT_LOG2, NT, WM, WN, XB>>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G::WAVES_EU, G::WAVES_EU))) void k_f8_tile(Exl3c4DevGemm a) {
     constexpr int MT = G::MT, WV = WM * WN, TM = G::TM, TN = G::TN;
-    __shared__ __align__(1024) char lds[BUFS * G::STAGE];
+    __shared__ __align__(1024) char lds[G::LDS];
     __shared__ int rows_x[MT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
@@ -249,77 +252,97 @@ __global__ __launch_bounds__(64 * WM * WN) void k_f8_tile(Exl3c4DevGemm a) {
     __syncthreads();
     if (ch.expert >= 0) {
         const gaddr we = entry(a.w, a.w_stride, ch.expert), wse = entry(a.ws, a.ws_stride, ch.expert);
-        // where each of the wave's loads starts, for this lane: lane l takes place l % 8 of row l / 8
-        const char* xp[G::XL];
-        gaddr wp[G::WL];
-        const char* xsp[G::XSL + 1];
+        // Each of the wave's loads of a stage: where it reads next, for this lane (lane l takes place l % 8 of row l / 8). A stage is 128 columns on.
+        gaddr xp[G::NX], wp[G::NW];
+        auto x_chunk = [&](int i) { return (lane & 7) ^ ((8 * (XT == F8 ? wave + i * WV : (wave + i * WV) >> 1) + (lane >> 3)) & 7); };
+        auto w_chunk = [&](int i) { return (lane & 7) ^ ((8 * (wave + i * WV) + (lane >> 3)) & 7); };
 #pragma unroll
         for (int i = 0; i < G::XL; ++i) {
             const int q = wave + i * WV, r = 8 * (XT == F8 ? q : q >> 1) + (lane >> 3);
-            xp[i] = a.x + (int64_t)max(rows_x[r], 0) * a.x_pitch + 16 * ((lane & 7) ^ (r & 7)) + (XT == F8 ? 0 : 128 * (q & 1));
+            xp[i] = (gaddr)a.x + (int64_t)max(rows_x[r], 0) * a.x_pitch + 16 * x_chunk(i) + (XT == F8 ? 0 : 128 * (q & 1));
         }
 #pragma unroll
-        for (int i = 0; i < G::WL; ++i) {
-            const int r = 8 * (wave + i * WV) + (lane >> 3);
-            wp[i] = we + (int64_t)w_row(r) * a.w_pitch + 16 * ((lane & 7) ^ (r & 7));
-        }
+        for (int i = 0; i < G::XSL; ++i)
+            xp[G::XL + i] = (gaddr)a.xs + (int64_t)max(rows_x[(64 * ((wave + i * WV) % max(G::XS, 1)) + lane) % MT], 0) * a.xs_pitch;
 #pragma unroll
-        for (int i = 0; i < G::XSL; ++i) {
-            const int r = (64 * ((wave + i * WV) % max(G::XS, 1)) + lane) % MT;
-            xsp[i] = (const char*)a.xs + (int64_t)max(rows_x[r], 0) * a.xs_pitch;
-        }
-        // the scales of the tile's weight rows: even lanes of its first block (SwiGLU: of the gate rows), odd lanes of the second (of the up rows)
-        const gaddr wsp = wse + (SW ? scale_row(n0, lane & 1, a.n_out) : scale_row(min(n0 + (lane & 1) * 128, a.N - 1), 0, a.N)) * a.ws_pitch;
-        const int stages = (a.K + 127) / 128;
+        for (int i = 0; i < G::WL; ++i) wp[i] = we + (int64_t)w_row(8 * (wave + i * WV) + (lane >> 3)) * a.w_pitch + 16 * w_chunk(i);
+        // the scales of the tile's weight rows: even lanes of its first block (SwiGLU: of the gate rows), odd lanes of the second (of the up rows);
+        // every wave the same ones, so that a wait counts alike in all
+        wp[G::WL] = wse + (SW ? scale_row(n0, lane & 1, a.n_out) : scale_row(min(n0 + (lane & 1) * 128, a.N - 1), 0, a.N)) * a.ws_pitch;
+        const int stages = (a.K + 127) / 128, past = a.K - 128 * (stages - 1);          // columns of the last stage
         const uint32_t at0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-        auto load = [&](int t, int buf) {
-            const uint32_t to = at0 + buf * G::STAGE;
-            const int64_t k = (int64_t)t * 128;
-            const bool full = k + 128 <= a.K;
+        // load i of x or of the weights (all 0: of no lane)
+        auto load_x = [&](int i, uint32_t to, int all) {
+            if (i < G::XL) dma16_of(xp[i], to + (wave + i * WV) * 1024, all);
+            else dma4_of(xp[i], to + G::AT_XS + ((wave + (i - G::XL) * WV) % max(G::XS, 1)) * 256, all);
+            xp[i] += i < G::XL ? G::XROW : 4;
+        };
+        auto load_w = [&](int i, int all) {
+            if (i < G::WL) dma16_of(wp[i], at0 + G::AT_W + (wave + i * WV) * 1024, all);
+            else dma4_of(wp[i], at0 + G::AT_WS, all);
+            wp[i] += i < G::WL ? 128 : 4;
+        };
+        // before the last stage's loads: what lies past K reads as zeros
+        auto end_x = [&]() {
 #pragma unroll
-            for (int i = 0; i < G::XL; ++i) {
-                const int q = wave + i * WV, r = 8 * (XT == F8 ? q : q >> 1) + (lane >> 3);
-                const int col = XT == F8 ? 16 * ((lane & 7) ^ (r & 7)) : 8 * ((lane & 7) ^ (r & 7)) + 64 * (q & 1);
-                const char* p = xp[i] + (int64_t)t * G::XROW;
-                if (!full && k + col >= a.K) p = (const char*)&k_zero;
-                dma16((gaddr)p, to + q * 1024);
-            }
+            for (int i = 0; i < G::XL; ++i)
+                if ((XT == F8 ? 16 * x_chunk(i) : 8 * x_chunk(i) + 64 * ((wave + i * WV) & 1)) >= past) xp[i] = (gaddr)&k_zero;
+        };
+        auto end_w = [&]() {
 #pragma unroll
-            for (int i = 0; i < G::WL; ++i) {
-                const int q = wave + i * WV, r = 8 * q + (lane >> 3);
-                gaddr p = wp[i] + (int64_t)t * 128;
-                if (!full && k + 16 * ((lane & 7) ^ (r & 7)) >= a.K) p = (gaddr)&k_zero;
-                dma16(p, to + G::AT_W + q * 1024);
-            }
-#pragma unroll
-            for (int i = 0; i < G::XSL; ++i)
-                dma4((gaddr)(xsp[i] + 4 * (int64_t)t), to + G::AT_XS + ((wave + i * WV) % max(G::XS, 1)) * 256);
-            dma4(wsp + 4 * (int64_t)t, to + G::AT_WS);           // (every wave the same ones: a wait counts alike in all)
+            for (int i = 0; i < G::WL; ++i)
+                if (16 * w_chunk(i) >= past) wp[i] = (gaddr)&k_zero;
+        };
+        // -1 where stage t is one, else 0 (through a VGPR: the compiler else may leave the mask itself in one)
+        auto there = [&](int t) {
+            int v = (t - stages) >> 31;
+            asm volatile("" : "+v"(v));
+            return __builtin_amdgcn_readfirstlane(v);
         };
         const int xr = wm * TM * 16 + l16, wr = wn * TN * 16 + l16;      // the lane's row in the first tile of each
-        auto multiply = [&](int buf) {
-            const char* X = lds + buf * G::STAGE;
-            const char* W = X + G::AT_W;
+        // One stage's products. between(s) is called at s = 0 .. SLOTS - 1 among them, from s = 1 on with the weights in registers.
+        constexpr int SLOTS = WIDE ? TN : TM;
+        auto multiply = [&](int slot_x, auto between) {
+            const char* X = lds + slot_x * G::XSLOT;
+            const char* W = lds + G::AT_W;
             const float* XS = (const float*)(X + G::AT_XS);
-            const float* WS = (const float*)(X + G::AT_WS);
+            const float* WS = (const float*)(lds + G::AT_WS);
             auto codes = [&](const char* p, int row) {
                 return Codes{ *(const uint4*)(p + row * 128 + 16 * (g ^ (l16 & 7))), *(const uint4*)(p + row * 128 + 16 * ((4 + g) ^ (l16 & 7))) };
             };
             // (a wave's weight rows lie in one block of 128; with SwiGLU its even tiles in the gate's, its odd ones in the up's)
             const float sw[2] = { WS[SW ? 0 : (wn * TN * 16) >> 7], WS[1] };
+            Codes wv[TN];
+#pragma unroll
+            for (int n = 0; n < TN; ++n) wv[n] = codes(W, wr + 16 * n);
             if constexpr (!WIDE) {
-                Codes wv[TN];
+                // Row tile m + 1's operand is read while tile m's products run; a sum is scaled LAG products behind its own.
+                constexpr int LAG = 3;
+                Codes xv[2];
+                float f[2][2];
+                f32x4 p[LAG + 1];
+                xv[0] = codes(X, xr);
+                f[0][0] = f[0][1] = XS[xr];
+                f[0][0] *= sw[0], f[0][1] *= sw[1];
 #pragma unroll
-                for (int n = 0; n < TN; ++n) wv[n] = codes(W, wr + 16 * n);
+                for (int i = 0; i < TM * TN + LAG; ++i) {
+                    const int m = i / TN, n = i % TN;
+                    if (i < TM * TN) {
+                        if (n == 0) {
+                            if (m + 1 < TM) xv[(m + 1) & 1] = codes(X, xr + 16 * (m + 1));
+                            between(m);
+                        }
+                        p[i % (LAG + 1)] = mma_f8(wv[n], xv[m & 1], f32x4{ 0, 0, 0, 0 });
+                    }
+                    if (i >= LAG) {
+                        const int k = i - LAG, km = k / TN, kn = k % TN;
+                        if (kn == 0 && km > 0) {
+                            const float sx = XS[xr + 16 * km];
+                            f[km & 1][0] = sx * sw[0], f[km & 1][1] = sx * sw[1];
+                        }
 #pragma unroll
-                for (int m = 0; m < TM; ++m) {
-                    const Codes xv = codes(X, xr + 16 * m);
-                    const float sx = XS[xr + 16 * m], f[2] = { sx * sw[0], sx * sw[1] };
-#pragma unroll
-                    for (int n = 0; n < TN; ++n) {
-                        const f32x4 p = mma_f8(wv[n], xv, f32x4{ 0, 0, 0, 0 });
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[n][m][r] = __builtin_fmaf(p[r], f[SW ? n & 1 : 0], acc[n][m][r]);
+                        for (int r = 0; r < 4; ++r)
+                            acc[kn][km][r] = __builtin_fmaf(p[k % (LAG + 1)][r], f[km & 1][SW ? kn & 1 : 0], acc[kn][km][r]);
                     }
                 }
             } else {
@@ -341,11 +364,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_f8_tile(Exl3c4DevGemm a) {
                 }
 #pragma unroll
                 for (int n = 0; n < TN; ++n) {
-                    const Codes q = codes(W, wr + 16 * n);
+                    between(n);
                     f32x4 p[TM] = {};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 w = widen_part<WIDER<XT>>(q, j);
+                        const uint4 w = widen_part<WIDER<XT>>(wv[n], j);
 #pragma unroll
                         for (int m = 0; m < TM; ++m) p[m] = mma<WIDER<XT>>(w, xv[m][j], p[m]);
                     }
@@ -358,20 +381,46 @@ __global__ __launch_bounds__(64 * WM * WN) void k_f8_tile(Exl3c4DevGemm a) {
                 }
             }
         };
+        if (stages == 1) end_w();
 #pragma unroll
-        for (int i = 0; i < BUFS - 1; ++i)
-            if (i < stages) load(i, i);
-        int buf = 0;
+        for (int i = 0; i < G::NW; ++i) load_w(i, -1);
+#pragma unroll
+        for (int q = 0; q < XB - 1; ++q) {
+            if (q + 1 == stages) end_x();
+#pragma unroll
+            for (int i = 0; i < G::NX; ++i) load_x(i, at0 + q * G::XSLOT, there(q));
+        }
+        int slot_x = 0;
         for (int t = 0; t < stages; ++t) {
-            if (BUFS == 2 || t + 1 >= stages) wait_loads<0>();
-            else wait_loads<G::LOADS>();
+            // the weights and x of stage t are here (the loads behind theirs are x's of stage t + 1)
+            if (XB == 2 || t + 1 >= stages) wait_loads<0>();
+            else wait_loads<G::NX>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            const int next = buf == 0 ? BUFS - 1 : buf - 1;      // the buffer of stage t - 1, read by all before the barrier
-            if (t + BUFS - 1 < stages) load(t + BUFS - 1, next);
-            multiply(buf);
+            if (t + 2 == stages) end_w();
+            if (t + XB == stages) end_x();
+            const uint32_t to_x = at0 + (slot_x == 0 ? XB - 1 : slot_x - 1) * G::XSLOT;  // the place of x of stage t - 1, read by all before the barrier
+            // Behind the last stage no lane loads: a branch would keep the products of one row tile from running on beside the next one's (8192 tokens
+            // over 8 experts, 2816 x 2048: 123 us for 114, when one workgroup filled a CU).
+            const int more_w = there(t + 1), more_x = there(t + XB - 1);
+            multiply(slot_x, [&](int s) {
+                constexpr int AT = SLOTS > 1 ? 1 : 0;                        // the loads follow in one to four slots
+                constexpr int FOR = SLOTS - AT > 4 ? 4 : SLOTS - AT;
+                if (s == AT) {                                               // every wave has read the weights
+                    asm volatile("" ::: "memory");
+                    __builtin_amdgcn_s_waitcnt(0xC07F);                      // lgkmcnt(0)
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+#pragma unroll
+                for (int i = 0; i < G::NW + G::NX; ++i)
+                    if (s == AT + i * FOR / (G::NW + G::NX)) {
+                        if (i < G::NW) load_w(i, more_w);
+                        else load_x(i - G::NW, to_x, more_x);
+                    }
+            });
             asm volatile("" ::: "memory");
-            buf = buf + 1 == BUFS ? 0 : buf + 1;
+            slot_x = slot_x + 1 == XB ? 0 : slot_x + 1;
         }
     }
     static_assert(WV * TILE_ROWS<SW, TN> * 4 <= (int)sizeof(lds), "the rows fit the stages' buffers");
@@ -389,31 +438,44 @@ int launch_rows(Exl3c4DevGemm& a, hipStream_t st) {
     return launched();
 }
 
-template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS>
+template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB>
 int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     constexpr int cols = SW ? NT / 2 : NT;
     a.tiles = (a.n_out + cols - 1) / cols;
     const int64_t grid = (chunk_bound(a.T, a.n_expert, 1 << MT_LOG2) * a.tiles + 7) / 8 * 8;
     if (grid > THREADS / (64 * WM * WN)) return EXL3C4_E_SHAPE;
-    hipLaunchKernelGGL((k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, BUFS>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
+    hipLaunchKernelGGL((k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
     return launched();
 }
 
 // Which kernel, and how large a tile: by the types, the sizes and the rows that an expert has at least on average, r = T / min(E, T) -- never by
-// the routing, which is on the device. Returns a tile's rows (32, 64, 128, 256), or for few rows an expert the strips of a workgroup (2, 4).
+// the routing, which is on the device. Larger tiles read weights and rows less often; smaller ones waste less of a chunk, make more workgroups and
+// start sooner; the rows kernel splits k over its waves, so that few workgroups are enough. `units`: workgroups of a tile, each expert half a chunk
+// short of whole ones. Measured on one card, us, the product alone (E / top-k, N x K, tokens; 512/10, 1024 x 2048 with SwiGLU where nothing else is said):
+//   rows against 32        bf16 x: 1 token 8.6 / 13.3, 4 19.3 / 20.3, 8 30 / 27, 32 97 / 95; F8 x: 8 30 / 27, 16 55 / 50, 32 95 / 91.
+//                          64/6, 32 tokens 29 / 23; 8/2, 200 16.3 / 13.8. One expert, bf16 x: 2048 x 2048, 77 rows 10.1 / 13.7, 300 22 / 18;
+//                          8192 x 8192, 64 rows 48 / 58; 4096 x 4096, 16 rows 11.5 / 23, 300 59 / 36.
+//   2 strips against 4     one row, 8192 x 8192 16.5 / 23.5; 4096 x 4096, 16 rows 11.5 / 15.2; 8192 x 8192, 64 rows 61 / 48, which read the weights
+//                          once for each 16 rows, mostly from L2.
+//   32 rows against 64     as codes: 400 tokens 184 / 189, 613 Zipf 2560 x 640 160 / 158, 1500 221 / 193, 8/2 800 15.9 / 21. bf16 x: 400 184 / 197,
+//                          613 Zipf 2560 x 640 166 / 185, 1500 220 / 203, 8/2 800 19 / 28. F8 x, f32 y: 200 183 / 203, 1500 233 / 222.
+//   64 against 128         as codes: 1500 193 / 204, 2048 Zipf 226 / 229, 4096 275 / 218, 64/6 2000 53 / 45, 8/2 8192 2816 x 2048 148 / 113.
+// As codes a tile of 256 x 256 with a CU to itself took 131 there before the loads went among the products and 114 to 118 since, and was slower
+// everywhere else; 128 x 128 130 (73 for 77 at 2048 x 1408, sorted rows in); weights in two places 232 at 64 rows, and 2% less at 32 rows and 100 to 400
+// tokens. Widened: 128 x 128 in eight waves 344, 128 x 256 211 against 202 of 64 x 256.
+// Returns a tile's rows (32, 64, 128), or for few rows an expert the strips of a workgroup (2, 4).
 int choose(bool wide, bool swiglu, int64_t T, int64_t n_expert, int64_t n_out, int64_t K) {
     const int64_t live = n_expert < T ? n_expert : T;
     // workgroups of tiles of `rows` x `cols` (SwiGLU: half as many columns of y)
     auto units = [&](int rows, int cols) {
         if (swiglu) cols /= 2;
-        return chunk_bound(T, n_expert, rows) * ((n_out + cols - 1) / cols);
+        const int64_t chunks = (T + live * rows / 2) / rows;
+        return (chunks > live ? chunks : live) * ((n_out + cols - 1) / cols);
     };
-    if (T <= (wide ? 8 : 1) * live || units(32, 128) < 64 || (T <= 4 * live && units(32, 128) < 256)) return units(16, 64) >= 1024 ? 4 : 2;
-    if (wide) return units(64, 128) < 256 ? 32 : 64;
-    if (T > 160 * live && units(256, 256) >= 256 && K >= 2048) return 256;
-    if (T > 64 * live && units(128, 128) >= 256) return 128;
-    if (T <= 16 * live || units(64, 128) < 256) return 32;
-    return 64;
+    if (units(32, 128) < 64 + K / 32) return T > 16 * live && units(16, 64) >= 256 ? 4 : 2;
+    if (!wide && T > 56 * live && units(128, 256) >= 256) return 128;
+    if (T > 18 * live && units(64, 256) >= 256) return 64;
+    return 32;
 }
 
 template <int XT, bool WIDE, bool SW>
@@ -421,12 +483,11 @@ int launch(Exl3c4DevGemm& a, hipStream_t st) {
     const int path = choose(WIDE, SW, a.T, a.n_expert, a.n_out, a.K);
     if (path == 2) return launch_rows<XT, SW, 2>(a, st);
     if (path == 4) return launch_rows<XT, SW, 4>(a, st);
-    if (path == 32) return launch_tile<XT, WIDE, SW, 5, 128, 1, 4, 3>(a, st);
-    if constexpr (!WIDE) {
-        if (path == 256) return launch_tile<XT, WIDE, SW, 8, 256, 2, 4, 2>(a, st);
-        if (path == 128) return launch_tile<XT, WIDE, SW, 7, 128, 2, 2, 2>(a, st);
-    }
-    return launch_tile<XT, WIDE, SW, 6, 128, 1, 4, 2>(a, st);
+    if (path == 32) return launch_tile<XT, WIDE, SW, 5, 128, 1, 4, XT == F8 ? 3 : 2>(a, st);
+    if constexpr (!WIDE)
+        if (path == 128) return launch_tile<XT, WIDE, SW, 7, 256, 1, 4, 2>(a, st);
+    if constexpr (XT == F8 && WIDE) return launch_tile<XT, WIDE, SW, 6, 128, 1, 4, 3>(a, st);
+    else return launch_tile<XT, WIDE, SW, 6, 256, 1, 4, XT == F8 ? 3 : 2>(a, st);
 }
 
 template <int XT, bool WIDE>

@@ -108,22 +108,47 @@ def test_products(ex, xt, tokens, top_k, E, N, K):
     check(ex, xt, "f32", False, tokens, top_k, E, N - 1, K, gather=False, seed=1)
 
 
-# (T, experts, columns of y) that take each kernel and tile; the last column tile is not whole
-SIZES = {2: (40, 3, 200), 4: (40, 40, 1650), 32: (150, 2, 1450), 64: (250, 4, 3700), 128: (260, 2, 5510), 256: (700, 2, 13320)}
+# (T, experts, weight rows, K) that take each kernel and tile; the last column tile is not whole, and k ends inside a block
+SIZES = {2: (40, 3, 200, 144), 4: (200, 3, 1650, 2064), 32: (150, 2, 1810, 144), 64: (250, 4, 13330, 144), 128: (700, 4, 9500, 272)}
 
 
 @pytest.mark.parametrize("xt,yt,p", [(x, y, p) for x, y in (("f16", "f32"), ("bf16", "f32"), ("f8", "f32"), ("f8", "f16"))
-                                     for p in ((2, 4, 32, 64) if y == "f32" else (2, 4, 32, 64, 128, 256))])
+                                     for p in ((2, 4, 32, 64) if y == "f32" else (2, 4, 32, 64, 128))])
 @pytest.mark.parametrize("swiglu", [False, True])
 def test_each_kernel(ex, xt, yt, p, swiglu):
-    """Sizes that take each kernel, their last tiles partly past the rows and columns, k ending inside a block, runs that leave rows out."""
-    T, E, n_out = SIZES[p]
-    K = 2064 if p == 256 else 144
-    assert path(ex, xt, yt, swiglu, T, E, n_out, K) == p
+    """Sizes that take each kernel, their last tiles partly past the rows and columns, runs that leave rows out."""
+    T, E, N, K = SIZES[p]
+    assert path(ex, xt, yt, swiglu, T, E, N // 2 if swiglu else N, K) == p
     off = np.array([0] + [T * (e + 1) // E - (e == 0) for e in range(E)], np.int32)
     off[-1] = T - 2
     order = np.random.default_rng(T).permutation(T).astype(np.int32)
-    check(ex, xt, yt, swiglu, T, 1, E, n_out * (2 if swiglu else 1), K, route=(order, off))
+    check(ex, xt, yt, swiglu, T, 1, E, N, K, route=(order, off))
+
+
+@pytest.mark.parametrize("xt,yt,p", [("bf16", "f32", 32), ("bf16", "f32", 64), ("f8", "f32", 32), ("f8", "f32", 64), ("f8", "bf16", 32),
+                                     ("f8", "bf16", 64), ("f8", "bf16", 128)])
+@pytest.mark.parametrize("K", [16, 128, 240, 256, 384, 400, 512, 1040])
+def test_each_tile_by_stages(ex, xt, yt, p, K):
+    """One stage, two, three and more, whole and partly past K: the loads' places in turn, and none behind the last."""
+    T, E, N, _ = SIZES[p]
+    N += 800 if K >= 384 and p == 32 else 0                         # a longer k asks for more workgroups
+    assert path(ex, xt, yt, False, T, E, N, K) == p
+    g = torch.Generator().manual_seed(K)
+    w = w_operand(ex, g, 1, N, K, False)
+    x = torch.randn((T, K), generator=g)
+    off = np.array([T * e // E for e in range(E + 1)], np.int32)
+    # experts that share one matrix, by a table of pointers
+    xd, xv, xp = x_operand(ex, x, xt)
+    y = torch.full((T + 1, N + 3), float("nan"), dtype=TYPES[yt], device="cuda")
+    gm = ex.make_gemm(xd, w[0], None, torch.from_numpy(off).cuda(), y[:T, :N])
+    tw = torch.full((E,), w[0].codes.data_ptr(), dtype=torch.int64, device="cuda")
+    ts = torch.full((E,), w[0].scales.data_ptr(), dtype=torch.int64, device="cuda")
+    gm.n_expert, gm.w, gm.w_scales, gm.w_stride, gm.ws_stride = E, tw.data_ptr(), ts.data_ptr(), 0, 0
+    assert ex.moe_gemm(gm) == 0
+    torch.cuda.synchronize()
+    want, tol = f8ref.gemm(xv, w[1], None, [0, T], T, 1, False, (xp, w[2]) if xt == "f8" and yt != "f32" else None)
+    assert mx4ref.close(y[:T, :N].cpu(), want, tol)
+    assert torch.isnan(y[T]).all() and torch.isnan(y[:, N:]).all()
 
 
 @pytest.mark.parametrize("xt", XS)
