@@ -165,7 +165,7 @@ typedef struct Exl3c4DevRoute {
     int32_t      type, score, group_score, renorm, n_expert, top_k, n_group, top_group;
     int32_t      group;            /* experts a group; group_inv: e * group_inv >> 20 = e / group for e < 1024 (group > 512 has one group) */
     uint32_t     group_inv;
-    int32_t      part_log2;        /* the 2^part_log2 lanes that a group has of a wave */
+    int32_t      groups_log2;      /* ceil(log2 n_group) */
     float        scale;
 } Exl3c4DevRoute;
 /* moe_route's router; scatter: with the scatter, at most 16 tokens */

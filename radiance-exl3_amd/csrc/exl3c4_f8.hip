@@ -5,8 +5,9 @@
 // are rounded once in f32, so that another implementation of these steps gives the same codes. The largest magnitude is found on the bits, where
 // infinities and NaNs are the largest. v_cvt_pk_fp8_f32 rounds to nearest even (checked for every tie against that rule).
 //
-// A lane takes 8 columns (loads of 16 or 32 bytes, stores of 8), 16 lanes a block's row. Blocks of one row: the 16 lanes find the largest by DPP.
-// Blocks of 128 rows: a workgroup each, every value of the block in its registers, so that memory is read once.
+// Blocks of one row: a lane takes 16 bytes of values, 8 columns of 16 bits or 4 of 32, so that a wave's loads and stores are whole lines; the 16 or 32
+// lanes of a block find the largest by DPP. Blocks of 128 rows: a workgroup each, 8 columns a lane and every value of the block in its registers, so
+// that memory is read once. The same columns a lane on the way back.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -17,34 +18,40 @@ namespace {
 
 constexpr int F32 = EXL3C4_F32, F16 = EXL3C4_F16, BF16 = EXL3C4_BF16;
 constexpr int WG = 256;
-constexpr int PER = 4;                                          // slots (8 columns) a lane, where rows are apart
+constexpr int PER = 4;                                          // slots (16 bytes of values) a lane, where rows are apart
 constexpr int64_t SLOTS = (int64_t)1 << 31;                     // slots a launch indexes in 32 bits
 constexpr float TOP = 448.f;                                    // e4m3's largest
 constexpr uint32_t LEAST = 31u << 23;                           // 2^-96, the least magnitude that sets a scale: 448 / a stays finite
 
 typedef float float2_t __attribute__((ext_vector_type(2)));
-// 8 elements at any address their type may have
-struct __attribute__((packed, aligned(2))) Eight16 { uint32_t v[4]; };
-struct __attribute__((packed, aligned(4))) Eight32 { uint32_t v[8]; };
-template <int DT> constexpr int words = DT == F32 ? 8 : 4;
+// 16 bytes at any address their type may have
+struct __attribute__((packed, aligned(2))) Words { uint32_t v[4]; };
+template <int DT> constexpr int COLS = DT == F32 ? 4 : 8;       // values in 16 bytes
+template <int DT> constexpr int SIZE = DT == F32 ? 4 : 2;
 
-// Columns c .. c + 7 of a row at p (its column c), those from `cols` on as zeros.
-template <int DT> __device__ __forceinline__ void load8(uint32_t* v, const char* p, uint32_t c, uint32_t cols) {
-    if (c + 8 <= cols) {
-        if constexpr (DT == F32) {
-            const Eight32 q = *(const Eight32*)p;
+// Columns c .. of a row at p (its column c) in 16 bytes, those from `cols` on as zeros: the row's last 16 bytes where they would pass its end, shifted
+// (2-byte loads of each took 20480 x 650 f16 from 9 to 14 us).
+template <int DT> __device__ __forceinline__ void load16b(uint32_t* v, const char* p, uint32_t c, uint32_t cols) {
+    constexpr uint32_t C = COLS<DT>;
+    if (cols >= C) {                                             // (uniform)
+        const uint32_t past = c + C > cols ? c + C - cols : 0;
+        const Words q = *(const Words*)(p - (int64_t)past * SIZE<DT>);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = q.v[i];
-        } else {
-            const Eight16 q = *(const Eight16*)p;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = q.v[i];
+        for (int i = 0; i < 4; ++i) v[i] = q.v[i];
+        if (past) {
+            uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+            if (past >= C / 2) lo = hi, hi = 0;
+            if (past >= C) lo = 0;
+            const uint32_t bits = (past & (C / 2 - 1)) * (8 * SIZE<DT>);
+            lo = lo >> bits | (hi << 1) << (63 - bits);
+            hi >>= bits;
+            v[0] = (uint32_t)lo, v[1] = (uint32_t)(lo >> 32), v[2] = (uint32_t)hi, v[3] = (uint32_t)(hi >> 32);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < words<DT>; ++i) v[i] = 0;
+        for (int i = 0; i < 4; ++i) v[i] = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < (int)C; ++i)
             if (c + i < cols) {
                 if constexpr (DT == F32) v[i] = ((const uint32_t*)p)[i];
                 else v[i >> 1] |= (uint32_t)((const uint16_t*)p)[i] << (16 * (i & 1));
@@ -56,12 +63,12 @@ template <int DT> __device__ __forceinline__ float value(const uint32_t* v, int 
     const uint32_t h = (v[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
     return DT == BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
-// The largest magnitude of the 8 as f32 bits (of f16, an infinity or a NaN stays one).
+// The largest magnitude of 16 bytes as f32 bits (of f16, an infinity or a NaN stays one).
 template <int DT> __device__ __forceinline__ uint32_t magnitude(const uint32_t* v) {
     uint32_t m = 0;
     if constexpr (DT == F32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, v[i] & 0x7FFFFFFFu);
+        for (int i = 0; i < 4; ++i) m = max(m, v[i] & 0x7FFFFFFFu);
         return m;
     } else {
 #pragma unroll
@@ -69,35 +76,53 @@ template <int DT> __device__ __forceinline__ uint32_t magnitude(const uint32_t* 
         return DT == BF16 ? m << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)m));
     }
 }
-// The largest of a row of 16 lanes, in each of them.
+// The largest of a row of 16 lanes, in each of them; and of two such rows, of lanes 0 .. 31 and of 32 .. 63.
 __device__ __forceinline__ uint32_t max16(uint32_t v) {
     v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));       // quad_perm: lane ^ 1
     v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));       // lane ^ 2
     v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));      // row_half_mirror: the other quad of 8
     return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));   // row_mirror: the other 8
 }
+__device__ __forceinline__ uint32_t max32(uint32_t v) {
+    v = max16(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(r[0], r[1]);
+}
 
+// A block's scale a / 448 and 448 / a, each rounded once: a quotient's remainder by a multiply-add, and the quotient corrected by it. 448 / a is taken
+// of a's mantissa, whose reciprocal has one step of Newton's behind the hardware's; with that one off by up to two steps both are right for every
+// mantissa (all of them tried). (The compiler's division is 14 instructions for each, of every lane: 20480 x 650 f16 14 us with them.)
 struct Scale {
     float s, inv;
     __device__ __forceinline__ explicit Scale(uint32_t top) {
-        const float a = __uint_as_float(max(top, LEAST));
-        const bool bad = top >= 0x7F800000u;
-        s = bad ? __uint_as_float(0x7FC00000u) : a / TOP;
-        inv = bad ? 0.f : TOP / a;
+        const uint32_t u = max(top, LEAST);
+        const float a = __uint_as_float(u), m = __uint_as_float((u & 0x7FFFFFu) | 0x3F800000u);
+        constexpr float TH = 1.f / TOP;
+        const float q = a * TH;
+        float y = __builtin_amdgcn_rcpf(m);
+        y = __builtin_fmaf(__builtin_fmaf(-m, y, 1.f), y, y);
+        const float p = TOP * y;
+        s = __builtin_fmaf(__builtin_fmaf(-q, TOP, a), TH, q);
+        inv = __builtin_amdgcn_ldexpf(__builtin_fmaf(__builtin_fmaf(-p, m, TOP), y, p), 127 - (int)(u >> 23));
+        if (top >= 0x7F800000u) s = __uint_as_float(0x7FC00000u), inv = 0.f;
     }
 };
-// 8 values' codes (a block with an infinity or a NaN: zeros).
-template <int DT> __device__ __forceinline__ uint2 codes_of(const uint32_t* v, const Scale& k) {
-    uint32_t q[2] = { 0, 0 };
-    if (k.inv == 0.f) return { 0, 0 };
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(value<DT>(v, 4 * h) * k.inv, value<DT>(v, 4 * h + 1) * k.inv, q[h], false);
-        q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(value<DT>(v, 4 * h + 2) * k.inv, value<DT>(v, 4 * h + 3) * k.inv, q[h], true);
-    }
-    return { q[0], q[1] };
+// The codes of four values from the i-th of 16 bytes on (inv 0, of a block with an infinity or a NaN: zeros).
+template <int DT> __device__ __forceinline__ uint32_t four_codes(const uint32_t* v, int i, const Scale& k) {
+    int q = __builtin_amdgcn_cvt_pk_fp8_f32(value<DT>(v, i) * k.inv, value<DT>(v, i + 1) * k.inv, 0, false);
+    q = __builtin_amdgcn_cvt_pk_fp8_f32(value<DT>(v, i + 2) * k.inv, value<DT>(v, i + 3) * k.inv, q, true);
+    return k.inv == 0.f ? 0u : (uint32_t)q;
+}
+template <int DT> __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t* v, const Scale& k) {
+    if constexpr (DT == F32) *(uint32_t*)p = four_codes<DT>(v, 0, k);
+    else *(uint2*)p = { four_codes<DT>(v, 0, k), four_codes<DT>(v, 4, k) };
 }
 
+// Slots of a launch: lanes_row of them a row. s / lanes_row by a multiplication (s < 2^31, lanes_row at least 2; exact).
+struct Slots {
+    uint32_t row0, count, lanes_row, mul, shift;
+    __device__ __forceinline__ uint32_t row(uint32_t s) const { return __umulhi(s, mul) >> shift; }
+};
 // Row r of all the matrices': matrix r / rows, its row r % rows.
 struct Where { uint32_t mat, row; };
 __device__ __forceinline__ Where where(const Exl3c4DevF8& a, uint32_t r) {
@@ -106,48 +131,55 @@ __device__ __forceinline__ Where where(const Exl3c4DevF8& a, uint32_t r) {
     return { m, r - m * a.rows };
 }
 
-// Blocks of one row. Slots first .. slots - 1 are 8 columns each, lanes_row a row (whole blocks), from row row0 on.
+// Blocks of one row: whole blocks of lanes a row.
 template <int DT>
-__global__ __launch_bounds__(WG) void k_f8_quant_rows(Exl3c4DevF8 a, uint32_t row0, uint32_t slots, uint32_t lanes_row) {
-    uint32_t v[PER][words<DT>], row[PER], at[PER];
+__global__ __launch_bounds__(WG) void k_f8_quant_rows(Exl3c4DevF8 a, Slots sl) {
+    constexpr uint32_t C = COLS<DT>, BLOCK_LOG2 = DT == F32 ? 5 : 4;
+    uint32_t v[PER][4], at[PER];
     const uint32_t first = blockIdx.x * (WG * PER) + threadIdx.x;
     Where w[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const uint32_t s = min(first + j * WG, slots - 1);       // (a slot past the last is it again, not stored)
-        row[j] = s / lanes_row;
-        at[j] = s - row[j] * lanes_row;
-        w[j] = where(a, row0 + row[j]);
-        load8<DT>(v[j], a.v + w[j].mat * a.v_stride + w[j].row * a.v_pitch + (int64_t)(8 * at[j]) * (words<DT> / 2), 8 * at[j], a.cols);
+        const uint32_t s = min(first + j * WG, sl.count - 1), row = sl.row(s);     // (a slot past the last is it again, not stored)
+        at[j] = s - row * sl.lanes_row;
+        w[j] = where(a, sl.row0 + row);
+        load16b<DT>(v[j], a.v + w[j].mat * a.v_stride + w[j].row * a.v_pitch + (int64_t)at[j] * 16, C * at[j], a.cols);
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        // (the 16 lanes of a block are in one row of lanes, all inside the slots or all the last one again)
-        const Scale k(max16(magnitude<DT>(v[j])));
-        if (first + j * WG >= slots) continue;
-        if (8 * at[j] < a.code_cols)
-            *(uint2*)(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + 8 * at[j]) = codes_of<DT>(v[j], k);
-        if ((at[j] & 15) == 0) *(float*)((char*)a.scales + w[j].mat * a.scales_stride + w[j].row * a.scales_pitch + (at[j] >> 4) * 4) = k.s;
+        // (the lanes of a block are neighbours in a wave, all inside the slots or all the last one again)
+        const uint32_t m = magnitude<DT>(v[j]);
+        const Scale k(DT == F32 ? max32(m) : max16(m));
+        if (first + j * WG >= sl.count) continue;
+        if (C * at[j] < a.code_cols) store_codes<DT>(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + C * at[j], v[j], k);
+        if ((at[j] & ((1u << BLOCK_LOG2) - 1)) == 0)
+            *(float*)((char*)a.scales + w[j].mat * a.scales_stride + w[j].row * a.scales_pitch + (at[j] >> BLOCK_LOG2) * 4) = k.s;
     }
 }
 
 // Blocks of 128 rows: workgroup b takes block b of the matrices' grids of down x across blocks.
 template <int DT>
 __global__ __launch_bounds__(WG) void k_f8_quant_blocks(Exl3c4DevF8 a, uint32_t across, uint32_t down) {
+    constexpr int H = 8 / COLS<DT>;                              // 16-byte parts of 8 columns
     __shared__ uint32_t top[WG / 64];
     const uint32_t per = across * down, m = blockIdx.x / per, in = blockIdx.x - m * per, rb = in / across, cb = in - rb * across;
     const uint32_t c = 128 * cb + 8 * (threadIdx.x & 15), r0 = 128 * rb + (threadIdx.x >> 4);
-    const char* p = a.v + m * a.v_stride + (int64_t)c * (words<DT> / 2);
-    uint32_t v[8][words<DT>], t = 0;
+    const char* p = a.v + m * a.v_stride + (int64_t)c * SIZE<DT>;
+    uint32_t v[8][H][4], t = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const uint32_t r = r0 + 16 * j;
 #pragma unroll
-        for (int i = 0; i < words<DT>; ++i) v[j][i] = 0;
-        if (r < a.rows) load8<DT>(v[j], p + r * a.v_pitch, c, a.cols);
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j][h][i] = 0;
+            if (r < a.rows) load16b<DT>(v[j][h], p + r * a.v_pitch + 16 * h, c + COLS<DT> * h, a.cols);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t = max(t, magnitude<DT>(v[j]));
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int h = 0; h < H; ++h) t = max(t, magnitude<DT>(v[j][h]));
     t = max16(t);
     t = max(max((uint32_t)__builtin_amdgcn_readlane((int)t, 0), (uint32_t)__builtin_amdgcn_readlane((int)t, 16)),
             max((uint32_t)__builtin_amdgcn_readlane((int)t, 32), (uint32_t)__builtin_amdgcn_readlane((int)t, 48)));
@@ -158,61 +190,59 @@ __global__ __launch_bounds__(WG) void k_f8_quant_blocks(Exl3c4DevF8 a, uint32_t 
     if (c < a.code_cols)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (r0 + 16 * j < a.rows) *(uint2*)(q + (r0 + 16 * j) * a.codes_pitch) = codes_of<DT>(v[j], k);
+            if (r0 + 16 * j < a.rows)
+                *(uint2*)(q + (r0 + 16 * j) * a.codes_pitch) = { four_codes<DT>(v[j][0], 0, k), four_codes<DT>(v[j][H - 1], 4 % COLS<DT>, k) };
     if (threadIdx.x == 0) *(float*)((char*)a.scales + m * a.scales_stride + rb * a.scales_pitch + cb * 4) = k.s;
 }
 
 template <int DT>
-__global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, uint32_t row0, uint32_t slots, uint32_t lanes_row) {
-    uint2 q[PER];
-    uint32_t at[PER];
+__global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, Slots sl) {
+    constexpr uint32_t C = COLS<DT>, BLOCK_LOG2 = DT == F32 ? 5 : 4;
+    uint32_t q[PER][C / 4], at[PER];
     float scale[PER];
     Where w[PER];
     const uint32_t first = blockIdx.x * (WG * PER) + threadIdx.x;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const uint32_t s = min(first + j * WG, slots - 1), row = s / lanes_row;
-        at[j] = s - row * lanes_row;
-        w[j] = where(a, row0 + row);
-        q[j] = *(const uint2*)(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + 8 * at[j]);
-        scale[j] = *(const float*)((const char*)a.scales + w[j].mat * a.scales_stride + (w[j].row >> a.block_log2) * a.scales_pitch + (at[j] >> 4) * 4);
+        const uint32_t s = min(first + j * WG, sl.count - 1), row = sl.row(s);
+        at[j] = s - row * sl.lanes_row;
+        w[j] = where(a, sl.row0 + row);
+        const uint32_t* p = (const uint32_t*)(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + C * at[j]);
+        if constexpr (DT == F32) q[j][0] = *p;
+        else {
+            const uint2 u = *(const uint2*)p;
+            q[j][0] = u.x, q[j][1] = u.y;
+        }
+        scale[j] = *(const float*)((const char*)a.scales + w[j].mat * a.scales_stride + (w[j].row >> a.block_log2) * a.scales_pitch + (at[j] >> BLOCK_LOG2) * 4);
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        if (first + j * WG >= slots) continue;
-        float f[8];
-#define CVT(i, word, hi) { const float2_t p = __builtin_amdgcn_cvt_pk_f32_fp8(word, hi); f[i] = p[0] * scale[j]; f[i + 1] = p[1] * scale[j]; }
-        CVT(0, q[j].x, false) CVT(2, q[j].x, true) CVT(4, q[j].y, false) CVT(6, q[j].y, true)
-#undef CVT
-        const uint32_t c = 8 * at[j];
-        char* p = a.v + w[j].mat * a.v_stride + w[j].row * a.v_pitch + (int64_t)c * (words<DT> / 2);
-        uint32_t o[words<DT>];
+        if (first + j * WG >= sl.count) continue;
+        float f[C];
 #pragma unroll
-        for (int i = 0; i < words<DT>; ++i) {
-            if constexpr (DT == F32) o[i] = __float_as_uint(f[i]);
-            else if constexpr (DT == F16)
-                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]) << 16;
-            else
-                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) << 16;
+        for (int i = 0; i < (int)C / 4; ++i) {
+            const float2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(q[j][i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(q[j][i], true);
+            f[4 * i] = lo[0] * scale[j], f[4 * i + 1] = lo[1] * scale[j], f[4 * i + 2] = hi[0] * scale[j], f[4 * i + 3] = hi[1] * scale[j];
         }
-        if (c + 8 <= a.cols) {
-            if constexpr (DT == F32) {
-                Eight32 e;
+        const uint32_t c = C * at[j];
+        char* p = a.v + w[j].mat * a.v_stride + w[j].row * a.v_pitch + (int64_t)at[j] * 16;
+        Words o;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e.v[i] = o[i];
-                *(Eight32*)p = e;
-            } else {
-                Eight16 e;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e.v[i] = o[i];
-                *(Eight16*)p = e;
-            }
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == F32) o.v[i] = __float_as_uint(f[i]);
+            else if constexpr (DT == F16)
+                o.v[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]) << 16;
+            else
+                o.v[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) << 16;
+        }
+        if (c + C <= a.cols) {
+            *(Words*)p = o;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < (int)C; ++i)
                 if (c + i < a.cols) {
-                    if constexpr (DT == F32) ((uint32_t*)p)[i] = o[i];
-                    else ((uint16_t*)p)[i] = (uint16_t)(o[i >> 1] >> (16 * (i & 1)));
+                    if constexpr (DT == F32) ((uint32_t*)p)[i] = o.v[i];
+                    else ((uint16_t*)p)[i] = (uint16_t)(o.v[i >> 1] >> (16 * (i & 1)));
                 }
         }
     }
@@ -220,13 +250,17 @@ __global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, uint32_t row0,
 
 int launched() { return hipGetLastError() == hipSuccess ? 0 : EXL3C4_E_DEVICE; }
 
-// All the matrices' rows in launches whose slots fit 32 bits (17 G columns each: one launch in all but the largest cases).
+// All the matrices' rows in launches whose slots fit 31 bits (8 G columns each: one launch in all but the largest cases). lanes: at least 2 a row.
 template <class K>
 int each_part(K kernel, const Exl3c4DevF8& a, uint32_t lanes, hipStream_t st) {
-    const uint32_t all = a.n * a.rows, most = (uint32_t)(SLOTS / lanes < 1 ? 1 : SLOTS / lanes);
+    const uint32_t all = a.n * a.rows, most = (uint32_t)((SLOTS - 1) / lanes < 1 ? 1 : (SLOTS - 1) / lanes);
+    uint32_t l = 1;                                              // ceil(log2 lanes): ceil(2^(31 + l) / lanes) fits 32 bits, and its product is exact below 2^31
+    while (((uint32_t)1 << l) < lanes) ++l;
+    const uint32_t mul = (uint32_t)((((uint64_t)1 << (31 + l)) + lanes - 1) / lanes);
     for (uint32_t r = 0; r < all;) {
-        const uint32_t n = all - r < most ? all - r : most, slots = n * lanes;
-        hipLaunchKernelGGL(kernel, dim3((slots + WG * PER - 1) / (WG * PER)), dim3(WG), 0, st, a, r, slots, lanes);
+        const uint32_t n = all - r < most ? all - r : most;
+        const Slots sl = { r, n * lanes, lanes, mul, l - 1 };
+        hipLaunchKernelGGL(kernel, dim3((sl.count + WG * PER - 1) / (WG * PER)), dim3(WG), 0, st, a, sl);
         if (const int rc = launched()) return rc;
         r += n;
     }
@@ -239,7 +273,7 @@ extern "C" int exl3c4_dev_f8_quant(const Exl3c4DevF8* a, int32_t dtype, void* st
     const hipStream_t st = (hipStream_t)stream;
     const uint32_t across = (a->cols + 127) / 128;
     if (a->block_log2 == 0)
-        return each_part(dtype == F32 ? k_f8_quant_rows<F32> : dtype == F16 ? k_f8_quant_rows<F16> : k_f8_quant_rows<BF16>, *a, 16 * across, st);
+        return each_part(dtype == F32 ? k_f8_quant_rows<F32> : dtype == F16 ? k_f8_quant_rows<F16> : k_f8_quant_rows<BF16>, *a, (dtype == F32 ? 32 : 16) * across, st);
     const uint32_t down = (a->rows + 127) / 128, blocks = a->n * across * down;
     if (blocks == 0) return 0;
     const auto f = dtype == F32 ? k_f8_quant_blocks<F32> : dtype == F16 ? k_f8_quant_blocks<F16> : k_f8_quant_blocks<BF16>;
@@ -249,5 +283,6 @@ extern "C" int exl3c4_dev_f8_quant(const Exl3c4DevF8* a, int32_t dtype, void* st
 
 extern "C" int exl3c4_dev_f8_dequant(const Exl3c4DevF8* a, int32_t dtype, void* stream) {
     const auto f = dtype == F32 ? k_f8_dequant<F32> : dtype == F16 ? k_f8_dequant<F16> : k_f8_dequant<BF16>;
-    return each_part(f, *a, (a->cols + 7) / 8, (hipStream_t)stream);
+    const uint32_t per = dtype == F32 ? 4 : 8, lanes = (a->cols + per - 1) / per;
+    return each_part(f, *a, lanes < 2 ? 2 : lanes, (hipStream_t)stream);      // (a second lane of a single one's row stores nothing)
 }

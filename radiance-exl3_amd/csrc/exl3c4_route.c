@@ -102,7 +102,7 @@ int exl3c4_moe_route(const Exl3c4Route* r, void* stream) {
                          .type = r->logits_type, .score = r->score, .group_score = r->group_score, .renorm = r->renorm,
                          .n_expert = (int32_t)r->n_expert, .top_k = r->top_k, .n_group = r->n_group, .top_group = r->top_group,
                          .group = group, .group_inv = ((1u << 20) + (uint32_t)group - 1u) / (uint32_t)group, .scale = r->scale };
-    for (int32_t lanes = 64; lanes / 2 >= r->n_group; lanes /= 2) ++d.part_log2;
+    while ((1 << d.groups_log2) < r->n_group) ++d.groups_log2;
     if (scatter && r->n_tok <= FUSED_MAX_TOKENS) return exl3c4_dev_score(&d, 1, stream);
     rc = exl3c4_dev_score(&d, 0, stream);
     if (rc || !scatter) return rc;

@@ -45,13 +45,14 @@ struct Pick { int id; float w; };
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
     return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), d) << 32) | (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)v, d);
 }
-// The value of lane l ^ J, without the LDS pipe's bpermute: DPP moves for J = 1, 2 (quad_perm) and 8 (row_ror 8), a
-// ds_swizzle (xor mode, within 32 lanes) for 4, gfx950's permlane swaps for 16 and 32 (each lane takes the half of
+// The value of lane l ^ J, without the LDS pipe's bpermute: DPP moves for J = 1, 2 (quad_perm) and 8 (row_ror 8), two
+// for 4 (row_half_mirror is ^ 7, quad_perm ^ 3), gfx950's permlane swaps for 16 and 32 (each lane takes the half of
 // the swapped pair that came from its partner). Every lane of the wave must be active.
 template <int J> __device__ __forceinline__ uint32_t xor_lane(uint32_t v, int lane) {
     if constexpr (J == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false);
     else if constexpr (J == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false);
-    else if constexpr (J == 4) return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x101F);
+    else if constexpr (J == 4)
+        return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
     else if constexpr (J == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, false);
     else if constexpr (J == 16) {
         const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
@@ -217,13 +218,19 @@ __global__ __launch_bounds__(256) void k_router(const void* logits, int64_t n_to
 // issue for longer than the few pairs take), as waves without a pair rank none. 1 / 80 / 320 / 1,280 pairs over 512
 // experts, us a launch of a chain of them: 4.76 / 4.90 / 4.87 / 5.28 with sixteen loads always, 2.50 / 3.69 / 4.31 / 4.69
 // now; the single workgroup before took 3.28 / 4.83 / 9.11 / 27.8.
+// A base that 32 bits hold (FAR: another one) lets a pair's expert be found in them: 81,920 pairs over 512 experts 18.1 -> SCATTER_US us.
 constexpr int SC_THREADS = 1024, SC_SEG = 256, SC_MAX_WG = 256;
-__device__ __forceinline__ int expert_of(int32_t id, int64_t base, int n_expert) {
-    const int64_t g = (int64_t)id - base;
-    return (g >= 0 && g < n_expert) ? (int)g : -1;
+template <bool FAR> __device__ __forceinline__ int expert_of(int32_t id, int64_t base, int n_expert) {
+    if constexpr (FAR) {
+        const int64_t g = (int64_t)id - base;
+        return (g >= 0 && g < n_expert) ? (int)g : -1;
+    } else {
+        const uint32_t g = (uint32_t)id - (uint32_t)base;
+        return id >= (int32_t)base && g < (uint32_t)n_expert ? (int)g : -1;
+    }
 }
 
-template <int LOADS>
+template <int LOADS, bool FAR>
 __global__ __launch_bounds__(SC_THREADS) void k_scatter(const int32_t* ids, uint32_t T, int64_t base, int32_t n_expert,
                                                         uint32_t seg, int32_t* sorted, int32_t* off, int32_t* count,
                                                         int32_t* row_of) {
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(SC_THREADS) void k_scatter(const int32_t* ids, uint
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const uint32_t i = i0 + SC_THREADS * j + tid;
-            const int e = i < T ? expert_of(f[j], base, n_expert) : -1;
+            const int e = i < T ? expert_of<FAR>(f[j], base, n_expert) : -1;
             if (e >= 0) atomicAdd(&hist[(i < lo ? 0 : SC_THREADS) + e], 1);
         }
     }
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(SC_THREADS) void k_scatter(const int32_t* ids, uint
         const uint32_t i = c0 + tid;
         int e = -1;
         if (tid < SC_SEG) {
-            if (i < hi) e = expert_of(c0 == lo ? mine : ids[i], base, n_expert);
+            if (i < hi) e = expert_of<FAR>(c0 == lo ? mine : ids[i], base, n_expert);
             eid[tid] = e;
             rank_l[tid] = 0;
         }
@@ -372,8 +379,10 @@ __global__ __launch_bounds__(1024) void k_route_scatter(const void* logits, int3
 }
 
 // ------------------------------------------------------------------------------------------ moe_route
-// The order of experts and of groups is decided in 64 bits: values of two experts that f32 could not tell apart are common among thousands of
-// tokens, and this card's f64 multiply-adds issue as fast as f32's. Every number behind the logits is f64, the weights are rounded once.
+// The order of experts and of groups is that of their values in 64 bits, for among thousands of tokens there are always experts whose values f32 would
+// not tell apart. f32 finds who can be among the first (all within its error of them), f64 ranks those: one evaluation a lane. Groups whose place f32 leaves
+// open, and more than 64 such experts, are evaluated in f64 as a whole. Weights come out of the f64 scores, rounded once.
+// 8192 tokens, 8 groups of 64 experts, top-10 with a bias: f64 for every expert took 22 us.
 
 // e^x for x <= 0 (below -800: 0): x = n ln 2 + r with ln 2 in two parts, |r| <= ln 2 / 2, and the exponential series up to r^13, whose rest is
 // below 2^-52 of e^r.
@@ -431,141 +440,248 @@ __device__ __forceinline__ float logit(const Exl3c4DevRoute& a, int64_t at) {
 }
 __device__ __forceinline__ bool is_out(float v) { return !(v > -INFINITY); }       // -infinity or NaN
 
-// One token by one wave: the experts e = lane + 64 j in registers. Lane r < top_k ends with the r-th expert and its weight. key, id: the wave's 64
-// places of LDS; value: its 64 RPL places (GROUPS).
-template <int RPL, bool GROUPS>
-__device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row, int lane, uint64_t* key, int* id, double* value) {
-    float l[RPL], b[RPL];
-    const int E = a.n_expert;
-    if (a.type == EXL3C4_F32) {
-        const float* p = (const float*)a.logits + row;
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) l[j] = lane + 64 * j < E ? p[lane + 64 * j] : -INFINITY;
-    } else {
-        const uint16_t* p = (const uint16_t*)a.logits + row;
-        uint16_t h[RPL];
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) h[j] = lane + 64 * j < E ? p[lane + 64 * j] : a.type == EXL3C4_BF16 ? (uint16_t)0xFF80u : (uint16_t)0xFC00u;
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) l[j] = a.type == EXL3C4_BF16 ? __uint_as_float((uint32_t)h[j] << 16) : (float)__builtin_bit_cast(_Float16, h[j]);
-    }
-    if (a.bias)
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) b[j] = lane + 64 * j < E ? a.bias[lane + 64 * j] : 0.f;
-    // softmax: the largest logit and the sum's inverse
-    const bool soft = a.score == EXL3C4_SCORE_SOFTMAX, top2 = GROUPS && a.group_score == EXL3C4_GROUP_TOP2;
-    double m = 0.0, inv = 1.0, s[RPL];
-    if (soft) {
-        float mf = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) mf = fmaxf(mf, l[j]);        // (a NaN never wins)
-        mf = fmaxf(mf, xor_lanef<32>(mf, lane));
-        mf = fmaxf(mf, xor_lanef<16>(mf, lane));
-        mf = fmaxf(mf, xor_lanef<8>(mf, lane));
-        mf = fmaxf(mf, xor_lanef<4>(mf, lane));
-        mf = fmaxf(mf, xor_lanef<2>(mf, lane));
-        mf = fmaxf(mf, xor_lanef<1>(mf, lane));
-        m = mf;
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) {
-            s[j] = is_out(l[j]) ? 0.0 : exp64(l[j] == mf ? 0.0 : (double)l[j] - m);      // (infinity - infinity is none)
-            sum += s[j];
-        }
-        inv = inverse64(fmax(wave_sum(sum, lane), 1.0));           // (1 at least, but for a row that is out as a whole)
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) s[j] *= inv;
-    } else if (a.bias || top2) {
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) s[j] = sigmoid64(l[j]);
-    }
-    uint64_t k[RPL];
-#pragma unroll
-    for (int j = 0; j < RPL; ++j) {
-        const double c = a.bias ? s[j] + (double)b[j] : (double)l[j];
-        k[j] = is_out(l[j]) || (a.bias && is_out(b[j])) ? 0 : order64(c);
-    }
-    if constexpr (GROUPS) {
-        // the values by expert through LDS; then 2^part_log2 lanes a group find its two largest
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) {
-            const double v = a.bias ? s[j] + (double)b[j] : top2 ? s[j] : (double)l[j];
-            value[lane + 64 * j] = k[j] ? v : -INFINITY;
-        }
-        wave_sync();
-        const int part = 1 << a.part_log2, g = lane >> a.part_log2;
+// What a token's experts are ranked by: softmax's largest logit and its sum's inverse.
+struct Soft { float m; double inv; };
+__device__ __forceinline__ double score64(const Exl3c4DevRoute& a, const Soft& sm, float l) {
+    if (a.score == EXL3C4_SCORE_SIGMOID) return sigmoid64(l);
+    return exp64(l == sm.m ? 0.0 : (double)l - (double)sm.m) * sm.inv;             // (infinity - infinity is none)
+}
+// An f32 score is within 2^-21 of its value: sigmoid's exponent, exponential, sum, reciprocal and product lose 5 steps of 2^-24 together, softmax's (from f64
+// exponentials) 3. A choice is off by that and its own rounding; a sum of two by twice as much.
+__device__ __forceinline__ float error_of(float c) { return 0x1p-21f + 0x1p-23f * fabsf(c); }
+__device__ __forceinline__ float sigmoid32(float l) {
+    const float t = __builtin_amdgcn_exp2f(fabsf(l) * -1.44269504088896340736f), q = __builtin_amdgcn_rcpf(1.f + t);
+    return l >= 0.f ? q : t * q;
+}
+// The order of floats as unsigned numbers (-0 as +0); 0 stands for none, which a NaN is.
+__device__ __forceinline__ uint32_t order32(float v) {
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return v == v ? (u >> 31 ? ~u : u | 0x80000000u) : 0u;
+}
+__device__ __forceinline__ float value_of32(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
+
+// An expert's choice in f64, its logit and bias read again (the rare paths: rolled, and without a hold on the registers of the others).
+__device__ __forceinline__ double choice64(const Exl3c4DevRoute& a, const Soft& sm, int64_t row, int e, bool by_logit) {
+    const float l = logit(a, row + e);
+    return by_logit ? (double)l : score64(a, sm, l) + (a.bias ? (double)a.bias[e] : 0.0);
+}
+// The groups that stay, by f64: bit g for group g.
+__device__ __forceinline__ uint64_t groups64(const Exl3c4DevRoute& a, const Soft& sm, int64_t row, int lane) {
+    uint64_t mine = 0;                                           // lane g: group g's value
+#pragma unroll 1
+    for (int g = 0; g < a.n_group; ++g) {
         double v1 = -INFINITY, v2 = -INFINITY;
-        if (g < a.n_group)
-            for (int i = lane & (part - 1); i < a.group; i += part) {
-                const double v = value[g * a.group + i];
-                v2 = fmax(v2, fmin(v1, v));
-                v1 = fmax(v1, v);
-            }
-        wave_sync();                                             // read before the next token's values
-        for (int d = 1; d < part; d <<= 1) {
+#pragma unroll 1
+        for (int i = lane; i < a.group; i += 64) {
+            const int e = g * a.group + i;
+            if (is_out(logit(a, row + e)) || (a.bias && is_out(a.bias[e]))) continue;
+            const double v = choice64(a, sm, row, e, false);
+            v2 = fmax(v2, fmin(v1, v));
+            v1 = fmax(v1, v);
+        }
+#pragma unroll 1
+        for (int d = 1; d < 64; d <<= 1) {
             const double o1 = __shfl_xor(v1, d), o2 = __shfl_xor(v2, d);
             v2 = fmax(fmax(v2, o2), fmin(v1, o1));
             v1 = fmax(v1, o1);
         }
-        const double gv = top2 && v2 > -INFINITY ? v1 + v2 : v1;
-        const uint64_t gk = gv > -INFINITY ? order64(gv) : 0;
-        int ahead = 0;
-        for (int q = 0; q < a.n_group; ++q) {
-            const uint64_t o = readlane64(gk, q << a.part_log2);
-            ahead += o > gk || (o == gk && q < g) ? 1 : 0;
-        }
-        const uint64_t stay = __ballot(g < a.n_group && ahead < a.top_group);
+        const double gv = a.group_score == EXL3C4_GROUP_TOP2 && v2 > -INFINITY ? v1 + v2 : v1;
+        if (lane == g) mine = gv > -INFINITY ? order64(gv) : 0;
+    }
+    int ahead = 0;
+#pragma unroll 1
+    for (int q = 0; q < a.n_group; ++q) {
+        const uint64_t o = readlane64(mine, q);
+        ahead += o > mine || (o == mine && q < lane) ? 1 : 0;
+    }
+    return __ballot(lane < a.n_group && ahead < a.top_group);
+}
+
+// A candidate's key, id, logit and bias; behind the ranking its id and score.
+struct Cand { double s; float l, b; int id; };
+// One token by one wave: the experts e = lane + 64 j in registers. Lane r < top_k ends with the r-th expert and its weight. cand: the wave's 64 places
+// of LDS; value: its 64 RPL places (GROUPS).
+template <int RPL, bool GROUPS>
+__device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row, int lane, Cand* cand, float* value) {
+    // (loads past the last expert repeat it: a mask for each load would cost as much as the score)
+    float l[RPL], b[RPL];
+    const int E = a.n_expert;
+    int at[RPL];
+#pragma unroll
+    for (int j = 0; j < RPL; ++j) at[j] = j + 1 < RPL ? lane + 64 * j : min(lane + 64 * j, E - 1);
+    if (RPL > 1 && E <= 64 * (RPL - 1))                          // more than the last of a lane's can be past it
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) at[j] = min(lane + 64 * j, E - 1);
+    if (a.type == EXL3C4_F32) {
+        const float* p = (const float*)a.logits + row;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) l[j] = p[at[j]];
+    } else {
+        const uint16_t* p = (const uint16_t*)a.logits + row;
+        uint16_t h[RPL];
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) h[j] = p[at[j]];
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) l[j] = a.type == EXL3C4_BF16 ? __uint_as_float((uint32_t)h[j] << 16) : (float)__builtin_bit_cast(_Float16, h[j]);
+    }
+    const bool biased = a.bias != nullptr, soft = a.score == EXL3C4_SCORE_SOFTMAX, top2 = GROUPS && a.group_score == EXL3C4_GROUP_TOP2;
+#pragma unroll
+    for (int j = 0; j < RPL; ++j) b[j] = 0.f;
+    if (biased)
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) b[j] = a.bias[at[j]];
+    if (E < 64 * RPL)
+#pragma unroll
+        for (int j = 0; j < RPL; ++j)
+            if (lane + 64 * j >= E) l[j] = -INFINITY;
+    // s: the scores in f32, as far as something is ranked by them
+    Soft sm = { 0.f, 1.0 };
+    float s[RPL];
+    if (soft) {
+        sm.m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) sm.m = fmaxf(sm.m, l[j]);  // (a NaN never wins)
+        sm.m = fmaxf(sm.m, xor_lanef<32>(sm.m, lane));
+        sm.m = fmaxf(sm.m, xor_lanef<16>(sm.m, lane));
+        sm.m = fmaxf(sm.m, xor_lanef<8>(sm.m, lane));
+        sm.m = fmaxf(sm.m, xor_lanef<4>(sm.m, lane));
+        sm.m = fmaxf(sm.m, xor_lanef<2>(sm.m, lane));
+        sm.m = fmaxf(sm.m, xor_lanef<1>(sm.m, lane));
+        double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < RPL; ++j) {
-            const uint32_t of = (uint32_t)(lane + 64 * j) * a.group_inv >> 20;           // the expert's group (past the last expert: its key is 0)
-            if (!((stay >> ((of << a.part_log2) & 63)) & 1)) k[j] = 0;
+            const double e = is_out(l[j]) ? 0.0 : score64(a, sm, l[j]);
+            s[j] = is_out(l[j]) ? __builtin_nanf("") : (float)e;
+            sum += e;
+        }
+        sm.inv = inverse64(fmax(wave_sum(sum, lane), 1.0));        // (1 at least, but for a row that is out as a whole)
+        const float inv = (float)sm.inv;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) s[j] *= inv;
+    } else if (biased || top2) {
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) s[j] = sigmoid32(l[j]);
+    }
+    // c: the choices, NaN for an expert that is out. Without a bias they are the logits, and f32 is exact.
+    float c[RPL];
+#pragma unroll
+    for (int j = 0; j < RPL; ++j) {
+        c[j] = biased ? s[j] + b[j] : l[j];                      // (NaN where l or b is, which fminf passes over)
+        c[j] = fminf(l[j], b[j]) > -INFINITY ? c[j] : __builtin_nanf("");
+    }
+    if constexpr (GROUPS) {
+        // the values by expert through LDS; then of 2^groups_log2 lanes, 64 >> groups_log2 times over, lane g finds group g's two largest in a part of it
+        const bool exact = !biased && !top2;
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) value[lane + 64 * j] = c[j] != c[j] ? -INFINITY : biased || exact ? c[j] : s[j];
+        wave_sync();
+        const int g = lane & ((1 << a.groups_log2) - 1), parts = 64 >> a.groups_log2;
+        float v1 = -INFINITY, v2 = -INFINITY;
+        if (g < a.n_group)
+            for (int i = lane >> a.groups_log2; i < a.group; i += parts) {
+                const float v = value[g * a.group + i];
+                v2 = fmaxf(v2, fminf(v1, v));
+                v1 = fmaxf(v1, v);
+            }
+        wave_sync();                                             // read before the next token's values
+        auto meet = [&](float o1, float o2) {
+            v2 = fmaxf(fmaxf(v2, o2), fminf(v1, o1));
+            v1 = fmaxf(v1, o1);
+        };
+        if (a.groups_log2 < 6) meet(xor_lanef<32>(v1, lane), xor_lanef<32>(v2, lane));
+        if (a.groups_log2 < 5) meet(xor_lanef<16>(v1, lane), xor_lanef<16>(v2, lane));
+        if (a.groups_log2 < 4) meet(xor_lanef<8>(v1, lane), xor_lanef<8>(v2, lane));
+        if (a.groups_log2 < 3) meet(xor_lanef<4>(v1, lane), xor_lanef<4>(v2, lane));
+        if (a.groups_log2 < 2) meet(xor_lanef<2>(v1, lane), xor_lanef<2>(v2, lane));
+        const float gv = top2 && v2 > -INFINITY ? v1 + v2 : v1;
+        // Twice the error of its value, from two choices': of two groups that f32 may have in the wrong order the one that is less certain sees it.
+        const float near = exact || gv == INFINITY || gv == -INFINITY ? 0.f : 0x1p-19f + 0x1p-21f * (fabsf(v1) + (top2 && v2 > -INFINITY ? fabsf(v2) : 0.f));
+        const float above = gv + near, below = gv - near;
+        int ahead = 0, beside = 0;                               // groups ahead for sure; ahead or too close to tell (its own among them)
+        if (exact) {
+            for (int q = 0; q < a.n_group; ++q) {
+                const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gv), q));
+                ahead += o > gv || (o == gv && q < g) ? 1 : 0;
+            }
+        } else {
+            for (int q = 0; q < a.n_group; ++q) {
+                const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gv), q));
+                ahead += o > above ? 1 : 0;
+                beside += o >= below ? 1 : 0;
+            }
+            // those without an expert come last, by number; a single one that is certain has itself beside it
+            if (gv == -INFINITY) {
+                for (int q = 0; q < g; ++q) ahead += __builtin_amdgcn_readlane(__float_as_uint(gv), q) == __float_as_uint(-INFINITY) ? 1 : 0;
+                beside = ahead + 1;
+            }
+        }
+        uint64_t stay = __ballot(g < a.n_group && ahead < a.top_group);      // bit g: group g (and again for each part)
+        if (!exact && __any(g < a.n_group && ahead < a.top_group && beside > a.top_group)) stay = groups64(a, sm, row, lane);
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) {
+            const uint32_t of = (uint32_t)(lane + 64 * j) * a.group_inv >> 20;     // the expert's group (past the last expert: c is NaN)
+            const uint32_t word = a.n_group > 32 && of > 31 ? (uint32_t)(stay >> 32) : (uint32_t)stay;
+            if (!((word >> (of & 31)) & 1)) c[j] = __builtin_nanf("");
         }
     }
-    // As in route_token: the top_k keys have a high word of at least thr, the top_k-th largest of the lanes' own largest; those candidates are gathered
-    // one a lane and ranked (equal keys by id), more than 64 of them by top_k rounds of a wave maximum.
-    uint64_t most = 0;
+    // At least top_k experts have a choice of thr, the top_k-th largest of the lanes' own largest. Whoever is among the first top_k is so by less than twice
+    // the error below it: those are gathered one a lane and ranked in f64, equal ones by id; more than 64 of them by top_k rounds of a wave maximum.
+    float most = c[0];
 #pragma unroll
-    for (int j = 0; j < RPL; ++j) most = k[j] > most ? k[j] : most;
-    const uint32_t thr = (uint32_t)__builtin_amdgcn_readlane((int)sort_desc32((uint32_t)(most >> 32), lane), a.top_k - 1);
+    for (int j = 1; j < RPL; ++j) most = fmaxf(most, c[j]);
+    const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)sort_desc32(order32(most), lane), a.top_k - 1);
+    float thr = kth ? value_of32(kth) : -INFINITY;
+    if (biased && thr < INFINITY && kth) thr -= 2.f * error_of(thr) + 0x1p-22f * fabsf(thr);        // (and the subtraction's own rounding)
     int n = 0;
 #pragma unroll
     for (int j = 0; j < RPL; ++j) {
-        const bool c = k[j] != 0 && (uint32_t)(k[j] >> 32) >= thr;
-        const uint64_t bal = __ballot(c);
+        const bool in = c[j] >= thr;
+        const uint64_t bal = __ballot(in);
         const int at = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0));
-        if (c && at < 64) {
-            key[at] = k[j];
-            id[at] = lane + 64 * j;
-        }
+        if (in && at < 64) cand[at].l = l[j], cand[at].b = b[j], cand[at].id = lane + 64 * j;
         n += __popcll(bal);
     }
     wave_sync();
     int mine = -1;
+    double w = 0.0;
     if (n <= 64) {
-        const uint64_t ck = lane < n ? key[lane] : 0;
-        const int ce = lane < n ? id[lane] : 0x7FFFFFFF;
+        Cand own = { 0.0, 0.f, 0.f, 0x7FFFFFFF };
+        uint64_t ck = 0;
+        if (lane < n) {
+            own = cand[lane];
+            own.s = score64(a, sm, own.l);
+            ck = order64(biased ? own.s + (double)own.b : (double)own.l);
+        }
         int rank = 0;
-        for (int c = 0; c < n; ++c) {
-            const uint64_t o = readlane64(ck, c);
-            const int oe = __builtin_amdgcn_readlane(ce, c);
-            rank += o > ck || (o == ck && oe < ce) ? 1 : 0;
+        for (int q = 0; q < n; ++q) {                            // (ids ascend neither in the candidates nor in the lanes: ties are rare, and looked at apart)
+            const uint64_t o = readlane64(ck, q);
+            rank += o > ck ? 1 : 0;
+            if (__any(lane < n && o == ck && lane != q)) {
+                const int oe = __builtin_amdgcn_readlane(own.id, q);
+                rank += o == ck && oe < own.id ? 1 : 0;
+            }
         }
         wave_sync();
-        if (lane < n) id[rank] = ce;
+        if (lane < n) cand[rank].s = own.s, cand[rank].id = own.id;
         wave_sync();
-        if (lane < n && lane < a.top_k) mine = id[lane];
+        if (lane < n && lane < a.top_k) mine = cand[lane].id, w = cand[lane].s;
     } else {
+        uint32_t in = 0;                                         // which of the lane's experts can be chosen
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) in |= (c[j] == c[j] ? 1u : 0u) << j;
         uint64_t last = ~(uint64_t)0;
         int last_id = -1;
+#pragma unroll 1
         for (int r = 0; r < a.top_k; ++r) {
             uint64_t best = 0;
             int at = 0x7FFFFFFF;                                 // (ids ascend with j: the first of equal keys is the lowest)
-#pragma unroll
+#pragma unroll 1
             for (int j = 0; j < RPL; ++j) {
                 const int e = lane + 64 * j;
-                if ((k[j] < last || (k[j] == last && e > last_id)) && k[j] > best) best = k[j], at = e;
+                const uint64_t k = in >> j & 1 ? order64(choice64(a, sm, row, e, !biased)) : 0;
+                if ((k < last || (k == last && e > last_id)) && k > best) best = k, at = e;
             }
-#pragma unroll
+#pragma unroll 1
             for (int d = 32; d >= 1; d >>= 1) {
                 const uint64_t o = shfl_xor64(best, d);
                 const int oe = __shfl_xor(at, d);
@@ -575,13 +691,9 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
             last_id = at;
             if (lane == r && best != 0) mine = at;
         }
+        if (mine >= 0) w = score64(a, sm, logit(a, row + mine));
     }
     wave_sync();                                                 // read before the next token's
-    double w = 0.0;
-    if (mine >= 0) {
-        const float v = logit(a, row + mine);
-        w = soft ? exp64(v == (float)m ? 0.0 : (double)v - m) * inv : sigmoid64(v);
-    }
     if (a.renorm) {
         const double sum = wave_sum(w, lane);
         w = sum > 0.0 ? w / sum : 0.0;
@@ -592,13 +704,12 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
 // A wave a token.
 template <int RPL, bool GROUPS>
 __global__ __launch_bounds__(256) void k_score(Exl3c4DevRoute a) {
-    __shared__ uint64_t key[4][64];
-    __shared__ int id[4][64];
-    __shared__ double value[4][GROUPS ? 64 * RPL : 1];
+    __shared__ Cand cand[4][64];
+    __shared__ float value[4][GROUPS ? 64 * RPL : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t t = (int64_t)blockIdx.x * 4 + wave;
     if (t >= a.n_tok) return;
-    const Pick p = score_token<RPL, GROUPS>(a, t * a.pitch, lane, key[wave], id[wave], value[wave]);
+    const Pick p = score_token<RPL, GROUPS>(a, t * a.pitch, lane, cand[wave], value[wave]);
     if (lane < a.top_k) {
         a.ids[t * a.top_k + lane] = p.id;
         a.w[t * a.top_k + lane] = p.w;
@@ -608,14 +719,13 @@ __global__ __launch_bounds__(256) void k_score(Exl3c4DevRoute a) {
 // With the scatter, for at most 16 tokens, in one workgroup (as k_route_scatter).
 template <int RPL, bool GROUPS>
 __global__ __launch_bounds__(1024) void k_score_scatter(Exl3c4DevRoute a) {
-    __shared__ uint64_t key[16][64];
-    __shared__ int id[16][64];
-    __shared__ double value[16][GROUPS ? 64 * RPL : 1];
+    __shared__ Cand cand[16][64];
+    __shared__ float value[16][GROUPS ? 64 * RPL : 1];
     __shared__ int ids_l[16 * 64], cnt[64 * RPL + 17];
     const int lane = threadIdx.x & 63, t = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < a.n_expert; i += blockDim.x) cnt[i] = 0;
     if (t < a.n_tok) {
-        const Pick p = score_token<RPL, GROUPS>(a, (int64_t)t * a.pitch, lane, key[t], id[t], value[t]);
+        const Pick p = score_token<RPL, GROUPS>(a, (int64_t)t * a.pitch, lane, cand[t], value[t]);
         if (lane < a.top_k) {
             a.ids[t * a.top_k + lane] = p.id;
             a.w[t * a.top_k + lane] = p.w;
@@ -727,7 +837,10 @@ extern "C" int exl3c4_dev_scatter(const int32_t* ids, int64_t T, int64_t base, i
     const int64_t segs = T > 0 ? (T + SC_SEG - 1) / SC_SEG : 1;
     const int64_t per = row_of == ids ? segs : (segs + SC_MAX_WG - 1) / SC_MAX_WG;
     const unsigned wgs = (unsigned)((segs + per - 1) / per);
-    const auto f = T <= SC_THREADS ? k_scatter<1> : T <= 4 * SC_THREADS ? k_scatter<4> : k_scatter<16>;
+    const bool far = base < INT32_MIN || base > INT32_MAX;
+    const auto f = T <= SC_THREADS       ? (far ? k_scatter<1, true> : k_scatter<1, false>)
+                   : T <= 4 * SC_THREADS ? (far ? k_scatter<4, true> : k_scatter<4, false>)
+                                         : (far ? k_scatter<16, true> : k_scatter<16, false>);
     hipLaunchKernelGGL(f, dim3(wgs), dim3(SC_THREADS), 0, (hipStream_t)stream, ids, (uint32_t)T, base, n_expert,
                        (uint32_t)(per * SC_SEG), sorted, off, count, row_of);
     return launched();

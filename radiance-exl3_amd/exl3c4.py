@@ -141,16 +141,21 @@ class F8:
         return F8, (self.codes, self.scales, self.cols, self.block)
 
     def planes(self):
-        """The C side's view of the planes as they are now."""
-        q = self._planes
+        """A reference to the C side's view of the planes as they are now."""
+        q = self._planes                                       # [the struct, the reference, the addresses that it holds]
         if q is None:
             if self.scales.shape[-2] != (self.rows + self.block - 1) // self.block:
                 raise ValueError("the scales have other rows of blocks than these rows: view gate and up as the two matrices that they are")
             cm, sm = _matrices(self.codes), _matrices(self.scales)
-            q = F8Planes(self.mats, self.rows, self.cols, self.block, None, cm[0], cm[1], None, sm[0], sm[1])
+            view = F8Planes(self.mats, self.rows, self.cols, self.block, None, cm[0], cm[1], None, sm[0], sm[1])
+            q = [view, C.byref(view), None, None]
             super().__setattr__("_planes", q)
-        q.codes, q.scales = self.codes.data_ptr(), self.scales.data_ptr()
-        return q
+        codes, scales = self.codes.data_ptr(), self.scales.data_ptr()
+        if codes != q[2]:
+            q[0].codes = q[2] = codes
+        if scales != q[3]:
+            q[0].scales = q[3] = scales
+        return q[1]
 
 
 def lib():
@@ -688,8 +693,7 @@ def _convert_f8(fn, v, q: F8, stream, quant: bool) -> int:
     dt = _dtypes.get(v.dtype)
     if dt is None:
         dt = _dt(v)
-    planes = C.byref(q.planes())
-    args = (v.data_ptr(), dt, pitch, stride, planes) if quant else (planes, v.data_ptr(), dt, pitch, stride)
+    args = (v.data_ptr(), dt, pitch, stride, q.planes()) if quant else (q.planes(), v.data_ptr(), dt, pitch, stride)
     if stream is not None and dev == _cuda.current_device():
         return fn(*args, stream.cuda_stream)
     return _launch_on(v.device, stream, fn, *args)

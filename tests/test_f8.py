@@ -85,7 +85,7 @@ def test_no_rows_launch_nothing():
 @pytest.mark.parametrize("change", [{"T": 1 << 20, "x_rows": 1 << 20, "n_expert": 1 << 20}, {"T": 1 << 30, "x_rows": 1 << 30, "n_expert": 1}],
                          ids=["rows", "tiles"])
 def test_more_threads_than_a_launch_holds_are_refused(change):
-    n = 1024 if change["n_expert"] > 1 else 1 << 16
+    n = 1 << 14 if change["n_expert"] > 1 else 1 << 16
     assert rc(gemm(N=n, y_pitch=n, w_stride=n * 272, ws_stride=n // 128 * 12, **change)) == SHAPE
 
 

@@ -182,3 +182,52 @@ def test_streams_and_a_replayed_graph(ex):
             want = routeref.scatter(wi, 256)
             assert np.array_equal(ids.view(n_tok, 8).cpu().numpy(), wi)
             assert np.array_equal(so.cpu().numpy(), want[0]) and np.array_equal(off.cpu().numpy(), want[1]) and np.array_equal(row.cpu().numpy(), want[3])
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_groups_whose_sums_32_bits_do_not_tell_apart(ex, score):
+    """Biases of unlike sign and size whose pairs bring each group's sum to within some 2^-28 of the others', among them exactly equal ones."""
+    g = torch.Generator().manual_seed(8)
+    l = torch.randn((12, 64), generator=g)
+    s = torch.sigmoid(l.double()) if score == "sigmoid" else torch.softmax(l.double(), 1)
+    for t in range(12):
+        for big in (0.0, 3.0, 40.0):
+            b = torch.full((64,), -100.0, dtype=torch.float64)
+            for grp in range(16):                                # two experts a group that count: one up, one down
+                b[4 * grp] = big + 0.5 - s[t, 4 * grp]
+                b[4 * grp + 1] = -big + 0.25 - s[t, 4 * grp + 1]
+            check(ex, l[t:t + 1].cuda(), 6, score, b.float().cuda(), 16, 5, "top2")
+            check(ex, l[t:t + 1].cuda(), 6, score, b.float().cuda(), 16, 5, "max")
+    same = torch.randn((1, 4), generator=g).repeat(3, 16)            # every group the same
+    check(ex, same.cuda(), 9, score, None, 16, 3, "top2")
+    check(ex, same.cuda(), 9, score, torch.randn(4, generator=g).repeat(16).cuda(), 16, 3, "top2")
+
+
+@pytest.mark.parametrize("n_tok", [3, 40])
+@pytest.mark.parametrize("E", [65, 100, 129, 192, 193, 257, 320, 511, 513, 700, 961])
+def test_experts_that_do_not_fill_the_registers(ex, n_tok, E):
+    g = torch.Generator().manual_seed(E)
+    l = torch.randn((n_tok, E), generator=g)
+    l[:, -1] += 3                                                   # the last one is often chosen
+    b = (torch.randn(E, generator=g) * 0.1).cuda()
+    check(ex, l.cuda(), min(8, E), "sigmoid", b)
+    check(ex, l.bfloat16().cuda(), min(8, E), "softmax", b)
+    check(ex, l.half().cuda(), min(8, E), "softmax")
+
+
+@pytest.mark.parametrize("base", [-2 ** 31 - 2, -2 ** 31, -5, 2 ** 31 - 40, 2 ** 31 - 1, 2 ** 31, 2 ** 40, -2 ** 40])
+def test_the_scatters_base_over_its_range(ex, base):
+    """Ids over the whole of 32 bits against bases at its ends and beyond."""
+    rng = np.random.default_rng(1)
+    ids = rng.integers(-2 ** 31, 2 ** 31, (300, 6)).astype(np.int32)
+    near = np.clip(base + rng.integers(-3, 60, ids.shape), -2 ** 31, 2 ** 31 - 1).astype(np.int32)
+    ids = np.where(rng.random(ids.shape) < 0.7, near, ids)
+    E, T = 50, ids.size
+    g = ids.reshape(-1).astype(np.int64) - base
+    want = routeref.scatter(np.where((g >= 0) & (g < E), g, -1).reshape(ids.shape), E)
+    i = torch.from_numpy(ids).cuda()
+    st, off, cnt, row = (torch.full((n,), -9, dtype=torch.int32, device="cuda") for n in (T, E + 1, E, T))
+    assert ex.moe_scatter(i, E, st, off, cnt, row, base) == 0
+    torch.cuda.synchronize()
+    for got, w in zip((st, off, cnt, row), want):
+        assert np.array_equal(got.cpu().numpy(), w)
