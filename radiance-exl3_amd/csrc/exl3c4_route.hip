@@ -243,7 +243,28 @@ __global__ __launch_bounds__(SC_THREADS) void k_scatter(const int32_t* ids, uint
     const int mine = tid < SC_SEG && lo + tid < hi ? ids[lo + tid] : 0;   // the first SC_SEG pairs, loaded ahead
     hist[tid] = hist[SC_THREADS + tid] = 0;
     __syncthreads();
-    for (uint32_t i0 = 0; i0 < T; i0 += SC_THREADS * LOADS) {
+    uint32_t counted = 0;
+    if constexpr (LOADS == 16) {
+        // whole rounds of four ids a thread, four rounds' loads out together; a wave's 256 ids lie before the segment or not (it starts at a multiple)
+        struct __attribute__((packed, aligned(4))) Four { int32_t v[4]; };
+        constexpr uint32_t ROUND = 4 * SC_THREADS;
+        auto count = [&](const Four& q, uint32_t i0) {
+            int* h = hist + (__builtin_amdgcn_readfirstlane(i0 + 256 * wv) < lo ? 0 : SC_THREADS);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = expert_of<FAR>(q.v[j], base, n_expert);
+                if (e >= 0) atomicAdd(&h[e], 1);
+            }
+        };
+        for (; counted + 4 * ROUND <= T; counted += 4 * ROUND) {
+            Four q[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q[r] = *(const Four*)(ids + counted + r * ROUND + 4 * tid);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) count(q[r], counted + r * ROUND);
+        }
+    }
+    for (uint32_t i0 = counted; i0 < T; i0 += SC_THREADS * LOADS) {
         int32_t f[LOADS];
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
