@@ -391,6 +391,39 @@ __global__ __launch_bounds__(64 * WAVES) void k_mg_rows(Exl3c4DevGemm a) {
 // 181 -> 172, but a workgroup less a CU: 2048 Zipf 153 -> 163). Neither the rows' pitch (K = 2048 against 2112) nor the order within
 // a line changes the loads' rate.
 template <bool B> struct Is { static constexpr bool value = B; };
+// A lane holds columns 16 n + 4 g .. + 3 of row 16 (m0 + m) + l16 of the tile (SwiGLU: of gate tile 2 n and up tile 2 n + 1); col0: the wave's
+// first column of y. 16 rows at a time cross LDS, in the wave's own part of it (`rows`, TILE_ROWS floats), so that a row's columns go out together, and what
+// differs by type and edge is code for one store (stores straight from the lanes, 8 bytes a row each, took the same time and 30 times the code).
+template <bool SW, int TN> constexpr int TILE_ROWS = 16 * (16 * (SW ? TN / 2 : TN) + 4);
+template <bool SW, int TM, int TN>
+__device__ __forceinline__ void store_tile(const Exl3c4DevGemm& a, const Chunk& ch, const int* rows_x, float* rows, const f32x4 (&acc)[TN][TM],
+                                           int m0, int col0, int lane) {
+    constexpr int TO = SW ? TN / 2 : TN, LANES = 4 * TO, PITCH = 16 * TO + 4;
+    const int l16 = lane & 15, g = lane >> 4;
+    const int ysz = a.y_type == EXL3C4_F32 ? 4 : 2;
+    const bool whole = ((uintptr_t)a.y | (uintptr_t)a.y_pitch) % (4 * ysz) == 0;      // four columns are one aligned store
+    const int col = col0 + 4 * (lane % LANES);
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+#pragma unroll
+        for (int n = 0; n < TO; ++n) {
+            f32x4 v = SW ? acc[2 * n][m] : acc[n][m];
+            if (SW) v = swiglu4(v, acc[SW ? 2 * n + 1 : n][m]);
+            *(f32x4*)(rows + l16 * PITCH + 16 * n + 4 * g) = v;
+        }
+        wave_sync();                                             // other lanes read what a lane has written
+#pragma unroll 1
+        for (int i = 0; i < TO; ++i) {
+            const int q = i * (64 / LANES) + lane / LANES, r = (m0 + m) * 16 + q;
+            f32x4 v = *(const f32x4*)(rows + q * PITCH + 4 * (lane % LANES));
+            if (r >= ch.rows) continue;
+            if (rows_x[r] < 0) v = f32x4{ 0, 0, 0, 0 };
+            store4(a.y + (int64_t)(ch.row0 + r) * a.y_pitch + (int64_t)col * ysz, a.y_type, v, a.n_out - col, whole);
+        }
+        wave_sync();                                             // and are done before it is written again
+    }
+}
+
 template <int XT, int WT, bool SW, int MT_LOG2, int NT, int WM, int WN, int BUFS> struct Tile {
     static constexpr int MT = 1 << MT_LOG2, WAVES_ = WM * WN;
     static constexpr bool MIXED = WT == MX4 && XT != MX4;

@@ -202,6 +202,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_f8_rows(Exl3c4DevGemm a) {
     }
 }
 
+// Two values in 16 bits each.
+template <int T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (T == BF16) return __builtin_bit_cast(uint32_t, bf2_t{ (__bf16)lo, (__bf16)hi });
+    else return __builtin_bit_cast(uint32_t, half2_t{ (_Float16)lo, (_Float16)hi });
+}
+
 // ------------------------------------------------------------------------------------------ many rows an expert
 // A workgroup: a tile of MT rows of one expert against NT weight rows (with SwiGLU 16 gate rows and their 16 up rows in turn, so that a lane holds
 // both), k in stages of one block of 128 columns. A stage's rows and scales go from memory to LDS without registers. A wave reads its weight rows into
@@ -423,9 +429,48 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             slot_x = slot_x + 1 == XB ? 0 : slot_x + 1;
         }
     }
-    static_assert(WV * TILE_ROWS<SW, TN> * 4 <= (int)sizeof(lds), "the rows fit the stages' buffers");
-    __syncthreads();
-    store_tile<SW, TM, TN>(a, ch, rows_x, (float*)lds + wave * TILE_ROWS<SW, TN>, acc, wm * TM, n0 + wn * (SW ? TN / 2 : TN) * 16, lane);
+    // A lane holds columns 16 n + 4 g .. + 3 of row 16 m + l16 of the wave's (SwiGLU: of gate tile 2 n and up tile 2 n + 1). PM row tiles at a time cross
+    // LDS in y's type, so that whole rows of the tile go out by 16 bytes a lane (8 bytes a lane from each wave's own columns: 613 tokens Zipf, 2560 x
+    // 640, STORE_US).
+    constexpr int TO = SW ? TN / 2 : TN, OC = 16 * TO * WN, MOST = WIDE ? 4 : 2;      // (y is f32 where the codes are widened only)
+    constexpr int FIT = G::LDS / (16 * (OC * MOST + 16)), PM = FIT >= TM ? TM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
+    static_assert(WM == 1 && FIT >= 1 && TM % PM == 0, "a pass's rows fit");
+    const int size_log2 = MOST == 4 && a.y_type == EXL3C4_F32 ? 2 : 1, pitch = (OC << size_log2) + 16;
+    const int per_log2 = 4 - size_log2, row_log2 = __builtin_ctz(OC) - per_log2;      // columns in 16 bytes; 16 bytes a row
+    struct __attribute__((packed, aligned(2))) Part { uint32_t v[4]; };
+#pragma unroll
+    for (int m0 = 0; m0 < TM; m0 += PM) {
+        __syncthreads();                                         // the stages, or the pass before, are read
+#pragma unroll
+        for (int m = m0; m < m0 + PM; ++m)
+#pragma unroll
+            for (int n = 0; n < TO; ++n) {
+                f32x4 v = SW ? acc[2 * n][m] : acc[n][m];
+                if (SW) v = swiglu4(v, acc[SW ? 2 * n + 1 : n][m]);
+                char* p = lds + ((m - m0) * 16 + l16) * pitch + ((wn * TO * 16 + 16 * n + 4 * g) << size_log2);
+                if (size_log2 == 2) *(f32x4*)p = v;
+                else *(uint2*)p = a.y_type == BF16 ? uint2{ pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]) } : uint2{ pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]) };
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * PM << row_log2; i += 64 * WV) {
+            const int q = i >> row_log2, r = 16 * m0 + q, c = (i & ((1 << row_log2) - 1)) << per_log2, col = n0 + c;
+            if (r >= ch.rows || col >= a.n_out) continue;
+            Part v = *(const Part*)__builtin_assume_aligned(lds + q * pitch + (c << size_log2), 16);
+            if (rows_x[r] < 0) v = Part{ { 0, 0, 0, 0 } };
+            char* y = a.y + (int64_t)(ch.row0 + r) * a.y_pitch + ((int64_t)col << size_log2);
+            if (col + (1 << per_log2) <= a.n_out) {
+                *(Part*)y = v;
+            } else if (size_log2 == 2) {
+#pragma unroll
+                for (int u = 0; u < 3; ++u)
+                    if (col + u < a.n_out) ((uint32_t*)y)[u] = v.v[u];
+            } else {
+#pragma unroll
+                for (int u = 0; u < 7; ++u)
+                    if (col + u < a.n_out) ((uint16_t*)y)[u] = (uint16_t)(v.v[u >> 1] >> (16 * (u & 1)));
+            }
+        }
+    }
 }
 
 template <int XT, bool SW, int NS>
