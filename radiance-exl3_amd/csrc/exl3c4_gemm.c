@@ -47,6 +47,11 @@ int exl3c4_mx4_dequant(const void* codes, int64_t codes_pitch, const void* scale
                                   out, out_dtype, out_pitch, stream);
 }
 
+/* Whether matrices stride apart, of rows pitch apart (at least 1) that end after `last`, overlap (pitch * rows may pass 64 bits). */
+static int overlap(int64_t stride, int64_t rows, int64_t pitch, int64_t last) {
+    return stride < last || (stride - last) / pitch < rows - 1;
+}
+
 /* The F8 planes of n matrices and their values: what both conversions refuse, then the launch's block. */
 static int f8_check(const Exl3c4F8* q, const void* v, int32_t dtype, int64_t pitch, int64_t stride, Exl3c4DevF8* a) {
     if (!q || (q->block != 1 && q->block != 128)) return EXL3C4_E_INVAL;
@@ -58,14 +63,15 @@ static int f8_check(const Exl3c4F8* q, const void* v, int32_t dtype, int64_t pit
     if (q->n * q->rows > 0 && (!q->codes || !q->scales || !v)) return EXL3C4_E_INVAL;
     if (pitch < q->cols || q->codes_pitch < code_cols || q->scales_pitch < across) return EXL3C4_E_STRIDE;
     if (pitch > MAX_PITCH || q->codes_pitch > MAX_PITCH || q->scales_pitch > MAX_PITCH) return EXL3C4_E_STRIDE;
-    if (q->n > 1 && q->rows > 0) {                            /* a matrix's last row ends with its last column */
+    const int apart = q->n > 1 && q->rows > 0;
+    if (apart) {                                              /* a matrix's last row ends with its last column */
         const int64_t most = (int64_t)1 << 60;
         if (stride > most || q->codes_stride > most || q->scales_stride > most) return EXL3C4_E_STRIDE;
-        if (stride < (q->rows - 1) * pitch + q->cols || q->codes_stride < (q->rows - 1) * q->codes_pitch + code_cols ||
-            q->scales_stride < (down - 1) * q->scales_pitch + across)
+        if (overlap(stride, q->rows, pitch, q->cols) || overlap(q->codes_stride, q->rows, q->codes_pitch, code_cols) ||
+            overlap(q->scales_stride, down, q->scales_pitch, across))
             return EXL3C4_E_STRIDE;
     }
-    if ((uintptr_t)v % (uintptr_t)size_of(dtype) || (uintptr_t)q->codes % 16 || q->codes_pitch % 16 || (q->n > 1 && q->codes_stride % 16) ||
+    if ((uintptr_t)v % (uintptr_t)size_of(dtype) || (uintptr_t)q->codes % 16 || q->codes_pitch % 16 || (apart && q->codes_stride % 16) ||
         (uintptr_t)q->scales % 4)
         return EXL3C4_E_ALIGN;
     const int64_t size = size_of(dtype);
@@ -75,9 +81,9 @@ static int f8_check(const Exl3c4F8* q, const void* v, int32_t dtype, int64_t pit
     a->v_pitch = pitch * size;
     a->codes_pitch = q->codes_pitch;
     a->scales_pitch = q->scales_pitch * 4;
-    a->v_stride = q->n > 1 ? stride * size : 0;
-    a->codes_stride = q->n > 1 ? q->codes_stride : 0;
-    a->scales_stride = q->n > 1 ? q->scales_stride * 4 : 0;
+    a->v_stride = apart ? stride * size : 0;
+    a->codes_stride = apart ? q->codes_stride : 0;
+    a->scales_stride = apart ? q->scales_stride * 4 : 0;
     a->n = (uint32_t)q->n;
     a->rows = (uint32_t)q->rows;
     a->cols = (uint32_t)q->cols;

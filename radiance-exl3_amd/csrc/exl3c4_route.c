@@ -88,6 +88,7 @@ int exl3c4_moe_route(const Exl3c4Route* r, void* stream) {
     if (r->n_group < 1 || r->n_group > 64 || r->n_expert % r->n_group || r->top_group < 1 || r->top_group > r->n_group ||
         r->top_k > r->top_group * (r->n_expert / r->n_group))
         return EXL3C4_E_SHAPE;
+    if (r->pitch > (int64_t)1 << 36) return EXL3C4_E_STRIDE;      /* past any memory; its products stay in 64 bits */
     if ((uintptr_t)r->bias % 4) return EXL3C4_E_ALIGN;
     const int scatter = r->expert_offset != NULL;
     if (!scatter && (r->sorted_tok || r->expert_count || r->row_of)) return EXL3C4_E_INVAL;

@@ -41,6 +41,14 @@ def test_conversions_refuse(change, want):
     assert conv(**change) == want
 
 
+@pytest.mark.parametrize("change", [{"pitch": 1 << 35, "xs": 1 << 40}, {"codes_pitch": 1 << 35, "codes_stride": 1 << 40},
+                                    {"scales_pitch": 1 << 40, "scales_stride": 1 << 41}, {"xs": -1}, {"codes_stride": -(1 << 62)}], ids=str)
+def test_matrices_that_overlap_are_refused_whatever_64_bits_hold(change):
+    """2^29 rows, 2^22 rows of blocks: (rows - 1) * pitch is 2^64 less the pitch (2^62 less it for the scales)."""
+    d = dict(n=2, rows=1 << 29, cols=100, pitch=100, xs=1 << 60, codes_pitch=112, codes_stride=1 << 60, scales_pitch=1, scales_stride=1 << 60)
+    assert conv(**d | change) == STRIDE
+
+
 def test_a_conversion_without_planes_is_refused():
     L = exl3c4.lib()
     assert L.exl3c4_f8_quant(P, 0, 300, 0, None, None) == INVAL and L.exl3c4_f8_dequant(None, P, 0, 300, 0, None) == INVAL

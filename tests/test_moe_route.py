@@ -39,6 +39,10 @@ def test_moe_route_refuses(change, want):
     assert route(**change) == want
 
 
+def test_a_pitch_past_any_memory_is_refused():
+    assert route(pitch=(1 << 36) + 1) == STRIDE and route(pitch=1 << 62) == STRIDE
+
+
 def test_no_tokens_without_a_scatter_launch_nothing():
     none = dict(sorted_tok=None, expert_offset=None, expert_count=None, row_of=None)
     assert route(n_tok=0, logits=None, expert_ids=None, expert_w=None, **none) == 0
