@@ -137,3 +137,78 @@ def test_planes_of_e4m3_tensors_and_another_stream(ex):
         c, s = f8ref.quant(x.cpu(), 1)
         v = f8ref.values(c, s, 256, 1)
         assert ((out.cpu().double() - v).abs() <= 2.0 ** -24 * v.abs()).all()
+
+
+def far(t, pitch, stride):
+    """t [mats, rows, cols] with its rows `pitch` and its matrices `stride` bytes apart."""
+    size = t.element_size()
+    v = torch.empty(t.shape[0] * stride // size, dtype=t.dtype, device="cuda").as_strided(t.shape, (stride // size, pitch // size, 1))
+    return v.copy_(t)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("block,rows,pitch,stride", [(1, 3, 1 << 31, 3 << 31), (128, 130, 1 << 25, 130 << 25), (1, 5, 1 << 12, 5 << 30), (128, 5, 1 << 12, 5 << 30)])
+def test_offsets_past_32_bits(ex, t, block, rows, pitch, stride):
+    """Rows and matrices more than 4 GiB apart: the codes, scales and values of the same without gaps."""
+    x = torch.randn((2, rows, 300), generator=torch.Generator().manual_seed(1)).to(TYPES[t]).cuda()
+    q = ex.f8_empty(x.shape, block)
+    assert ex.f8_quant(x, q) == 0
+    fq = ex.F8(far(torch.zeros_like(q.codes), pitch, stride), far(torch.zeros_like(q.scales), pitch, stride), 300, block)
+    assert ex.f8_quant(far(x, pitch, stride), fq) == 0
+    out, fout = torch.empty_like(x), far(torch.zeros_like(x), pitch, stride)
+    assert ex.f8_dequant(q, out) == 0 and ex.f8_dequant(fq, fout) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q.codes, fq.codes) and torch.equal(q.scales, fq.scales) and torch.equal(out, fout)
+    del fq, fout
+    torch.cuda.empty_cache()
+
+
+def test_more_values_than_one_launch_indexes(ex):
+    """2^17 slots of 16 bytes a row and 16,400 rows: a second launch from row 16,383 on."""
+    rows, cols, some = 16400, 1 << 20, [0, 5, 16382, 16383, 16384, 16399]
+    x = torch.empty((rows, cols), dtype=torch.float16, device="cuda").zero_()
+    part = torch.randn((len(some), cols), device="cuda").half()
+    for i, r in enumerate(some):
+        x[r] = part[i]
+    few, q = ex.f8_empty((len(some), cols), 1), ex.f8_empty((rows, cols), 1)
+    q.codes.fill_(0xA5)
+    assert ex.f8_quant(part, few) == 0 and ex.f8_quant(x, q) == 0
+    out = x.view(torch.bfloat16)
+    out.fill_(-7.0)
+    want = torch.empty((len(some), cols), dtype=torch.bfloat16, device="cuda")
+    assert ex.f8_dequant(few, want) == 0 and ex.f8_dequant(q, out) == 0
+    torch.cuda.synchronize()
+    for i, r in enumerate(some):
+        assert torch.equal(q.codes[r], few.codes[i]) and torch.equal(q.scales[r], few.scales[i]) and torch.equal(out[r], want[i])
+    for a, b in zip([-1] + some, some + [rows]):
+        for r in range(a + 1, b, 2048):
+            assert not q.codes[r:min(r + 2048, b)].any() and not out[r:min(r + 2048, b)].any()
+    del x, out, q
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("block", [1, 128])
+def test_replayed_graphs_beside_each_other(ex, block):
+    """Two captured graphs of both conversions, replayed on two streams at once several times, with new values in between."""
+    sets = []
+    for i in range(2):
+        x = torch.empty((2, 200 + i, 650), dtype=torch.bfloat16, device="cuda")
+        q, out, st, graph = ex.f8_empty(x.shape, block), torch.empty_like(x, dtype=torch.float32), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        x.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=st):
+            assert ex.f8_quant(x, q, st) == 0 and ex.f8_dequant(q, out, st) == 0
+        sets.append((x, q, out, st, graph))
+    for k in range(4):
+        for i, (x, q, out, st, graph) in enumerate(sets):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(10 * k + i)) * 2.0 ** (k - 2))
+        torch.cuda.synchronize()
+        for _, _, _, st, graph in sets:
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, q, out, _, _ in sets:
+            own, values = ex.f8_empty(x.shape, block), torch.empty_like(out)
+            assert ex.f8_quant(x, own) == 0 and ex.f8_dequant(own, values) == 0
+            torch.cuda.synchronize()
+            assert torch.equal(q.codes, own.codes) and torch.equal(q.scales, own.scales) and torch.equal(out, values)

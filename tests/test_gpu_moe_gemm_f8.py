@@ -286,3 +286,41 @@ def test_same_bits_on_two_streams_and_in_a_replayed_graph(ex):
         c, s = f8ref.quant(x.cpu()[None], 1)
         y, tol = f8ref.gemm(f8ref.values(c, s, 272, 1)[0], wv, order, off, 400, 2, True)
         assert mx4ref.close(ys[2].cpu(), y, tol)
+
+
+def far(t, pitch):
+    """t with its rows `pitch` bytes apart."""
+    n, size = t.shape[:-1].numel(), t.element_size()
+    strides = [pitch // size, 1]
+    for d in t.shape[1:-1][::-1]:
+        strides.insert(0, strides[0] * d)
+    v = torch.empty(n * pitch // size, dtype=t.dtype, device="cuda").as_strided(t.shape, strides)
+    return v.copy_(t)
+
+
+@pytest.mark.parametrize("xt,yt", [("f16", "f16"), ("bf16", "f32"), ("f8", "f32"), ("f8", "bf16")])
+@pytest.mark.parametrize("T,pitch", [(6, 1 << 30), (2600, 1 << 22)])
+def test_offsets_past_32_bits(ex, xt, yt, T, pitch):
+    """Rows of x, of y and of weights, scales and experts that lie more than 4 GiB apart: the bits of the same operands without gaps."""
+    E, N, K = 2, 40, 256
+    assert path(ex, xt, yt, False, T, E, N, K) == (2 if T == 6 else 32)
+    g = torch.Generator().manual_seed(7)
+    off = torch.tensor([0, T // 3, T], dtype=torch.int32, device="cuda")
+    x = torch.randn((T, K), generator=g).cuda()
+    if xt == "f8":
+        q = ex.f8_empty((T, K), 1)
+        assert ex.f8_quant(x, q) == 0
+        xs = q, ex.F8(far(q.codes, pitch), far(q.scales, pitch), K, 1)
+    else:
+        x = x.to(TYPES[xt])
+        xs = x, far(x, pitch)
+    w = w_operand(ex, g, E, N, K, False)[0]
+    wf = ex.F8(far(w.codes, 1 << 27), far(w.scales, 1 << 27), K, 128)
+    outs = []
+    for xq, wq, y in ((xs[0], w, torch.empty((T, N), dtype=TYPES[yt], device="cuda")), (xs[1], wf, far(torch.zeros((T, N), dtype=TYPES[yt], device="cuda"), pitch))):
+        assert ex.moe_gemm(ex.make_gemm(xq, wq, None, off, y)) == 0
+        torch.cuda.synchronize()
+        outs.append(y.cpu())
+    assert not outs[0].isnan().any() and torch.equal(*outs)
+    del xs, w, wf, x, xq, wq, y
+    torch.cuda.empty_cache()

@@ -231,3 +231,15 @@ def test_the_scatters_base_over_its_range(ex, base):
     torch.cuda.synchronize()
     for got, w in zip((st, off, cnt, row), want):
         assert np.array_equal(got.cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("n_tok", [16, 20])
+@pytest.mark.parametrize("t", list(TYPES))
+def test_rows_past_32_bits(ex, t, n_tok):
+    """Rows of logits 512 MiB apart."""
+    pitch = (1 << 29) // torch.empty((), dtype=TYPES[t]).element_size()
+    l = torch.empty(n_tok * pitch, dtype=TYPES[t], device="cuda").as_strided((n_tok, 96), (pitch, 1))
+    l.copy_(torch.randn((n_tok, 96), generator=torch.Generator().manual_seed(3)) * 2)
+    check(ex, l, 6, "sigmoid", (torch.arange(96) % 7).float().cuda() * 0.01, 8, 3, "top2")
+    del l
+    torch.cuda.empty_cache()
