@@ -430,8 +430,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
         }
     }
     // A lane holds columns 16 n + 4 g .. + 3 of row 16 m + l16 of the wave's (SwiGLU: of gate tile 2 n and up tile 2 n + 1). PM row tiles at a time cross
-    // LDS in y's type, so that whole rows of the tile go out by 16 bytes a lane (8 bytes a lane from each wave's own columns: 613 tokens Zipf, 2560 x
-    // 640, STORE_US).
+    // LDS in y's type, so that whole rows of the tile go out by 16 bytes a lane (8192 tokens over 8 experts, 2048 x 1408: 78 us with 8 bytes a lane
+    // from each wave's own columns, 68 so; 2816 x 2048 with SwiGLU 115 and 111; 2560 x 640 over 512 experts the same).
     constexpr int TO = SW ? TN / 2 : TN, OC = 16 * TO * WN, MOST = WIDE ? 4 : 2;      // (y is f32 where the codes are widened only)
     constexpr int FIT = G::LDS / (16 * (OC * MOST + 16)), PM = FIT >= TM ? TM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
     static_assert(WM == 1 && FIT >= 1 && TM % PM == 0, "a pass's rows fit");
