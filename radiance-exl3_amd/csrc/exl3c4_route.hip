@@ -331,6 +331,146 @@ __global__ __launch_bounds__(SC_THREADS) void k_scatter(const int32_t* ids, uint
     for (uint32_t i = live + blockIdx.x * SC_THREADS + tid; i < T; i += gridDim.x * SC_THREADS) sorted[i] = -1;
 }
 
+// moe_scatter by experts: a workgroup takes PO_EXPERTS or fewer neighbouring experts and reads every pair's id, each wave a part of the pairs. It counts the
+// pairs of lower experts, whose sum is its first row, and lists its own in LDS in their order; what the waves before it found then places each. Three
+// instructions an id (two comparisons and a count) in place of an LDS atomic, and no ranks among the pairs of a segment. What bounds it: every CU reads
+// all ids, 3.8 us of L2's rate for 81,920 pairs, and the same again goes into the pairs found.
+// k_scatter against it, us a launch (pairs, experts): 1, 512 2.8 / 3.2; 10, 512 2.9 / 3.3; 32, 8 3.2 / 3.3; 80, 512 3.9 / 3.5; 1,280 4.9 / 3.6; 6,130 6.3 / 4.2;
+// 20,480 7.7 / 5.8; 81,920 13.1 / 11.1 (a fifth of them on one expert 22 / 23, all 75 / 54); 200,000 28 / 22 (50 / 129: a list no longer holds a wave's own);
+// 49,152, 64 9.6 / 9.3 (20 / 14). Pairs of which seven eighths are no expert's, whose places one workgroup fills: 81,920, 64 12.5 / 13.1; 65,536, 32 9.4 / 11.7;
+// 131,072 pairs of 8 experts 31 / 93, for few workgroups place.
+constexpr uint32_t PO_LEAST = 33, PO_MOST = 1 << 17, PO_EACH = 1024;     // pairs from which on it is taken and up to which, and how many an expert
+constexpr int PO_THREADS = 1024, PO_WAVES = PO_THREADS / 64, PO_EXPERTS = 4, PO_LIST = 2048;
+template <bool BASE>
+__global__ __launch_bounds__(PO_THREADS) void k_pairs_by_expert(const int32_t* ids, uint32_t T, int32_t base, int32_t n_expert, uint32_t per, uint32_t seg,
+                                                                int32_t* sorted, int32_t* off, int32_t* count, int32_t* row_of) {
+    __shared__ int tot[PO_WAVES][PO_EXPERTS + 1];                 // a wave's pairs of each own expert, and of lower ones
+    __shared__ uint16_t list[PO_WAVES][PO_LIST];                  // its own pairs in order, from its part's first on: 4 pair + expert
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t first = blockIdx.x * per, n = min(per, (uint32_t)n_expert - first);
+    // the pairs that no expert has, in the workgroup's segment
+    if (row_of) {
+        const uint32_t lo = blockIdx.x * seg, hi = lo >= T ? lo : T - lo < seg ? T : lo + seg;
+        for (uint32_t i = lo + tid; i < hi; i += PO_THREADS)
+            if ((uint32_t)ids[i] - (uint32_t)base >= (uint32_t)n_expert) row_of[i] = -1;
+    }
+    const uint32_t part = ((T + PO_WAVES - 1) / PO_WAVES + 255) / 256 * 256, from = min(T, wv * part), to = min(T, from + part);
+    struct __attribute__((packed, aligned(4))) Four { uint32_t v[4]; };
+    constexpr uint32_t NONE = 0x80000000u;                        // (no id less the base: both are far from 2^31)
+    auto load = [&](uint32_t i) {
+        Four q = { { NONE, NONE, NONE, NONE } };
+        if (i + 4 <= to) {
+            q = *(const Four*)(ids + i);
+            if (BASE)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q.v[j] -= (uint32_t)base;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (i + j < to) q.v[j] = (uint32_t)ids[i + j] - (uint32_t)base;
+        }
+        return q;
+    };
+    int below = 0;
+    uint32_t listed = 0;
+    auto look = [&](const Four& q, uint32_t i) {
+        uint64_t hit[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t lower = __ballot(q.v[j] < first);
+            hit[j] = __ballot(q.v[j] < first + n) & ~lower;
+            below += q.v[j] < first ? 1 : 0;
+        }
+        if ((hit[0] | hit[1] | hit[2] | hit[3]) == 0) return;
+        uint32_t at = listed;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) at = __builtin_amdgcn_mbcnt_hi((uint32_t)(hit[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[j], at));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (hit[j] == 0) continue;                            // (uniform)
+            if (q.v[j] - first < n) {
+                if (at < PO_LIST) list[wv][at] = (uint16_t)(4 * (i - from + j) + q.v[j] - first);
+                ++at;
+            }
+            listed += (uint32_t)__popcll(hit[j]);
+        }
+    };
+    uint32_t i0 = from;
+    for (; i0 + 1024 <= to; i0 += 1024) {                         // four rounds' loads out together
+        Four q[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q[r] = load(i0 + 256 * r + 4 * lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) look(q[r], i0 + 256 * r + 4 * lane);
+    }
+    for (; i0 < to; i0 += 256) look(load(i0 + 4 * lane), i0 + 4 * lane);
+    below = wave_scan_incl(below);
+    // f(x, pair) for 64 of the own pairs in order, one a lane (x: its expert of these, or PO_EXPERTS for none)
+    auto each = [&](auto f) {
+        if (listed <= PO_LIST) {
+            for (uint32_t k = 0; k < listed; k += 64) {
+                const uint32_t v = k + lane < listed ? list[wv][k + lane] : 0u;
+                f(k + lane < listed ? v & 3 : PO_EXPERTS, from + (v >> 2));
+            }
+        } else {                                                  // too many: the ids again
+            for (uint32_t i = from; i < to; i += 512) {
+                uint32_t x[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) x[r] = i + 64 * r + lane < to ? (uint32_t)ids[i + 64 * r + lane] - (uint32_t)base - first : NONE;
+#pragma unroll 1
+                for (int r = 0; r < 8; ++r) {
+                    f(x[0] < n ? x[0] : PO_EXPERTS, i + 64 * r + lane);
+#pragma unroll
+                    for (int u = 0; u < 7; ++u) x[u] = x[u + 1];
+                }
+            }
+        }
+    };
+    int own[PO_EXPERTS] = {};
+    each([&](uint32_t x, uint32_t) {
+#pragma unroll
+        for (int e = 0; e < PO_EXPERTS; ++e)
+            if (e < (int)n) own[e] += __popcll(__ballot(x == (uint32_t)e));
+    });
+    if (lane == 63) {
+#pragma unroll
+        for (int e = 0; e < PO_EXPERTS; ++e) tot[wv][e] = own[e];
+        tot[wv][PO_EXPERTS] = below;
+    }
+    __syncthreads();
+    // each expert's first row, and the wave's in it (lane w: wave w's counts)
+    const int w16 = lane & (PO_WAVES - 1);
+    int row = __builtin_amdgcn_readlane(wave_scan_incl(tot[w16][PO_EXPERTS]), PO_WAVES - 1), next[PO_EXPERTS];
+#pragma unroll
+    for (int e = 0; e < PO_EXPERTS; ++e) {
+        const int c = tot[w16][e], incl = wave_scan_incl(c), all = __builtin_amdgcn_readlane(incl, PO_WAVES - 1);
+        next[e] = row + __builtin_amdgcn_readlane(incl - c, wv);
+        if (e < (int)n && tid == 0) {
+            off[first + e] = row;
+            if (count) count[first + e] = all;
+        }
+        row += all;
+    }
+    each([&](uint32_t x, uint32_t pair) {
+        int pos = -1;
+#pragma unroll
+        for (int e = 0; e < PO_EXPERTS; ++e) {
+            if (e >= (int)n) break;
+            const uint64_t m = __ballot(x == (uint32_t)e);
+            if (x == (uint32_t)e) pos = next[e] + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+            next[e] += __popcll(m);
+        }
+        if (pos >= 0) {
+            sorted[pos] = (int32_t)pair;
+            if (row_of) row_of[pair] = pos;
+        }
+    });
+    if (first + n == (uint32_t)n_expert) {                        // the last workgroup: behind the last row
+        if (tid == 0) off[n_expert] = row;
+        for (uint32_t i = row + tid; i < T; i += PO_THREADS) sorted[i] = -1;
+    }
+}
+
 // moe_scatter of the router's pairs (token t's top_k ids at t * top_k .., distinct experts, at most 32 tokens and
 // blockDim.x pairs) for at most blockDim.x experts: each expert's set of tokens as a bit mask (LDS atomics), its count
 // the mask's population; expert_offset the counts' exclusive scan (a DPP scan in each wave, then the waves' totals
@@ -860,6 +1000,13 @@ extern "C" int exl3c4_dev_scatter(const int32_t* ids, int64_t T, int64_t base, i
     const int64_t segs = T > 0 ? (T + SC_SEG - 1) / SC_SEG : 1;
     const int64_t per = row_of == ids ? segs : (segs + SC_MAX_WG - 1) / SC_MAX_WG;
     const unsigned wgs = (unsigned)((segs + per - 1) / per);
+    if (row_of != ids && T >= PO_LEAST && T <= PO_MOST && T <= (int64_t)PO_EACH * n_expert && base >= -(1 << 30) && base <= 1 << 30) {
+        // (ids written over by row_of while other workgroups read them, and bases that 32 bits do not take from every id, are k_scatter's)
+        const uint32_t by = ((uint32_t)n_expert + SC_MAX_WG - 1) / SC_MAX_WG, n = ((uint32_t)n_expert + by - 1) / by;
+        hipLaunchKernelGGL(base == 0 ? k_pairs_by_expert<false> : k_pairs_by_expert<true>, dim3(n), dim3(PO_THREADS), 0, (hipStream_t)stream, ids, (uint32_t)T, (int32_t)base, n_expert, by,
+                           ((uint32_t)T + n - 1) / n, sorted, off, count, row_of);
+        return launched();
+    }
     const bool far = base < INT32_MIN || base > INT32_MAX;
     const auto f = T <= SC_THREADS       ? (far ? k_scatter<1, true> : k_scatter<1, false>)
                    : T <= 4 * SC_THREADS ? (far ? k_scatter<4, true> : k_scatter<4, false>)

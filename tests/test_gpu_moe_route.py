@@ -243,3 +243,57 @@ def test_rows_past_32_bits(ex, t, n_tok):
     check(ex, l, 6, "sigmoid", (torch.arange(96) % 7).float().cuda() * 0.01, 8, 3, "top2")
     del l
     torch.cuda.empty_cache()
+
+
+def scatter_check(ex, ids, E, base=0, count=True, rows=True):
+    """moe_scatter of ids i32 [n_tok, top_k] on the device (of any 4-byte alignment) against the stable sort."""
+    n_tok, top_k = ids.shape
+    _, _, st, off, cnt, row = outputs(n_tok, E, top_k)
+    assert ex.moe_scatter(ids, E, st[:-3], off[:-3], cnt[:-3] if count else None, row[:-3] if rows else None, base) == 0
+    torch.cuda.synchronize()
+    e = ids.cpu().numpy().astype(np.int64).reshape(-1) - base
+    e = np.where((e >= 0) & (e < E), e, E)
+    order = np.argsort(e, kind="stable")
+    counts = np.bincount(e, minlength=E + 1)[:E]
+    live = int(counts.sum())
+    want = np.full(e.size, -1), np.concatenate(([0], np.cumsum(counts))), counts, np.full(e.size, -1)
+    want[0][:live] = order[:live]
+    want[3][order[:live]] = np.arange(live)
+    for got, w, there in zip((st, off, cnt, row), want, (True, True, count, rows)):
+        got = got.cpu().numpy()
+        assert (got[len(w):] == -77).all()
+        assert np.array_equal(got[:len(w)], w) if there else (got == -77).all()
+
+
+@pytest.mark.parametrize("E", [1, 3, 8, 64, 255, 256, 257, 512, 513, 768, 769, 1000, 1024])
+@pytest.mark.parametrize("n_tok,top_k", [(32, 1), (33, 1), (51, 5), (1024, 4), (4097, 1), (409, 10), (410, 10), (1640, 10), (8192, 9)])
+def test_the_scatter_by_experts(ex, E, n_tok, top_k):
+    """Numbers of experts around those that one, two, three and four a workgroup take, pairs around those of a wave's load and of its four loads together;
+    ids at an odd word, some of them no expert's."""
+    rng = np.random.default_rng(E * 7 + n_tok)
+    store = torch.zeros(n_tok * top_k + 1, dtype=torch.int32, device="cuda")
+    ids = store[1:].view(n_tok, top_k)
+    ids.copy_(torch.from_numpy(rng.integers(-2, E + 3, (n_tok, top_k)).astype(np.int32)))
+    scatter_check(ex, ids, E)
+    scatter_check(ex, ids, E, count=False, rows=False)
+    scatter_check(ex, ids, max(E // 4, 1), base=E // 3)
+    ids += 1 << 29
+    scatter_check(ex, ids, E, base=1 << 29)
+
+
+@pytest.mark.parametrize("n_tok,top_k,E", [(4096, 2, 8), (20000, 4, 20), (20000, 4, 100), (13107, 10, 512), (65536, 8, 512), (65536, 2, 8)])
+def test_scatters_of_one_expert_and_of_none(ex, n_tok, top_k, E):
+    """More pairs of an expert than a wave's list holds (2,048 of the 16th of the pairs): all of them, three quarters, nearly all; and no expert's at all."""
+    ids = torch.full((n_tok, top_k), E - 1, dtype=torch.int32, device="cuda")
+    scatter_check(ex, ids, E)
+    ids[:, 0] = torch.arange(n_tok, device="cuda") % E
+    scatter_check(ex, ids, E)
+    ids.fill_(0)
+    ids[n_tok // 2:, 1] = E // 2
+    scatter_check(ex, ids, E)
+    ids.fill_(-1)
+    scatter_check(ex, ids, E)
+    ids.fill_(-2 ** 31)
+    ids[5] = 2 ** 31 - 1
+    scatter_check(ex, ids, E, base=1 << 30)
+    scatter_check(ex, ids, E, base=-(1 << 30))
