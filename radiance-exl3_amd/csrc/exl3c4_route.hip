@@ -544,7 +544,10 @@ __global__ __launch_bounds__(1024) void k_route_scatter(const void* logits, int3
 // The order of experts and of groups is that of their values in 64 bits, for among thousands of tokens there are always experts whose values f32 would
 // not tell apart. f32 finds who can be among the first (all within its error of them), f64 ranks those: one evaluation a lane. Groups whose place f32 leaves
 // open, and more than 64 such experts, are evaluated in f64 as a whole. Weights come out of the f64 scores, rounded once.
-// 8192 tokens, 8 groups of 64 experts, top-10 with a bias: f64 for every expert took 22 us.
+// What bounds it: the VALU, some 800 instructions a token of 512 experts (of them the scores 110, the order of the lanes' largest 110, the candidates'
+// scores and ranks in f64 200); 16 MiB of logits are 3.4 us. 8192 tokens, 8 groups of 64 experts of which 4 stay, top-10 with a bias 13.5 us, 22 with f64 for
+// every expert; without groups 13.8 (softmax); 256 experts 10.5; one token 4.9 with its scatter, the whole of it latency. A group's place that stays open
+// is two groups' values in f64, in one token of some thousands: 613 tokens 5.2 us without one, 7.4 with (13.3 when every group was evaluated again).
 
 // e^x for x <= 0 (below -800: 0): x = n ln 2 + r with ln 2 in two parts (its first 37 bits, so that n times them is exact, and the rest), |r| <= ln 2 / 2,
 // and the exponential series up to r^13, whose rest is below 2^-52 of e^r.
@@ -570,7 +573,7 @@ __device__ __forceinline__ double exp64(double x) {
     p = fma(p, r, 1.0);
     return ldexp(p, (int)n);
 }
-// 1 / d for d in [1, 2^11]: the hardware's estimate (some 26 bits) and two steps of Newton's.
+// 1 / d for d in [2^-1000, 2^11]: the hardware's estimate (some 26 bits) and two steps of Newton's.
 __device__ __forceinline__ double inverse64(double d) {
     double q = __builtin_amdgcn_rcp(d);
     q = fma(fma(-d, q, 1.0), q, q);
@@ -583,13 +586,16 @@ __device__ __forceinline__ double sigmoid64(double l) {
 template <int J> __device__ __forceinline__ double xor_laned(double v, int lane) {
     return __builtin_bit_cast(double, xor_lane64<J>(__builtin_bit_cast(uint64_t, v), lane));
 }
-__device__ __forceinline__ double wave_sum(double v, int lane) {
-    v += xor_laned<32>(v, lane);
-    v += xor_laned<16>(v, lane);
+// The sum over a row of 16 lanes, and over all.
+__device__ __forceinline__ double row_sum(double v, int lane) {
     v += xor_laned<8>(v, lane);
     v += xor_laned<4>(v, lane);
     v += xor_laned<2>(v, lane);
     return v + xor_laned<1>(v, lane);
+}
+__device__ __forceinline__ double wave_sum(double v, int lane) {
+    v += xor_laned<32>(v, lane);
+    return row_sum(v + xor_laned<16>(v, lane), lane);
 }
 // An order of doubles as unsigned numbers (-0 as +0); 0 stands for none.
 __device__ __forceinline__ uint64_t order64(double v) {
@@ -628,11 +634,12 @@ __device__ __forceinline__ double choice64(const Exl3c4DevRoute& a, const Soft& 
     const float l = logit(a, row + e);
     return by_logit ? (double)l : score64(a, sm, l) + (a.bias ? (double)a.bias[e] : 0.0);
 }
-// The groups that stay, by f64: bit g for group g.
-__device__ __forceinline__ uint64_t groups64(const Exl3c4DevRoute& a, const Soft& sm, int64_t row, int lane) {
+// Which `places` of the groups `of` stay, by f64 (bit g for group g).
+__device__ __forceinline__ uint64_t groups64(const Exl3c4DevRoute& a, const Soft& sm, int64_t row, int lane, uint64_t of, int places) {
     uint64_t mine = 0;                                           // lane g: group g's value
 #pragma unroll 1
-    for (int g = 0; g < a.n_group; ++g) {
+    for (uint64_t left = of; left != 0; left &= left - 1) {
+        const int g = __builtin_ctzll(left);
         double v1 = -INFINITY, v2 = -INFINITY;
 #pragma unroll 1
         for (int i = lane; i < a.group; i += 64) {
@@ -653,11 +660,12 @@ __device__ __forceinline__ uint64_t groups64(const Exl3c4DevRoute& a, const Soft
     }
     int ahead = 0;
 #pragma unroll 1
-    for (int q = 0; q < a.n_group; ++q) {
+    for (uint64_t left = of; left != 0; left &= left - 1) {
+        const int q = __builtin_ctzll(left);
         const uint64_t o = readlane64(mine, q);
         ahead += o > mine || (o == mine && q < lane) ? 1 : 0;
     }
-    return __ballot(lane < a.n_group && ahead < a.top_group);
+    return __ballot((of >> lane & 1) != 0 && ahead < places);
 }
 
 // A candidate's key, id, logit and bias; behind the ranking its id and score.
@@ -757,8 +765,14 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
         if (a.groups_log2 < 3) meet(xor_lanef<4>(v1, lane), xor_lanef<4>(v2, lane));
         if (a.groups_log2 < 2) meet(xor_lanef<2>(v1, lane), xor_lanef<2>(v2, lane));
         const float gv = top2 && v2 > -INFINITY ? v1 + v2 : v1;
-        // Twice the error of its value, from two choices': of two groups that f32 may have in the wrong order the one that is less certain sees it.
-        const float near = exact || gv == INFINITY || gv == -INFINITY ? 0.f : 0x1p-19f + 0x1p-21f * (fabsf(v1) + (top2 && v2 > -INFINITY ? fabsf(v2) : 0.f));
+        // Twice the error of a value, from two choices': the largest of the groups', so that two that f32 may have in the wrong order see each other.
+        float near = exact || gv == INFINITY || gv == -INFINITY ? 0.f : 0x1p-19f + 0x1p-21f * fabsf(v1) + (top2 && v2 > -INFINITY ? 0x1p-21f * fabsf(v2) : 0.f);
+        near = fmaxf(near, xor_lanef<32>(near, lane));
+        near = fmaxf(near, xor_lanef<16>(near, lane));
+        near = fmaxf(near, xor_lanef<8>(near, lane));
+        near = fmaxf(near, xor_lanef<4>(near, lane));
+        near = fmaxf(near, xor_lanef<2>(near, lane));
+        near = fmaxf(near, xor_lanef<1>(near, lane));
         const float above = gv + near, below = gv - near;
         int ahead = 0, beside = 0;                               // groups ahead for sure; ahead or too close to tell (its own among them)
         if (exact) {
@@ -778,8 +792,12 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
                 beside = ahead + 1;
             }
         }
-        uint64_t stay = __ballot(g < a.n_group && ahead < a.top_group);      // bit g: group g (and again for each part)
-        if (!exact && __any(g < a.n_group && ahead < a.top_group && beside > a.top_group)) stay = groups64(a, sm, row, lane);
+        uint64_t stay = __ballot(lane < a.n_group && ahead < a.top_group);   // bit g: group g
+        if (!exact) {                                            // (two groups or so, of one token in some thousands)
+            const uint64_t open = __ballot(lane < a.n_group && ahead < a.top_group && beside > a.top_group);
+            stay &= ~open;
+            if (open != 0) stay |= groups64(a, sm, row, lane, open, a.top_group - __popcll(stay));
+        }
 #pragma unroll
         for (int j = 0; j < RPL; ++j) {
             const uint32_t of = (uint32_t)(lane + 64 * j) * a.group_inv >> 20;     // the expert's group (past the last expert: c is NaN)
@@ -816,17 +834,16 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
             ck = order64(biased ? own.s + (double)own.b : (double)own.l);
         }
         int rank = 0;
-        for (int q = 0; q < n; ++q) {                            // (ids ascend neither in the candidates nor in the lanes: ties are rare, and looked at apart)
-            const uint64_t o = readlane64(ck, q);
-            rank += o > ck ? 1 : 0;
-            if (__any(lane < n && o == ck && lane != q)) {
-                const int oe = __builtin_amdgcn_readlane(own.id, q);
-                rank += o == ck && oe < own.id ? 1 : 0;
-            }
-        }
+        for (int q = 0; q < n; ++q) rank += readlane64(ck, q) > ck ? 1 : 0;
         wave_sync();
         if (lane < n) cand[rank].s = own.s, cand[rank].id = own.id;
         wave_sync();
+        if (__any(lane < n && cand[rank].id != own.id)) {        // equal keys wrote one place: in the candidates' order, which is the ids'
+            for (int q = 0; q < n; ++q) rank += readlane64(ck, q) == ck && q < lane ? 1 : 0;
+            wave_sync();
+            if (lane < n) cand[rank].s = own.s, cand[rank].id = own.id;
+            wave_sync();
+        }
         if (lane < n && lane < a.top_k) mine = cand[lane].id, w = cand[lane].s;
     } else {
         uint32_t in = 0;                                         // which of the lane's experts can be chosen
@@ -858,8 +875,10 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
     }
     wave_sync();                                                 // read before the next token's
     if (a.renorm) {
-        const double sum = wave_sum(w, lane);
-        w = sum > 0.0 ? w / sum : 0.0;
+        const double sum = a.top_k > 16 ? wave_sum(w, lane) : row_sum(w, lane);
+        // (an f64 division is some 30 instructions; the reciprocal of a number below 2^-1000 may not be one)
+        if (__any(lane < a.top_k && !(sum > 0x1p-1000))) w = sum > 0.0 ? w / sum : 0.0;
+        else w *= inverse64(sum);
     }
     return Pick{ mine, (float)(w * (double)a.scale) };
 }

@@ -203,6 +203,19 @@ def test_groups_whose_sums_32_bits_do_not_tell_apart(ex, score):
     check(ex, same.cuda(), 9, score, torch.randn(4, generator=g).repeat(16).cuda(), 16, 3, "top2")
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("n_tok", [16, 4000])
+def test_groups_of_which_one_is_less_certain_in_32_bits(ex, score, n_tok):
+    """The sums of two groups differ by less than 2^-14, where the second's is one of 1000 and -1000: far less certain than the first's."""
+    g = torch.Generator().manual_seed(n_tok)
+    l = torch.randn((n_tok, 12), generator=g)
+    l[:, 4:6] = l[:, 0:2] + (torch.rand((n_tok, 2), generator=g) - 0.5) * 2.0 ** -12
+    out = -float("inf")
+    bias = torch.tensor([0.0, 0.0, out, out, 1000.0, -1000.0, out, out, -3.0, -3.0, out, out]).cuda()
+    check(ex, l.cuda(), 2, score, bias, 3, 1, "top2", scatter=n_tok == 16)
+    check(ex, l.cuda(), 3, score, bias, 3, 2, "top2", scatter=False)
+
+
 @pytest.mark.parametrize("n_tok", [3, 40])
 @pytest.mark.parametrize("E", [65, 100, 129, 192, 193, 257, 320, 511, 513, 700, 961])
 def test_experts_that_do_not_fill_the_registers(ex, n_tok, E):
