@@ -212,3 +212,15 @@ def test_replayed_graphs_beside_each_other(ex, block):
             assert ex.f8_quant(x, own) == 0 and ex.f8_dequant(own, values) == 0
             torch.cuda.synchronize()
             assert torch.equal(q.codes, own.codes) and torch.equal(q.scales, own.scales) and torch.equal(out, values)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_zeros_keep_their_sign(ex, t):
+    x = torch.zeros((2, 256), dtype=TYPES[t], device="cuda")
+    x[0, 1::2] = -0.0
+    x[1, ::3] = -0.0
+    x[1, 5] = -2.0
+    q = ex.f8_empty(x.shape, 1)
+    assert ex.f8_quant(x, q) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q.codes.cpu() >> 7, torch.signbit(x.cpu()).byte())
