@@ -69,6 +69,8 @@ __device__ __forceinline__ int64_t scale_row(int n, int half, int n_out) { retur
 // A workgroup: a chunk of up to 16 rows against NS strips of 16 weight rows (with SwiGLU half of them gate rows and half their up rows), each wave
 // a part of k; the weights go from memory straight to the matrix units' operands, each byte read once, and the parts' sums meet in LDS in a
 // fixed order. x is the A operand (rows of D), W the B operand: lane l ends with D[m = 4 g + r][n = l % 16].
+// What bounds it: for one token the start (offsets, rows, the first loads) and the last round trip, 8.6 us and 2.4 TB/s of 10 experts' 1024 x 2048; then memory, one
+// row against 8192 x 8192 16.4 us, 4.1 TB/s. Four steps ahead or loads past the caches: within 1%.
 constexpr int ROWS_LOG2 = 4;
 constexpr int WAVES = 4;
 
@@ -216,8 +218,9 @@ template <int T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // small and a CU holds several, one at its start or end under another's products.
 //
 // LDS. A row of a stage is 128 bytes (16-bit x: two such halves). The loads write lane after lane, 16 bytes each, so the order within a row is chosen
-// at the source: place p of row r holds the chunk p ^ (r & 7), and the 16 rows and four lane groups that read a matrix operand fall on all the
-// banks evenly. Behind x's rows a scale for each; behind the weights' those of the tile's blocks of weight rows.
+// at the source: place p of row r holds the chunk q = p ^ (r & 7), in a half of a 16-bit row the chunk whose number is q's with its highest bit moved to the end,
+// so that lane groups g and g + 1 read places that differ in their lowest bit: the 16 rows and four lane groups that read a matrix operand then fall on all the
+// banks evenly (16-bit rows by q itself: 39% of the LDS cycles were conflicts, 1% so; 4096 tokens over 8 experts 56.0 -> 54.4 us). Behind x's rows a scale for each; behind the weights' those of the tile's blocks of weight rows.
 //
 // Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, so that a sum's scale is one number of the
 // lane's row of x times one that the wave shares.
@@ -260,8 +263,11 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
         const gaddr we = entry(a.w, a.w_stride, ch.expert), wse = entry(a.ws, a.ws_stride, ch.expert);
         // Each of the wave's loads of a stage: where it reads next, for this lane (lane l takes place l % 8 of row l / 8). A stage is 128 columns on.
         gaddr xp[G::NX], wp[G::NW];
-        auto x_chunk = [&](int i) { return (lane & 7) ^ ((8 * (XT == F8 ? wave + i * WV : (wave + i * WV) >> 1) + (lane >> 3)) & 7); };
-        auto w_chunk = [&](int i) { return (lane & 7) ^ ((8 * (wave + i * WV) + (lane >> 3)) & 7); };
+        auto x_chunk = [&](int) {
+            const int q = (lane & 7) ^ (lane >> 3);
+            return XT == F8 ? q : ((q & 3) << 1) | (q >> 2);
+        };
+        auto w_chunk = [&](int) { return (lane & 7) ^ (lane >> 3); };
 #pragma unroll
         for (int i = 0; i < G::XL; ++i) {
             const int q = wave + i * WV, r = 8 * (XT == F8 ? q : q >> 1) + (lane >> 3);
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            xv[m][j] = *(const uint4*)(X + ((xr >> 3) + 2 * m) * 2048 + (j >> 1) * 1024 + (l16 & 7) * 128 + 16 * ((2 * g + (j & 1)) ^ (l16 & 7)));
+                            xv[m][j] = *(const uint4*)(X + ((xr >> 3) + 2 * m) * 2048 + (j >> 1) * 1024 + (l16 & 7) * 128 + 16 * ((g + 4 * (j & 1)) ^ (l16 & 7)));
                     }
                 }
 #pragma unroll
@@ -497,14 +503,15 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
 // the routing, which is on the device. Larger tiles read weights and rows less often; smaller ones waste less of a chunk, make more workgroups and
 // start sooner; the rows kernel splits k over its waves, so that few workgroups are enough. `units`: workgroups of a tile, each expert half a chunk
 // short of whole ones. Measured on one card, us, the product alone (E / top-k, N x K, tokens; 512/10, 1024 x 2048 with SwiGLU where nothing else is said):
-//   rows against 32        bf16 x: 1 token 8.6 / 13.3, 4 19.3 / 20.3, 8 30 / 27, 32 97 / 95; F8 x: 8 30 / 27, 16 55 / 50, 32 95 / 91.
-//                          64/6, 32 tokens 29 / 23; 8/2, 200 16.3 / 13.8. One expert, bf16 x: 2048 x 2048, 77 rows 10.1 / 13.7, 300 22 / 18;
-//                          8192 x 8192, 64 rows 48 / 58; 4096 x 4096, 16 rows 11.5 / 23, 300 59 / 36.
-//   2 strips against 4     one row, 8192 x 8192 16.5 / 23.5; 4096 x 4096, 16 rows 11.5 / 15.2; 8192 x 8192, 64 rows 61 / 48, which read the weights
+//   rows against 32        bf16 x: 1 token 8.6 / 13.3, 4 19.5 / 20.0, 8 30 / 27, 32 102 / 95; F8 x: 8 30 / 26, 16 55 / 49, 32 98 / 91.
+//                          64/6, 32 tokens 30 / 23; 8/2, 200 20 / 13. One expert, bf16 x: 2048 x 2048, 77 rows 10.7 / 13.2, 300 22 / 18;
+//                          8192 x 8192, 64 rows 48 / 57; 4096 x 4096, 16 rows 11.6 / 22, 300 74 / 35.
+//   2 strips against 4     one row, 8192 x 8192 16.4 / 23.6; 4096 x 4096, 16 rows 11.6 / 15.4; 8192 x 8192, 64 rows 61 / 48, which read the weights
 //                          once for each 16 rows, mostly from L2.
-//   32 rows against 64     as codes: 400 tokens 184 / 189, 613 Zipf 2560 x 640 160 / 158, 1500 221 / 193, 8/2 800 15.9 / 21. bf16 x: 400 184 / 197,
-//                          613 Zipf 2560 x 640 166 / 185, 1500 220 / 203, 8/2 800 19 / 28. F8 x, f32 y: 200 183 / 203, 1500 233 / 222.
-//   64 against 128         as codes: 1500 193 / 204, 2048 Zipf 226 / 229, 4096 275 / 218, 64/6 2000 53 / 45, 8/2 8192 2816 x 2048 148 / 113.
+//   32 rows against 64     as codes: 400 tokens 183 / 184, 613 Zipf 2560 x 640 160 / 168, 1500 218 / 192, 8/2 800 15.3 / 19.8. bf16 x: 400 184 / 200,
+//                          613 Zipf 2560 x 640 167 / 184, 1500 218 / 203, 8/2 800 19 / 27. F8 x, f32 y: 200 183 / 209, 1500 232 / 228.
+//   64 against 128         as codes: 1500 192 / 204, 2048 Zipf 224 / 230, 4096 274 / 218, 64/6 2000 52 / 42, 8/2 8192 2816 x 2048 144 / 111,
+//                          2048 x 1408, sorted rows in, 80 / 68.
 // As codes a tile of 256 x 256 with a CU to itself took 131 there before the loads went among the products and 114 to 118 since, and was slower
 // everywhere else; 128 x 128 130 (73 for 77 at 2048 x 1408, sorted rows in); weights in two places 232 at 64 rows, and 2% less at 32 rows and 100 to 400
 // tokens. Widened: 128 x 128 in eight waves 344, 128 x 256 211 against 202 of 64 x 256.
