@@ -104,6 +104,9 @@ class F8Planes(C.Structure):
                 ("scales", _p), ("scales_pitch", _i64), ("scales_stride", _i64)]
 
 
+_F8_CODES = ("torch.uint8", "torch.float8_e4m3fn")
+
+
 class F8:
     """Matrices in 8-bit floats (include/exl3c4.h) of values [..., rows, cols]: codes uint8 or float8_e4m3fn [..., rows, >= cols rounded up to 16],
     scales f32 [..., ceil(rows / block), >= ceil(cols / 128)], the columns they stand for and a block's rows: 1 (activations) or 128 (weights). The
@@ -118,7 +121,7 @@ class F8:
             raise ValueError("a block has 1 or 128 rows")
         rows = codes.shape[-2] if codes.dim() > 1 else 1
         if codes.dim() < 2 or codes.dim() != scales.dim() or codes.shape[:-2] != scales.shape[:-2] or cols < 1 or codes.shape[-1] < (cols + 15) // 16 * 16 or \
-                scales.shape[-2] < (rows + block - 1) // block or scales.shape[-1] < (cols + 127) // 128 or codes.element_size() != 1 or \
+                scales.shape[-2] < (rows + block - 1) // block or scales.shape[-1] < (cols + 127) // 128 or str(codes.dtype) not in _F8_CODES or \
                 scales.element_size() != 4 or not scales.is_floating_point() or codes.device != scales.device:
             raise ValueError("the F8 planes do not fit each other or their columns")
         put = super().__setattr__

@@ -180,6 +180,13 @@ def test_the_binding_refuses_what_does_not_fit():
             bad()
 
 
+@pytest.mark.parametrize("t", [torch.int8, torch.float8_e5m2, torch.float8_e4m3fnuz, torch.bool])
+def test_codes_of_another_type_are_refused(t):
+    with pytest.raises(ValueError):
+        exl3c4.F8(torch.zeros(4, 304, dtype=torch.uint8).view(t), torch.zeros(4, 3), 300, 1)
+    exl3c4.F8(torch.zeros(4, 304, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(4, 3), 300, 1)
+
+
 # ------------------------------------------------------------------------------------------ the reference
 def test_the_reference_rounds_to_the_nearest_code():
     """Every code's value comes back as itself, and every tie between neighbours goes to the even code; torch's own e4m3 agrees."""

@@ -113,3 +113,27 @@ def test_a_layer(ex, n_tok, f8_x):
         graph.replay()
         torch.cuda.synchronize()
         layer.check()
+
+
+@pytest.mark.parametrize("n_tok", [9, 37, 400])
+@pytest.mark.parametrize("f8_x", [False, True])
+def test_a_padded_batch(ex, n_tok, f8_x):
+    """Tokens of NaN (the first, some in between, the last) have no expert and come out as zeros; the others' bits are those of a batch without such tokens."""
+    layer = Layer(ex, n_tok, f8_x)
+    x = torch.randn(n_tok, H, generator=torch.Generator().manual_seed(n_tok))
+    layer.x.copy_(x)
+    layer.run()
+    torch.cuda.synchronize()
+    whole = layer.out.clone()
+    bad = torch.zeros(n_tok, dtype=torch.bool)
+    bad[0] = bad[n_tok // 2] = bad[-3:] = True
+    x[bad] = float("nan")
+    layer.x.copy_(x)
+    for t in (layer.h, layer.y, layer.out):
+        t.fill_(float("nan"))
+    layer.run()
+    torch.cuda.synchronize()
+    live = TOP_K * int((~bad).sum())
+    assert (layer.ids.cpu()[bad] == -1).all() and (layer.w.cpu()[bad] == 0).all() and int(layer.off[-1]) == live
+    assert (layer.st[live:] == -1).all() and not layer.h[live:].any() and not layer.y[live:].any()
+    assert not layer.out[bad.cuda()].any() and torch.equal(layer.out[~bad.cuda()], whole[~bad.cuda()])
