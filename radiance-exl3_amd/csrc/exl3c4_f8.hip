@@ -6,11 +6,13 @@
 // infinities and NaNs are the largest. v_cvt_pk_fp8_f32 rounds to nearest even (checked for every tie against that rule).
 //
 // Blocks of one row: a lane takes 16 bytes of values, 8 columns of 16 bits or 4 of 32, so that a wave's loads and stores are whole lines; the 16 or 32
-// lanes of a block find the largest by DPP. Blocks of 128 rows: a workgroup each, 8 columns a lane and every value of the block in its registers, so
-// that memory is read once. The same columns a lane on the way back.
+// lanes of a block find the largest by DPP. Blocks of 128 rows: a workgroup each, 16 lanes for the 256 bytes or twice 256 bytes of a row and every value of the block in its
+// registers, so that memory is read once. The same columns a lane on the way back.
 //
-// What bounds it: memory, with the VALU next to it (85% busy in rows). Quantising and back, us (TB/s of both sides' bytes): rows, 20480 x 650 f16 10.0 (4.0) and
-// 8.7, 8192 x 2048 f16 9.9 (5.1) and 8.9, f32 17.5 (4.8) and 14.2; blocks of 128 rows, 64000 x 2048 f32 145 (4.5) and 96; 64 x 2048 3.1 and 2.7, a launch.
+// What bounds it: memory, with the VALU next to it (85% busy in rows). What is read or written once goes past the caches (ONCE): values back 131072 x 1000 f32 94 us for
+// 114, f16 57 for 69; blocks of 128 rows, values in whole lines, 131072 x 1000 f32 135 for 157, f16 91 for 105 (their codes, a line a row, 105 -> 139: through the
+// caches). Quantising and back, us (TB/s of both sides' bytes): rows, 20480 x 650 f16 10.0 (4.0) and 8.7 (4.6), 8192 x 2048 f16 9.9 (5.1) and 8.9; blocks,
+// 131072 x 1000 f32 135 (4.9) and 94 (7.0, part of it into the cache behind L2); 64 x 2048 3.2 and 2.7, a launch.
 // Tried without a gain: a row's end shifted by selects of words in place of 64-bit shifts (20480 x 650 0.3 us less, 8192 x 2048 1 more: the loads' order).
 #include <hip/hip_runtime.h>
 
@@ -24,25 +26,32 @@ constexpr int F32 = EXL3C4_F32, F16 = EXL3C4_F16, BF16 = EXL3C4_BF16;
 constexpr int WG = 256;
 constexpr int PER = 4;                                          // slots (16 bytes of values) a lane, where rows are apart
 constexpr int64_t SLOTS = (int64_t)1 << 31;                     // slots a launch indexes in 32 bits
+// Codes up to which rows' are stored past the caches (below, ONCE). Quantising alone is faster so at any size (20480 x 650 f16 8.5 for 10.2 us, 8192 x 2048 7.8 for
+// 10.0); the products that read them then are not. A layer of route, quantising, products and gather, codes through the caches / past them: 512 experts, 2048 tokens (4
+// and 10 M codes) 354 / 341 us, 1500 334 / 326, 613 467 / 464; 8 experts, 4096 tokens (8 and 11 M) 149 / 151, 8192 (16 and 22 M) 241 / 247.
+constexpr uint64_t ONCE_MOST = 8 << 20;
 constexpr float TOP = 448.f;                                    // e4m3's largest
 constexpr uint32_t LEAST = 31u << 23;                           // 2^-96, the least magnitude that sets a scale: 448 / a stays finite
 
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 // 16 bytes at any address their type may have
-struct __attribute__((packed, aligned(2))) Words { uint32_t v[4]; };
 template <int DT> constexpr int COLS = DT == F32 ? 4 : 8;       // values in 16 bytes
 template <int DT> constexpr int SIZE = DT == F32 ? 4 : 2;
 
 // Columns c .. of a row at p (its column c) in 16 bytes, those from `cols` on as zeros: the row's last 16 bytes where they would pass its end, shifted
 // (2-byte loads of each took 20480 x 650 f16 from 9 to 14 us).
-template <int DT> __device__ __forceinline__ void load16b(uint32_t* v, const char* p, uint32_t c, uint32_t cols) {
+template <int DT, bool ONCE = false> __device__ __forceinline__ void load16b(uint32_t* v, const char* p, uint32_t c, uint32_t cols) {
     constexpr uint32_t C = COLS<DT>;
     if (cols >= C) {                                             // (uniform)
         const uint32_t past = c + C > cols ? c + C - cols : 0;
-        const Words q = *(const Words*)(p - (int64_t)past * SIZE<DT>);
+        u32x4 q;
+        if constexpr (ONCE) q = __builtin_nontemporal_load((const u32x4_at2*)(p - (int64_t)past * SIZE<DT>));
+        else q = *(const u32x4_at2*)(p - (int64_t)past * SIZE<DT>);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = q.v[i];
+        for (int i = 0; i < 4; ++i) v[i] = q[i];
         if (past) {
             uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
             if (past >= C / 2) lo = hi, hi = 0;
@@ -131,9 +140,17 @@ template <int DT> __device__ __forceinline__ uint32_t four_codes(const uint32_t*
     q = __builtin_amdgcn_cvt_pk_fp8_f32(scaled<DT>(v, i + 2, k.inv), scaled<DT>(v, i + 3, k.inv), q, true);
     return k.inv == 0.f ? 0u : (uint32_t)q;
 }
-template <int DT> __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t* v, const Scale& k) {
-    if constexpr (DT == F32) *(uint32_t*)p = four_codes<DT>(v, 0, k);
-    else *(uint2*)p = { four_codes<DT>(v, 0, k), four_codes<DT>(v, 4, k) };
+// (ONCE: past the caches)
+template <int DT, bool ONCE> __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t* v, const Scale& k) {
+    if constexpr (DT == F32) {
+        const uint32_t q = four_codes<DT>(v, 0, k);
+        if (ONCE) __builtin_nontemporal_store(q, (uint32_t*)p);
+        else *(uint32_t*)p = q;
+    } else {
+        const uint64_t q = four_codes<DT>(v, 0, k) | (uint64_t)four_codes<DT>(v, 4, k) << 32;
+        if (ONCE) __builtin_nontemporal_store(q, (uint64_t*)p);
+        else *(uint64_t*)p = q;
+    }
 }
 
 // Slots of a launch: lanes_row of them a row. s / lanes_row by a multiplication (s < 2^31, lanes_row at least 2; exact).
@@ -150,7 +167,7 @@ __device__ __forceinline__ Where where(const Exl3c4DevF8& a, uint32_t r) {
 }
 
 // Blocks of one row: whole blocks of lanes a row.
-template <int DT>
+template <int DT, bool ONCE>
 __global__ __launch_bounds__(WG) void k_f8_quant_rows(Exl3c4DevF8 a, Slots sl) {
     constexpr uint32_t C = COLS<DT>, BLOCK_LOG2 = DT == F32 ? 5 : 4;
     uint32_t v[PER][4], at[PER];
@@ -169,7 +186,7 @@ __global__ __launch_bounds__(WG) void k_f8_quant_rows(Exl3c4DevF8 a, Slots sl) {
         const uint32_t m = magnitude<DT>(v[j]);
         const Scale k(DT == F32 ? max32(m) : max16(m));
         if (first + j * WG >= sl.count) continue;
-        if (C * at[j] < a.code_cols) store_codes<DT>(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + C * at[j], v[j], k);
+        if (C * at[j] < a.code_cols) store_codes<DT, ONCE>(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + C * at[j], v[j], k);
         if ((at[j] & ((1u << BLOCK_LOG2) - 1)) == 0)
             *(float*)((char*)a.scales + w[j].mat * a.scales_stride + w[j].row * a.scales_pitch + (at[j] >> BLOCK_LOG2) * 4) = k.s;
     }
@@ -181,7 +198,7 @@ __global__ __launch_bounds__(WG) void k_f8_quant_blocks(Exl3c4DevF8 a, uint32_t 
     constexpr int H = 8 / COLS<DT>;                              // 16-byte parts of 8 columns
     __shared__ uint32_t top[WG / 64];
     const uint32_t per = across * down, m = blockIdx.x / per, in = blockIdx.x - m * per, rb = in / across, cb = in - rb * across;
-    const uint32_t c = 128 * cb + 8 * (threadIdx.x & 15), r0 = 128 * rb + (threadIdx.x >> 4);
+    const uint32_t c = 128 * cb + COLS<DT> * (threadIdx.x & 15), r0 = 128 * rb + (threadIdx.x >> 4);
     const char* p = a.v + m * a.v_stride + (int64_t)c * SIZE<DT>;
     uint32_t v[8][H][4], t = 0;
 #pragma unroll
@@ -191,7 +208,7 @@ __global__ __launch_bounds__(WG) void k_f8_quant_blocks(Exl3c4DevF8 a, uint32_t 
         for (int h = 0; h < H; ++h) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[j][h][i] = 0;
-            if (r < a.rows) load16b<DT>(v[j][h], p + r * a.v_pitch + 16 * h, c + COLS<DT> * h, a.cols);
+            if (r < a.rows) load16b<DT, true>(v[j][h], p + r * a.v_pitch + 256 * h, c + 64 * h, a.cols);
         }
     }
 #pragma unroll
@@ -205,15 +222,15 @@ __global__ __launch_bounds__(WG) void k_f8_quant_blocks(Exl3c4DevF8 a, uint32_t 
     __syncthreads();
     const Scale k(max(max(top[0], top[1]), max(top[2], top[3])));
     uint8_t* q = a.codes + m * a.codes_stride + c;
-    if (c < a.code_cols)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (r0 + 16 * j < a.rows)
-                *(uint2*)(q + (r0 + 16 * j) * a.codes_pitch) = { four_codes<DT>(v[j][0], 0, k), four_codes<DT>(v[j][H - 1], 4 % COLS<DT>, k) };
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            if (r0 + 16 * j < a.rows && c + 64 * h < a.code_cols) store_codes<DT, false>(q + (r0 + 16 * j) * a.codes_pitch + 64 * h, v[j][h], k);
     if (threadIdx.x == 0) *(float*)((char*)a.scales + m * a.scales_stride + rb * a.scales_pitch + cb * 4) = k.s;
 }
 
-template <int DT>
+template <int DT, bool ONCE>
 __global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, Slots sl) {
     constexpr uint32_t C = COLS<DT>, BLOCK_LOG2 = DT == F32 ? 5 : 4;
     uint32_t q[PER][C / 4], at[PER];
@@ -244,23 +261,24 @@ __global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, Slots sl) {
         }
         const uint32_t c = C * at[j];
         char* p = a.v + w[j].mat * a.v_stride + w[j].row * a.v_pitch + (int64_t)at[j] * 16;
-        Words o;
+        u32x4 o;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (DT == F32) o.v[i] = __float_as_uint(f[i]);
+            if constexpr (DT == F32) o[i] = __float_as_uint(f[i]);
             else if constexpr (DT == F16)
-                o.v[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]) << 16;
+                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]) << 16;
             else
-                o.v[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) << 16;
+                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) << 16;
         }
         if (c + C <= a.cols) {
-            *(Words*)p = o;
+            if constexpr (ONCE) __builtin_nontemporal_store(o, (u32x4_at2*)p);
+            else *(u32x4_at2*)p = o;
         } else {
 #pragma unroll
             for (int i = 0; i < (int)C; ++i)
                 if (c + i < a.cols) {
-                    if constexpr (DT == F32) ((uint32_t*)p)[i] = o.v[i];
-                    else ((uint16_t*)p)[i] = (uint16_t)(o.v[i >> 1] >> (16 * (i & 1)));
+                    if constexpr (DT == F32) ((uint32_t*)p)[i] = o[i];
+                    else ((uint16_t*)p)[i] = (uint16_t)(o[i >> 1] >> (16 * (i & 1)));
                 }
         }
     }
@@ -290,8 +308,13 @@ int each_part(K kernel, const Exl3c4DevF8& a, uint32_t lanes, hipStream_t st) {
 extern "C" int exl3c4_dev_f8_quant(const Exl3c4DevF8* a, int32_t dtype, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
     const uint32_t across = (a->cols + 127) / 128;
-    if (a->block_log2 == 0)
-        return each_part(dtype == F32 ? k_f8_quant_rows<F32> : dtype == F16 ? k_f8_quant_rows<F16> : k_f8_quant_rows<BF16>, *a, (dtype == F32 ? 32 : 16) * across, st);
+    if (a->block_log2 == 0) {
+        const bool once = (uint64_t)a->n * a->rows * a->cols <= ONCE_MOST;
+        const auto f = dtype == F32   ? (once ? k_f8_quant_rows<F32, true> : k_f8_quant_rows<F32, false>)
+                       : dtype == F16 ? (once ? k_f8_quant_rows<F16, true> : k_f8_quant_rows<F16, false>)
+                                      : (once ? k_f8_quant_rows<BF16, true> : k_f8_quant_rows<BF16, false>);
+        return each_part(f, *a, (dtype == F32 ? 32 : 16) * across, st);
+    }
     const uint32_t down = (a->rows + 127) / 128, blocks = a->n * across * down;
     if (blocks == 0) return 0;
     const auto f = dtype == F32 ? k_f8_quant_blocks<F32> : dtype == F16 ? k_f8_quant_blocks<F16> : k_f8_quant_blocks<BF16>;
@@ -300,7 +323,13 @@ extern "C" int exl3c4_dev_f8_quant(const Exl3c4DevF8* a, int32_t dtype, void* st
 }
 
 extern "C" int exl3c4_dev_f8_dequant(const Exl3c4DevF8* a, int32_t dtype, void* stream) {
-    const auto f = dtype == F32 ? k_f8_dequant<F32> : dtype == F16 ? k_f8_dequant<F16> : k_f8_dequant<BF16>;
+    // Past the caches what the one behind L2 (256 MiB) does not hold anyway; less may be read there by what comes next. Rows that are no 16-byte units go through
+    // the caches, which join their pieces (20480 x 650 f32 14.7 us past them, 11.9 so).
+    const uint64_t bytes = (uint64_t)a->n * a->rows * a->cols * (dtype == F32 ? 4 : 2);
+    const bool once = bytes > 256u << 20 && (((uintptr_t)a->v | (uint64_t)a->v_pitch | (uint64_t)a->v_stride) & 15) == 0;
+    const auto f = dtype == F32   ? (once ? k_f8_dequant<F32, true> : k_f8_dequant<F32, false>)
+                   : dtype == F16 ? (once ? k_f8_dequant<F16, true> : k_f8_dequant<F16, false>)
+                                  : (once ? k_f8_dequant<BF16, true> : k_f8_dequant<BF16, false>);
     const uint32_t per = dtype == F32 ? 4 : 8, lanes = (a->cols + per - 1) / per;
     return each_part(f, *a, lanes < 2 ? 2 : lanes, (hipStream_t)stream);      // (a second lane of a single one's row stores nothing)
 }

@@ -42,7 +42,7 @@ __device__ __forceinline__ int wave_max_before(int v, int lane) {
     return lane == 0 ? 0 : up;
 }
 
-struct Chunk { int expert, row0, rows, tile; };                 // expert -1: rows that no run holds (zeros)
+struct Chunk { int expert, row0, rows, tile, alone; };          // expert -1: rows that no run holds (zeros); alone: its run has no other chunk
 
 // 512 experts from `base` on, eight a lane: where each run starts, and the wave's inclusive sum of their chunks. The offsets are
 // clamped to [0, T], and one below an earlier one counts as that one (`reach`: the largest so far). So whatever the table holds, the runs, the
@@ -83,7 +83,7 @@ template <int MT_LOG2> struct Runs {
     __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(incl, 63); }
     // chunk c of these (c < total())
     __device__ __forceinline__ void find(int base, int lane, int c, Chunk& out) const {
-        int r = c - (incl - own), e = 0, row0 = 0, rows = 0;
+        int r = c - (incl - own), e = 0, row0 = 0, rows = 0, alone = 0;
         const uint64_t hit = __ballot(r >= 0 && r < own);
         bool found = false;
 #pragma unroll
@@ -94,6 +94,7 @@ template <int MT_LOG2> struct Runs {
                 e = base + 8 * lane + j;
                 row0 = v[j] + (r << MT_LOG2);
                 rows = min(1 << MT_LOG2, len - (r << MT_LOG2));
+                alone = n == 1;
             }
             r -= n;
         }
@@ -101,6 +102,7 @@ template <int MT_LOG2> struct Runs {
         out.expert = __builtin_amdgcn_readlane(e, from);
         out.row0 = __builtin_amdgcn_readlane(row0, from);
         out.rows = __builtin_amdgcn_readlane(rows, from);
+        out.alone = __builtin_amdgcn_readlane(alone, from);
     }
 };
 
@@ -113,7 +115,7 @@ template <int MT_LOG2> struct Runs {
 template <int MT_LOG2, bool XCD>
 __device__ __forceinline__ Chunk find_unit(const Exl3c4DevGemm& a, int lane) {
     typedef Runs<MT_LOG2> R;
-    Chunk out = { -1, 0, 0, 0 };
+    Chunk out = { -1, 0, 0, 0, 0 };
     R s;
     int live = 0, head = 0, tail = 0;
     for (int base = 0; base < a.n_expert; base += 512) {
@@ -162,7 +164,7 @@ __device__ __forceinline__ Chunk my_unit(const Exl3c4DevGemm& a, int lane, int w
     }
     __syncthreads();
     return { __builtin_amdgcn_readfirstlane(unit.expert), __builtin_amdgcn_readfirstlane(unit.row0),
-             __builtin_amdgcn_readfirstlane(unit.rows), __builtin_amdgcn_readfirstlane(unit.tile) };
+             __builtin_amdgcn_readfirstlane(unit.rows), __builtin_amdgcn_readfirstlane(unit.tile), __builtin_amdgcn_readfirstlane(unit.alone) };
 }
 
 // The row of x that sorted row i reads, or -1: none (the row is zeros).
@@ -277,6 +279,12 @@ __device__ __forceinline__ void dma4(gaddr from, uint32_t lds) {
 // The same where `all` is -1, and nothing where it is 0 (uniform; the whole wave is active): no lane loads, without a branch.
 __device__ __forceinline__ void dma16_of(gaddr from, uint32_t lds, int all) {
     asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dwordx4 %0, off\n\ts_mov_b64 exec, -1" ::"v"(from), "s"(lds), "s"(all) : "memory", "m0");
+}
+// And where `once` is not 0 (uniform), past the caches: bytes that no other workgroup reads. (The branch is in the asm, so that it divides nothing.)
+__device__ __forceinline__ void dma16_of(gaddr from, uint32_t lds, int all, int once) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\ts_cmp_lg_u32 %3, 0\n\ts_cbranch_scc1 .Lonce%=\n\t"
+                 "global_load_lds_dwordx4 %0, off\n\ts_branch .Lthen%=\n.Lonce%=:\n\tglobal_load_lds_dwordx4 %0, off nt\n.Lthen%=:\n\ts_mov_b64 exec, -1"
+                 ::"v"(from), "s"(lds), "s"(all), "s"(once) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void dma4_of(gaddr from, uint32_t lds, int all) {
     asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1" ::"v"(from), "s"(lds), "s"(all) : "memory", "m0");

@@ -220,7 +220,8 @@ template <int T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // LDS. A row of a stage is 128 bytes (16-bit x: two such halves). The loads write lane after lane, 16 bytes each, so the order within a row is chosen
 // at the source: place p of row r holds the chunk q = p ^ (r & 7), in a half of a 16-bit row the chunk whose number is q's with its highest bit moved to the end,
 // so that lane groups g and g + 1 read places that differ in their lowest bit: the 16 rows and four lane groups that read a matrix operand then fall on all the
-// banks evenly (16-bit rows by q itself: 39% of the LDS cycles were conflicts, 1% so; 4096 tokens over 8 experts 56.0 -> 54.4 us). Behind x's rows a scale for each; behind the weights' those of the tile's blocks of weight rows.
+// banks evenly (16-bit rows by q itself: 39% of the LDS cycles were conflicts, 1% so; 4096 tokens over 8 experts 56.0 -> 54.4 us). Behind x's rows a scale for
+// each; behind the weights' those of the tile's blocks of weight rows.
 //
 // Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, so that a sum's scale is one number of the
 // lane's row of x times one that the wave shares.
@@ -233,13 +234,16 @@ template <int XT, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB> struct T
     static constexpr int NX = XL + XSL, NW = WL + 1;                         // a wave's loads of x and of weights, every stage
     static constexpr int AT_XS = XG * 1024, XSLOT = AT_XS + XS * 256, AT_W = XB * XSLOT, AT_WS = AT_W + WG * 1024, LDS = AT_WS + 256;
     static constexpr int TM = MT / WM / 16, TN = NT / WN / 16;               // matrix tiles a wave
+    // Rows of y past the caches, of larger tiles: 1500 tokens 188 -> 172, 2048 Zipf 222 -> 213, 4096 216 -> 210, 8192 over 8 experts, 2048 x 1408 71 -> 64, and whole layers of
+    // 1500 to 4096 tokens by 4% (in tiles of 32 rows 400 tokens 162 -> 165, a layer of 613 456 -> 464).
+    static constexpr bool LATER = MT_LOG2 > 5;
     // waves a SIMD, by the workgroups whose LDS a CU holds: what the compiler may use registers for
     static constexpr int GROUPS = 160 * 1024 / (LDS + 4 * MT + 1024), EU = GROUPS * WAVES_ / 4, WAVES_EU = EU > 8 ? 8 : EU;
     static_assert(XG % WAVES_ == 0 && WG % WAVES_ == 0 && (NX + NW) * 2 < 64 && TN % 2 == 0, "tile");
     static_assert((NT == 128 || NT == 256) && (XB == 2 || XB == 3), "one or two blocks of weight rows; places of x");
 };
 
-template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB, class G = Tile<XT, SW, MT_LOG2, NT, WM, WN, XB>>
+template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB, bool ONCE, class G = Tile<XT, SW, MT_LOG2, NT, WM, WN, XB>>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G::WAVES_EU, G::WAVES_EU))) void k_f8_tile(Exl3c4DevGemm a) {
     constexpr int MT = G::MT, WV = WM * WN, TM = G::TM, TN = G::TN;
     __shared__ __align__(1024) char lds[G::LDS];
@@ -290,7 +294,9 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             xp[i] += i < G::XL ? G::XROW : 4;
         };
         auto load_w = [&](int i, int all) {
-            if (i < G::WL) dma16_of(wp[i], at0 + G::AT_W + (wave + i * WV) * 1024, all);
+            const uint32_t to = at0 + G::AT_W + (wave + i * WV) * 1024;
+            if (i < G::WL && ONCE) dma16_of(wp[i], to, all, ch.alone);
+            else if (i < G::WL) dma16_of(wp[i], to, all);
             else dma4_of(wp[i], at0 + G::AT_WS, all);
             wp[i] += i < G::WL ? 128 : 4;
         };
@@ -444,6 +450,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
     const int size_log2 = MOST == 4 && a.y_type == EXL3C4_F32 ? 2 : 1, pitch = (OC << size_log2) + 16;
     const int per_log2 = 4 - size_log2, row_log2 = __builtin_ctz(OC) - per_log2;      // columns in 16 bytes; 16 bytes a row
     struct __attribute__((packed, aligned(2))) Part { uint32_t v[4]; };
+    typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 #pragma unroll
     for (int m0 = 0; m0 < TM; m0 += PM) {
         __syncthreads();                                         // the stages, or the pass before, are read
@@ -465,7 +472,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             if (rows_x[r] < 0) v = Part{ { 0, 0, 0, 0 } };
             char* y = a.y + (int64_t)(ch.row0 + r) * a.y_pitch + ((int64_t)col << size_log2);
             if (col + (1 << per_log2) <= a.n_out) {
-                *(Part*)y = v;
+                if constexpr (G::LATER) __builtin_nontemporal_store(u32x4{ v.v[0], v.v[1], v.v[2], v.v[3] }, (u32x4_at2*)y);
+                else *(Part*)y = v;
             } else if (size_log2 == 2) {
 #pragma unroll
                 for (int u = 0; u < 3; ++u)
@@ -495,7 +503,15 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     a.tiles = (a.n_out + cols - 1) / cols;
     const int64_t grid = (chunk_bound(a.T, a.n_expert, 1 << MT_LOG2) * a.tiles + 7) / 8 * 8;
     if (grid > THREADS / (64 * WM * WN)) return EXL3C4_E_SHAPE;
-    hipLaunchKernelGGL((k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
+    // Weights of runs that are one chunk, which no other workgroup reads, go past the caches where those of all experts that can be live are more than the one behind
+    // L2 holds (256 MiB), so that the next pass does not find them there; and then faster. Six sets of weights in turn, us: bf16 x, 32 tokens 95 -> 86; F8 x,
+    // 100 158 -> 138, 400 184 -> 163, 613 Zipf 2560 x 640 163 -> 158, 1500 194 -> 188. Of fewer, one set again and again, 8 tokens 27 -> 33, 64/6 32 tokens 23 -> 30.
+    // (For all runs' weights 2048 Zipf takes 241 for 226.) The choice is a branch at each load: 3% of a batch that does not need it, hence a kernel of its own, and in
+    // tiles of 128 rows more than it gives (4096 tokens 218 -> 226).
+    const int64_t live = a.n_expert < a.T ? a.n_expert : a.T;
+    const bool once = MT_LOG2 < 7 && live * a.N > ((int64_t)256 << 20) / a.K;
+    const auto f = once ? k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB, (MT_LOG2 < 7)> : k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB, false>;
+    hipLaunchKernelGGL(f, dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
     return launched();
 }
 
@@ -503,15 +519,15 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
 // the routing, which is on the device. Larger tiles read weights and rows less often; smaller ones waste less of a chunk, make more workgroups and
 // start sooner; the rows kernel splits k over its waves, so that few workgroups are enough. `units`: workgroups of a tile, each expert half a chunk
 // short of whole ones. Measured on one card, us, the product alone (E / top-k, N x K, tokens; 512/10, 1024 x 2048 with SwiGLU where nothing else is said):
-//   rows against 32        bf16 x: 1 token 8.6 / 13.3, 4 19.5 / 20.0, 8 30 / 27, 32 102 / 95; F8 x: 8 30 / 26, 16 55 / 49, 32 98 / 91.
+//   rows against 32        bf16 x: 1 token 8.6 / 13.3, 4 19.6 / 20.0, 8 30 / 27, 32 102 / 83; F8 x: 8 30 / 26, 16 55 / 56, 32 98 / 79.
 //                          64/6, 32 tokens 30 / 23; 8/2, 200 20 / 13. One expert, bf16 x: 2048 x 2048, 77 rows 10.7 / 13.2, 300 22 / 18;
-//                          8192 x 8192, 64 rows 48 / 57; 4096 x 4096, 16 rows 11.6 / 22, 300 74 / 35.
-//   2 strips against 4     one row, 8192 x 8192 16.4 / 23.6; 4096 x 4096, 16 rows 11.6 / 15.4; 8192 x 8192, 64 rows 61 / 48, which read the weights
+//                          8192 x 8192, 64 rows 48 / 57; 4096 x 4096, 16 rows 11.7 / 22, 300 74 / 35.
+//   2 strips against 4     one row, 8192 x 8192 16.5 / 23.6; 4096 x 4096, 16 rows 11.7 / 15.5; 8192 x 8192, 64 rows 61 / 48, which read the weights
 //                          once for each 16 rows, mostly from L2.
-//   32 rows against 64     as codes: 400 tokens 183 / 184, 613 Zipf 2560 x 640 160 / 168, 1500 218 / 192, 8/2 800 15.3 / 19.8. bf16 x: 400 184 / 200,
-//                          613 Zipf 2560 x 640 167 / 184, 1500 218 / 203, 8/2 800 19 / 27. F8 x, f32 y: 200 183 / 209, 1500 232 / 228.
-//   64 against 128         as codes: 1500 192 / 204, 2048 Zipf 224 / 230, 4096 274 / 218, 64/6 2000 52 / 42, 8/2 8192 2816 x 2048 144 / 111,
-//                          2048 x 1408, sorted rows in, 80 / 68.
+//   32 rows against 64     as codes: 400 tokens 160 / 165, 613 Zipf 2560 x 640 148 / 156, 1500 202 / 171, 8/2 800 15.9 / 21. bf16 x: 400 164 / 187,
+//                          613 Zipf 2560 x 640 156 / 172, 1500 200 / 191, 8/2 800 19 / 28. F8 x, f32 y: 200 161 / 200, 1500 217 / 215.
+//   64 against 128         as codes: 1500 172 / 200, 2048 Zipf 211 / 222, 4096 271 / 210, 64/6 2000 52 / 40, 8/2 8192 2816 x 2048 143 / 104,
+//                          2048 x 1408, sorted rows in, 79 / 64.
 // As codes a tile of 256 x 256 with a CU to itself took 131 there before the loads went among the products and 114 to 118 since, and was slower
 // everywhere else; 128 x 128 130 (73 for 77 at 2048 x 1408, sorted rows in); weights in two places 232 at 64 rows, and 2% less at 32 rows and 100 to 400
 // tokens. Widened: 128 x 128 in eight waves 344, 128 x 256 211 against 202 of 64 x 256.

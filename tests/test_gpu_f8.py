@@ -224,3 +224,20 @@ def test_zeros_keep_their_sign(ex, t):
     assert ex.f8_quant(x, q) == 0
     torch.cuda.synchronize()
     assert torch.equal(q.codes.cpu() >> 7, torch.signbit(x.cpu()).byte())
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("cols", [1024, 1022])
+def test_large_matrices_are_what_their_parts_are(ex, t, block, cols):
+    """More codes and values than the caches are meant to keep, which are stored past them: the same as of 1,280 rows at a time."""
+    rows = 1280 * 110
+    x = torch.randn((rows, cols), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(TYPES[t])
+    q, out = ex.f8_empty(x.shape, block), torch.empty_like(x)
+    assert ex.f8_quant(x, q) == 0 and ex.f8_dequant(q, out) == 0
+    part, values = ex.f8_empty((1280, cols), block), torch.empty((1280, cols), dtype=TYPES[t], device="cuda")
+    for r in range(0, rows, 1280 * 7):
+        assert ex.f8_quant(x[r:r + 1280], part) == 0 and ex.f8_dequant(part, values) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(q.codes[r:r + 1280], part.codes) and torch.equal(out[r:r + 1280], values)
+        assert torch.equal(q.scales[r // block:(r + 1280) // block], part.scales)

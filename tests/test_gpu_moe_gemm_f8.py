@@ -324,3 +324,41 @@ def test_offsets_past_32_bits(ex, xt, yt, T, pitch):
     assert not outs[0].isnan().any() and torch.equal(*outs)
     del xs, w, wf, x, xq, wq, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("xt,yt", [("bf16", "bf16"), ("f16", "f32"), ("f8", "bf16"), ("f8", "f32")])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("others,p", [(2, 32), (20, 64)])
+def test_weights_that_go_past_the_caches(ex, xt, yt, swiglu, others, p):
+    """More weights than the cache behind L2 holds (287 MB): runs of one chunk, of no row, of a chunk and a row, of whole chunks and of several, against the product
+    of their experts in 64 bits; the other experts' rows are written."""
+    E, N, K = 80, 3500, 1024
+    lens = [others] * E
+    some = {0: 1, 3: 0, 4: 33, 5: 64, 6: 65, 40: 32, 79: 130}
+    for e, n in some.items():
+        lens[e] = n
+    off = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    T, n_out = int(off[-1]), N // 2 if swiglu else N
+    assert path(ex, xt, yt, swiglu, T, E, n_out, K) == p
+    g = torch.Generator().manual_seed(p)
+    dg = torch.Generator(device="cuda").manual_seed(p)
+    codes = torch.randint(0, 254, (E, N, K), dtype=torch.uint8, device="cuda", generator=dg)
+    codes += (codes >= 127).to(torch.uint8)                       # 127 and 255 are NaN
+    halves = 2 if swiglu else 1
+    scales = torch.rand((E, halves * ((N // halves + 127) // 128), K // 128), generator=g) * 0.01 + 0.0005
+    x = torch.randn((T, K), generator=g)
+    xd, xv, xp = x_operand(ex, x, xt)
+    y = torch.full((T, n_out), float("nan"), dtype=TYPES[yt], device="cuda")
+    gm = ex.make_gemm(xd, ex.F8(codes, scales.cuda(), K, 128), None, torch.from_numpy(off).cuda(), y, act=ex.ACT_SWIGLU if swiglu else ex.ACT_NONE)
+    for _ in range(2):
+        assert ex.moe_gemm(gm) == 0
+        torch.cuda.synchronize()
+        got = y.cpu()
+        assert not got.isnan().any()
+        for e in some:
+            rows = slice(off[e], off[e + 1])
+            c, s = codes[e:e + 1].cpu(), scales[e:e + 1]
+            cut = (xp[rows], f8ref.peaks(c, f8ref.weights(torch.full_like(c, 0x38), s, halves))) if xt == "f8" and yt != "f32" else None
+            want, tol = f8ref.gemm(xv[rows], f8ref.weights(c, s, halves), None, [0, lens[e]], lens[e], 1, swiglu, cut)
+            assert mx4ref.close(got[rows], want, tol), e
+        y.fill_(float("nan"))
