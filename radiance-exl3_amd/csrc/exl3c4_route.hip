@@ -405,6 +405,7 @@ __global__ __launch_bounds__(PO_THREADS) void k_pairs_by_expert(const int32_t* i
         for (int r = 0; r < 4; ++r) look(q[r], i0 + 256 * r + 4 * lane);
     }
     for (; i0 < to; i0 += 256) look(load(i0 + 4 * lane), i0 + 4 * lane);
+    wave_sync();                                                  // the list is read by other lanes than wrote it
     below = wave_scan_incl(below);
     // f(x, pair) for 64 of the own pairs in order, one a lane (x: its expert of these, or PO_EXPERTS for none)
     auto each = [&](auto f) {
