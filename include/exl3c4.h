@@ -368,7 +368,8 @@ int exl3c4_f8_dequant(const Exl3c4F8* q, void* out, int32_t out_dtype, int64_t o
  *       x_pitch; MX4: w_scales, ws_stride and ws_pitch likewise (ws_stride 0: a pointer array)
  *       F8: x by blocks of one row (x_scales f32, xs_pitch bytes apart), w by blocks of 128 (w_scales f32, rows of blocks ws_pitch and experts
  *       ws_stride bytes apart); with SWIGLU the gate half and the up half of W_e are matrices of their own, whose rows of blocks follow each
- *       other: ceil(N / 2 / 128) of gate, then as many of up
+ *       other: ceil(N / 2 / 128) of gate, then as many of up. Scales may be any f32 numbers, on both sides whatever their product (x's below
+ *       2^-126 come in with a step of 2^-149; where x's pass 2^100 and the weights' 2^102 both, a block's sum of zero may come out as NaN)
  *       F8 x and y of 16 bits: beside sums in f32, experts of many rows take the matrix unit's 8-bit products, which cut each of eight
  *       neighbouring columns' products below 2^-13 of the largest of the eight (y in f32: every product is exact)
  *   y   [T, N or N / 2], y_pitch elements apart; shares no memory with the operands

@@ -4,7 +4,7 @@
 //
 // THE MATRIX STEP. A block of 128 columns is one step: y += sw sx (sum over the block of w x). Scales are any f32 numbers, so they come in as a
 // multiply-add of the sum, which begins at zero. It is taken in one of two ways:
-//   widened   the codes become 16-bit floats, which hold every e4m3 (bf16 for bf16 x, else f16), and four v_mfma_f32_16x16x32 add their products, each
+//   widened   the codes become 16-bit floats, which hold every e4m3 (f16 for f16 x, else bf16), and four v_mfma_f32_16x16x32 add their products, each
 //             exact in f32.
 //   as codes  one v_mfma_f32_16x16x128_f8f6f4, at some three times the rate. It adds eight neighbouring columns' products on a grid: each is cut
 //             towards zero to a multiple of 2^(E - 13), E the largest of the eight sums of the two codes' exponents; the eights are then added in
@@ -31,33 +31,48 @@ constexpr int F8 = EXL3C4_F8;
 // A lane's 32 codes of a row's block.
 struct Codes { uint4 h[2]; };
 
-__device__ __forceinline__ f32x4 mma_f8(const Codes& a, const Codes& b, f32x4 c) {
+// A weights' scale as f 2^(byte - 127), f of magnitude 1 to 2 and the byte as the matrix unit and the conversions take it. The product of x's scale and the weights'
+// may be no f32 number, or one of few bits, though the sum that it scales brings it back: so f32 multiplies x's by f alone, and the power comes in before
+// the sum, in the matrix unit or with the codes as they widen. It ends at 2^-108 and 2^102, between which f32 holds every sum of a block (f takes what is
+// beyond, as it does zeros, infinities and NaN). (Splitting x's scale too, a row each: the tiles of codes 109 -> 114 us, 66 -> 69.)
+struct Scale {
+    float f;
+    int byte;
+    __device__ __forceinline__ explicit Scale(float s) {
+        byte = min(max((int)(__float_as_uint(s) >> 23 & 255), 127 - 108), 127 + 102);
+        f = __builtin_amdgcn_ldexpf(s, 127 - byte);
+    }
+    __device__ __forceinline__ float power() const { return __uint_as_float((uint32_t)byte << 23); }
+};
+
+// The products times 2^(by - 127).
+__device__ __forceinline__ f32x4 mma_f8(const Codes& a, const Codes& b, int by, f32x4 c) {
     const i32x8 A = { (int)a.h[0].x, (int)a.h[0].y, (int)a.h[0].z, (int)a.h[0].w, (int)a.h[1].x, (int)a.h[1].y, (int)a.h[1].z, (int)a.h[1].w };
     const i32x8 B = { (int)b.h[0].x, (int)b.h[0].y, (int)b.h[0].z, (int)b.h[0].w, (int)b.h[1].x, (int)b.h[1].y, (int)b.h[1].z, (int)b.h[1].w };
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 0, 0, 0, 127, 0, 127);      // (e8m0 127: times 1)
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 0, 0, 0, by, 0, 127);
 }
 
-// 8 codes as 8 bf16 or f16 (e4m3 has four bits and exponents of -9 to 8: exact).
-template <int XT> __device__ __forceinline__ uint4 widen8(uint32_t lo, uint32_t hi) {
+// 8 codes, times a power of two, as 8 bf16 or f16 (e4m3 has four bits and exponents of -9 to 8: exact).
+template <int XT> __device__ __forceinline__ uint4 widen8(uint32_t lo, uint32_t hi, float by) {
     if constexpr (XT == BF16)
-        return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true)) };
+        return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, by, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, by, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, by, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, by, true)) };
     else
-        return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true)) };
+        return { __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, by, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, by, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, by, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, by, true)) };
 }
 // Eight codes of the lane's 32, j = 0 .. 3.
-template <int XT> __device__ __forceinline__ uint4 widen_part(const Codes& q, int j) {
+template <int XT> __device__ __forceinline__ uint4 widen_part(const Codes& q, int j, float by = 1.f) {
     const uint4& w = q.h[j >> 1];
-    return j & 1 ? widen8<XT>(w.z, w.w) : widen8<XT>(w.x, w.y);
+    return j & 1 ? widen8<XT>(w.z, w.w, by) : widen8<XT>(w.x, w.y, by);
 }
 
 // The type that F8 codes widen to beside x of type XT.
-template <int XT> constexpr int WIDER = XT == BF16 ? BF16 : F16;
+template <int XT> constexpr int WIDER = XT == F16 ? F16 : BF16;
 
 __device__ __forceinline__ float load_f32(gaddr p) { return *(const __attribute__((address_space(1))) float*)p; }
 __device__ __forceinline__ float word(const uint4& v, int i) { return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w); }
@@ -133,11 +148,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_f8_rows(Exl3c4DevGemm a) {
         auto step = [&](const Codes* q, const uint4* v, const float* sw, const float* sx) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
+                const Scale k(sw[s]);
                 f32x4 p = { 0, 0, 0, 0 };
 #pragma unroll
-                for (int j = 0; j < 4; ++j) p = mma<WIDER<XT>>(XT == F8 ? widen_part<F16>(Codes{ v[0], v[1] }, j) : v[j], widen_part<WIDER<XT>>(q[s], j), p);
+                for (int j = 0; j < 4; ++j)
+                    p = XT == F8 ? mma<BF16>(widen_part<BF16>(Codes{ v[0], v[1] }, j), widen_part<BF16>(q[s], j, k.power()), p)
+                                 : mma<WIDER<XT>>(v[j], widen_part<WIDER<XT>>(q[s], j), p);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[r], XT == F8 ? sx[r] * sw[s] : sw[s], acc[s][r]);
+                for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[r], XT == F8 ? sx[r] * k.f : sw[s], acc[s][r]);
             }
         };
         int t = from;
@@ -330,6 +348,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             };
             // (a wave's weight rows lie in one block of 128; with SwiGLU its even tiles in the gate's, its odd ones in the up's)
             const float sw[2] = { WS[SW ? 0 : (wn * TN * 16) >> 7], WS[1] };
+            const Scale kw[2] = { Scale(sw[0]), Scale(sw[1]) };
             Codes wv[TN];
 #pragma unroll
             for (int n = 0; n < TN; ++n) wv[n] = codes(W, wr + 16 * n);
@@ -341,7 +360,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                 f32x4 p[LAG + 1];
                 xv[0] = codes(X, xr);
                 f[0][0] = f[0][1] = XS[xr];
-                f[0][0] *= sw[0], f[0][1] *= sw[1];
+                f[0][0] *= kw[0].f, f[0][1] *= kw[1].f;
 #pragma unroll
                 for (int i = 0; i < TM * TN + LAG; ++i) {
                     const int m = i / TN, n = i % TN;
@@ -350,13 +369,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                             if (m + 1 < TM) xv[(m + 1) & 1] = codes(X, xr + 16 * (m + 1));
                             between(m);
                         }
-                        p[i % (LAG + 1)] = mma_f8(wv[n], xv[m & 1], f32x4{ 0, 0, 0, 0 });
+                        p[i % (LAG + 1)] = mma_f8(wv[n], xv[m & 1], kw[SW ? n & 1 : 0].byte, f32x4{ 0, 0, 0, 0 });
                     }
                     if (i >= LAG) {
                         const int k = i - LAG, km = k / TN, kn = k % TN;
                         if (kn == 0 && km > 0) {
                             const float sx = XS[xr + 16 * km];
-                            f[km & 1][0] = sx * sw[0], f[km & 1][1] = sx * sw[1];
+                            f[km & 1][0] = sx * kw[0].f, f[km & 1][1] = sx * kw[1].f;
                         }
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
@@ -364,7 +383,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                     }
                 }
             } else {
-                // x's eights j of columns: 16 g + 8 j of the block's first half, then of its second
+                // x's eights j of columns: 16 g + 8 j of the block's first half, then of its second. (The weights' power comes in with x's codes where it is
+                // one for all: with the weights' a register more, and a spill's reload waits for the loads ahead, 34.0 -> 36.2 us of 300 rows of 4096 x 4096.)
                 uint4 xv[TM][4];
                 float sx[TM];
 #pragma unroll
@@ -372,7 +392,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                     if constexpr (XT == F8) {
                         const Codes c = codes(X, xr + 16 * m);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) xv[m][j] = widen_part<F16>(c, j);
+                        for (int j = 0; j < 4; ++j) xv[m][j] = widen_part<BF16>(c, j, SW ? 1.f : kw[0].power());
                         sx[m] = XS[xr + 16 * m];
                     } else {
 #pragma unroll
@@ -386,13 +406,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                     f32x4 p[TM] = {};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 w = widen_part<WIDER<XT>>(wv[n], j);
+                        const uint4 w = XT == F8 ? widen_part<BF16>(wv[n], j, SW ? kw[n & 1].power() : 1.f) : widen_part<WIDER<XT>>(wv[n], j);
 #pragma unroll
                         for (int m = 0; m < TM; ++m) p[m] = mma<WIDER<XT>>(w, xv[m][j], p[m]);
                     }
 #pragma unroll
                     for (int m = 0; m < TM; ++m) {
-                        const float f = XT == F8 ? sx[m] * sw[SW ? n & 1 : 0] : sw[SW ? n & 1 : 0];
+                        const float f = XT == F8 ? sx[m] * kw[SW ? n & 1 : 0].f : sw[SW ? n & 1 : 0];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[n][m][r] = __builtin_fmaf(p[m][r], f, acc[n][m][r]);
                     }
