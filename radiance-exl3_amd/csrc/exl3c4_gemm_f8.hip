@@ -31,10 +31,11 @@ constexpr int F8 = EXL3C4_F8;
 // A lane's 32 codes of a row's block.
 struct Codes { uint4 h[2]; };
 
-// A weights' scale as f 2^(byte - 127), f of magnitude 1 to 2 and the byte as the matrix unit and the conversions take it. The product of x's scale and the weights'
-// may be no f32 number, or one of few bits, though the sum that it scales brings it back: so f32 multiplies x's by f alone, and the power comes in before
-// the sum, in the matrix unit or with the codes as they widen. It ends at 2^-108 and 2^102, between which f32 holds every sum of a block (f takes what is
-// beyond, as it does zeros, infinities and NaN). (Splitting x's scale too, a row each: the tiles of codes 109 -> 114 us, 66 -> 69.)
+// A weights' scale as f 2^(byte - 127), f of magnitude 1 to 2 and the byte as the matrix unit and the conversions take it. A sum of codes' products, with F8 x
+// the product of the two scales as well, may be no f32 number, or one of few bits, though the other factors bring it back: so the power comes in before
+// the sum, in the matrix unit or with the codes as they widen, and f32 multiplies by f (x's scale times f) behind it. With f16 x both stay in f32's
+// range anyway. The power ends at 2^-108 and 2^102, between which f32 holds every sum of codes (f takes what is beyond, as it does zeros, infinities
+// and NaN). (Splitting x's scale too, a row each: the tiles of codes 109 -> 114 us, 66 -> 69.)
 struct Scale {
     float f;
     int byte;
@@ -152,10 +153,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_f8_rows(Exl3c4DevGemm a) {
                 f32x4 p = { 0, 0, 0, 0 };
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    p = XT == F8 ? mma<BF16>(widen_part<BF16>(Codes{ v[0], v[1] }, j), widen_part<BF16>(q[s], j, k.power()), p)
-                                 : mma<WIDER<XT>>(v[j], widen_part<WIDER<XT>>(q[s], j), p);
+                    p = mma<WIDER<XT>>(XT == F8 ? widen_part<BF16>(Codes{ v[0], v[1] }, j) : v[j], widen_part<WIDER<XT>>(q[s], j, XT == F16 ? 1.f : k.power()), p);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[r], XT == F8 ? sx[r] * k.f : sw[s], acc[s][r]);
+                for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[r], XT == F8 ? sx[r] * k.f : XT == BF16 ? k.f : sw[s], acc[s][r]);
             }
         };
         int t = from;
@@ -406,13 +406,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                     f32x4 p[TM] = {};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 w = XT == F8 ? widen_part<BF16>(wv[n], j, SW ? kw[n & 1].power() : 1.f) : widen_part<WIDER<XT>>(wv[n], j);
+                        const uint4 w = widen_part<WIDER<XT>>(wv[n], j, XT == F16 || (XT == F8 && !SW) ? 1.f : kw[SW ? n & 1 : 0].power());
 #pragma unroll
                         for (int m = 0; m < TM; ++m) p[m] = mma<WIDER<XT>>(w, xv[m][j], p[m]);
                     }
 #pragma unroll
                     for (int m = 0; m < TM; ++m) {
-                        const float f = XT == F8 ? sx[m] * kw[SW ? n & 1 : 0].f : sw[SW ? n & 1 : 0];
+                        const float k = XT == F16 ? sw[SW ? n & 1 : 0] : kw[SW ? n & 1 : 0].f, f = XT == F8 ? sx[m] * k : k;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[n][m][r] = __builtin_fmaf(p[m][r], f, acc[n][m][r]);
                     }

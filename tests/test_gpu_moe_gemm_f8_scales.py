@@ -1,5 +1,6 @@
 """moe_gemm with F8 on both sides where a block's two scales multiply to numbers that f32 does not hold, or holds with fewer bits, though it holds the
-sums: scales that multiply to 2^135 on the smallest codes, and to 2^-140 on the largest, zeros among them. On every kernel, against the product in 64 bits."""
+sums: scales that multiply to 2^135 on the smallest codes, and to 2^-140 on the largest, zeros among them; and bf16 rows whose products with codes alone
+f32 does not hold. On every kernel, against the product in 64 bits."""
 import numpy as np
 import pytest
 
@@ -97,3 +98,23 @@ def test_scales_of_zero_infinity_and_nan(ex, yt, p):
 def test_zeros_whatever_the_scales_with_swiglu(ex, yt, p):
     got, want, _ = product(ex, yt, p, ((0x00, 0x80), 2.0 ** 70, 2.0 ** 65), swiglu=True)
     assert (want == 0).all() and (got == 0).all()
+
+
+@pytest.mark.parametrize("yt,p", [(y, p) for y in ("f32", "bf16") for p in (2, 4, 32, 64)])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_bf16_rows_near_the_end_of_f32(ex, yt, p, swiglu):
+    """x up to 3e38 against weights far below 1 by their scale, not by their codes (gate and up: 2^-130, so that their product stays in f32)."""
+    T, E, N, K = SIZES[p]
+    assert path(ex, "bf16", yt, swiglu, T, E, N // 2 if swiglu else N, K) == p
+    g = torch.Generator().manual_seed(p)
+    x = (torch.randn((T, K), generator=g).clamp(-3, 3) * 1e38).bfloat16()
+    _, _, _, _, cw, ws, wv, _ = operands(g, (0x00, 0x7E, 0x78, 0xF9, 0xFE, 0x38), 1.0, 2.0 ** (-130 if swiglu else -24), T, E, N, K, swiglu)
+    off = np.array([T * e // E for e in range(E + 1)], np.int32)
+    n_out = N // 2 if swiglu else N
+    y = torch.full((T, n_out), 5.0, dtype=TYPES[yt], device="cuda")
+    gm = ex.make_gemm(x.cuda(), ex.F8(cw.cuda(), ws.cuda(), K, 128), None, torch.from_numpy(off).cuda(), y, act=ex.ACT_SWIGLU if swiglu else ex.ACT_NONE)
+    assert ex.moe_gemm(gm) == 0
+    torch.cuda.synchronize()
+    want, tol = f8ref.gemm(x.double(), wv, None, off, T, 1, swiglu)
+    assert want.abs().amax() < 3e38
+    assert mx4ref.close(y.cpu(), want, tol)
