@@ -370,8 +370,10 @@ int exl3c4_f8_dequant(const Exl3c4F8* q, void* out, int32_t out_dtype, int64_t o
  *       ws_stride bytes apart); with SWIGLU the gate half and the up half of W_e are matrices of their own, whose rows of blocks follow each
  *       other: ceil(N / 2 / 128) of gate, then as many of up. Scales may be any f32 numbers, on both sides whatever their product (x's below
  *       2^-126 come in with a step of 2^-149; where x's pass 2^100 and the weights' 2^102 both, a block's sum of zero may come out as NaN)
- *       F8 x and y of 16 bits: beside sums in f32, experts of many rows take the matrix unit's 8-bit products, which cut each of eight
- *       neighbouring columns' products below 2^-13 of the largest of the eight (y in f32: every product is exact)
+ *       F8 x and y of 16 bits: beside sums in f32, experts of many rows (by T, N, K and n_expert: tiles of rows) take the matrix unit's 8-bit
+ *       products. Of each eight neighbouring columns (8 j .. 8 j + 7) seven products may be cut, each by less than 2^-13 of the largest
+ *       product of the eight, where each code's magnitude counts as 2^-6 at least (a subnormal code counts by its exponent). So the bits of a
+ *       row may differ with the batch that it is in. Few rows, and any with y in f32: every product is exact
  *   y   [T, N or N / 2], y_pitch elements apart; shares no memory with the operands
  * 16-bit operands: K % 8 == 0, base, pitch and stride in multiples of 16 bytes; with an MX4 operand K % 32 == 0, with F8 K % 16 == 0; scale bases, pitches
  * and strides in multiples of 4 bytes. N is any. Refusals: INVAL (an unknown act, a required operand absent), DTYPE (another pair of

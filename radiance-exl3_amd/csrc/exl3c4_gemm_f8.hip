@@ -8,10 +8,12 @@
 //             exact in f32.
 //   as codes  one v_mfma_f32_16x16x128_f8f6f4, at some three times the rate. It adds eight neighbouring columns' products on a grid: each is cut
 //             towards zero to a multiple of 2^(E - 13), E the largest of the eight sums of the two codes' exponents; the eights are then added in
-//             f32 (found by giving it one product at a time beside a large one). A sum is off by less than 7 x 2^-13 of the largest product of
-//             each eight; of normally distributed rows by 1.4e-5 of the products' norm.
+//             f32 (found by giving it one product at a time beside a large one). A subnormal code's exponent is -6, however small it is: a sum is
+//             off by less than 7 x 2^-13 of each eight's largest product of magnitudes that count as 2^-6 at least; of normally distributed rows
+//             by 1.4e-5 of the products' norm.
 // Few rows against many weights are bound by memory, and widen. Tiles take F8 x as codes where y has 16 bits, whose own rounding (2^-9 or 2^-12 of the
-// value) and the codes' (2^-4) are far larger; where y is f32 they widen too.
+// value) and the codes' (2^-4) are far larger: from 64 bits bf16 rows are as far either way (1.7e-3 of the norm). Codes / widened, us: 8192 tokens
+// over 8 experts, 2816 x 2048 111 / 246; 4096 over 512 214 / 393; 1500 172 / 225; 800 over 8 16.5 / 20.8; 613 Zipf 147 / 153. Where y is f32 they widen.
 // Lane l holds of row l % 16, with g = l / 16, the 16 columns from 16 g and those from 64 + 16 g of the block.
 #include <hip/hip_runtime.h>
 
