@@ -267,7 +267,9 @@ int exl3c4_router_topk_scatter(const void* logits, int32_t logits_dtype, int64_t
  *     expert_ids i32 [n_tok][top_k]: the experts of the largest choice in the groups that stay, ties to the lower id, in that order;
  *                -1 for each slot behind the last one that is not out
  *     expert_w   f32 [n_tok][top_k]: their scores (0 of a slot with -1), divided by their sum where renorm is 1 (0 where that is 0), times scale
- * All of it in 64 bits (the order of two experts as well), the weights rounded once.
+ * All of it in 64 bits, the weights rounded once. The order is that of the choices as f64 has them, whose scores are within 2^-51 (SIGMOID) or 2^-48
+ * (SOFTMAX) of their values; two choices or two groups that differ by less may come in either order, the same one on every launch. Without
+ * a bias the order of experts, and of groups by GROUP_MAX, is exact.
  * Where expert_offset is not null the pairs are scattered as well, as exl3c4_moe_scatter does with expert_base 0 (slots of -1 are dropped;
  * expert_count and row_of may be null); up to 16 tokens in the same launch. Limits: 1 <= n_expert <= 1024, n_group divides n_expert, n_group <= 64,
  * top_group <= n_group, top_k <= min(64, top_group * n_expert / n_group). Refusals before anything is written: INVAL (a null pointer, an unknown
