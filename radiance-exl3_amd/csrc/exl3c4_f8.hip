@@ -1,19 +1,26 @@
-// exl3c4_f8.hip -- matrices of f16, bf16 or f32 to 8-bit floats with an f32 scale for each block of 128 columns (F8: e4m3 codes) and back, on
-// gfx950 (include/exl3c4.h has the format). No counterpart in the reference.
+// exl3c4_f8.hip -- matrices of f16, bf16 or f32 to 8-bit floats with an f32 scale for each block of 128 columns (F8: e4m3
+// codes) and back, on gfx950 (include/exl3c4.h has the format). No counterpart in the reference.
 //
-// A block's scale is a / 448 with a = max(largest magnitude, 2^-96), its codes x (448 / a) to the nearest e4m3: both quotients and the product
-// are rounded once in f32, so that another implementation of these steps gives the same codes. The largest magnitude is found on the bits, where
-// infinities and NaNs are the largest. v_cvt_pk_fp8_f32 rounds to nearest even (checked for every tie against that rule).
+// A block's scale is a / 448 with a = max(largest magnitude, 2^-96), its codes x (448 / a) to the nearest e4m3: both quotients
+// and the product are rounded once in f32, so that another implementation of these steps gives the same codes. The largest
+// magnitude is found on the bits, where infinities and NaNs are the largest. v_cvt_pk_fp8_f32 rounds to nearest even (checked
+// for every tie against that rule).
 //
-// Blocks of one row: a lane takes 16 bytes of values, 8 columns of 16 bits or 4 of 32, so that a wave's loads and stores are whole lines; the 16 or 32
-// lanes of a block find the largest by DPP. Blocks of 128 rows: a workgroup each, 16 lanes for the 256 bytes or twice 256 bytes of a row and every value of the block in its
-// registers, so that memory is read once. The same columns a lane on the way back.
+// Blocks of one row: a lane takes 16 bytes of values, 8 columns of 16 bits or 4 of 32, so that a wave's loads and stores are
+// whole lines; the 16 or 32 lanes of a block find the largest by DPP. Blocks of 128 rows: a workgroup each, 16 lanes for the
+// 256 bytes or twice 256 bytes of a row and every value of the block in its registers, so that memory is read once. The same
+// columns a lane on the way back.
 //
-// What bounds it: memory, with the VALU next to it (85% busy in rows). What is read or written once goes past the caches (ONCE): values back 131072 x 1000 f32 94 us for
-// 114, f16 57 for 69; blocks of 128 rows, values in whole lines, 131072 x 1000 f32 135 for 157, f16 91 for 105 (their codes, a line a row, 105 -> 139: through the
-// caches). Quantising and back, us (TB/s of both sides' bytes): rows, 20480 x 650 f16 10.0 (4.0) and 8.7 (4.6), 8192 x 2048 f16 9.9 (5.1) and 8.9; blocks,
-// 131072 x 1000 f32 135 (4.9) and 94 (7.0, part of it into the cache behind L2); 64 x 2048 3.2 and 2.7, a launch.
-// Tried without a gain: a row's end shifted by selects of words in place of 64-bit shifts (20480 x 650 0.3 us less, 8192 x 2048 1 more: the loads' order).
+// What bounds it: memory, with the VALU next to it (85% busy in rows). Each way alone, us (TB/s of both sides' bytes):
+//   rows of f16       20480 x 650 10.0 (4.0), back 8.7 (4.6); 8192 x 2048 9.9 (5.1), back 8.9
+//   blocks, f32       131072 x 1000 135 (4.9), back 94 (7.0, part of it into the cache behind L2); 64 x 2048 3.2, back 2.7: a
+//                     launch
+// What is read or written once goes past the caches (ONCE). Through them / past them, us, 131072 x 1000:
+//   values back                          f32 114 / 94, f16 69 / 57
+//   values in, blocks (whole lines)      f32 157 / 135, f16 105 / 91
+//   codes out, blocks (a line a row)     105 / 139: through them
+// Tried without a gain: a row's end shifted by selects of words in place of 64-bit shifts (20480 x 650 0.3 us less, 8192 x 2048
+// 1 more: the loads' order).
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -26,9 +33,11 @@ constexpr int F32 = EXL3C4_F32, F16 = EXL3C4_F16, BF16 = EXL3C4_BF16;
 constexpr int WG = 256;
 constexpr int PER = 4;                                          // slots (16 bytes of values) a lane, where rows are apart
 constexpr int64_t SLOTS = (int64_t)1 << 31;                     // slots a launch indexes in 32 bits
-// Codes up to which rows' are stored past the caches (below, ONCE). Quantising alone is faster so at any size (20480 x 650 f16 8.5 for 10.2 us, 8192 x 2048 7.8 for
-// 10.0); the products that read them then are not. A layer of route, quantising, products and gather, codes through the caches / past them: 512 experts, 2048 tokens (4
-// and 10 M codes) 354 / 341 us, 1500 334 / 326, 613 467 / 464; 8 experts, 4096 tokens (8 and 11 M) 149 / 151, 8192 (16 and 22 M) 241 / 247.
+// Codes up to which rows' are stored past the caches (ONCE). Quantising alone is faster so at any size, the products that read the codes
+// then are not. Codes through the caches / past them, us:
+//   quantising alone    20480 x 650 f16 10.2 / 8.5, 8192 x 2048 10.0 / 7.8
+//   a layer (route, quantising, products, gather)    512 experts, 2048 tokens (4 and 10 M codes) 354 / 341, 1500 334 / 326, 613 467 / 464;
+//                       8 experts, 4096 tokens (8 and 11 M) 149 / 151, 8192 (16 and 22 M) 241 / 247
 constexpr uint64_t ONCE_MOST = 8 << 20;
 constexpr float TOP = 448.f;                                    // e4m3's largest
 constexpr uint32_t LEAST = 31u << 23;                           // 2^-96, the least magnitude that sets a scale: 448 / a stays finite
@@ -41,8 +50,8 @@ typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 template <int DT> constexpr int COLS = DT == F32 ? 4 : 8;       // values in 16 bytes
 template <int DT> constexpr int SIZE = DT == F32 ? 4 : 2;
 
-// Columns c .. of a row at p (its column c) in 16 bytes, those from `cols` on as zeros: the row's last 16 bytes where they would pass its end, shifted
-// (2-byte loads of each took 20480 x 650 f16 from 9 to 14 us).
+// Columns c .. of a row at p (its column c) in 16 bytes, those from `cols` on as zeros: the row's last 16 bytes where they
+// would pass its end, shifted (2-byte loads of each took 20480 x 650 f16 from 9 to 14 us).
 template <int DT, bool ONCE = false> __device__ __forceinline__ void load16b(uint32_t* v, const char* p, uint32_t c, uint32_t cols) {
     constexpr uint32_t C = COLS<DT>;
     if (cols >= C) {                                             // (uniform)
@@ -105,9 +114,10 @@ __device__ __forceinline__ uint32_t max32(uint32_t v) {
     return max(r[0], r[1]);
 }
 
-// A block's scale a / 448 and 448 / a, each rounded once: a quotient's remainder by a multiply-add, and the quotient corrected by it. 448 / a is taken
-// of a's mantissa, whose reciprocal has one step of Newton's behind the hardware's; with that one off by up to two steps both are right for every
-// mantissa (all of them tried). (The compiler's division is 14 instructions for each, of every lane: 20480 x 650 f16 14 us with them.)
+// A block's scale a / 448 and 448 / a, each rounded once: a quotient's remainder by a multiply-add, and the quotient corrected
+// by it. 448 / a is taken of a's mantissa, whose reciprocal has one step of Newton's behind the hardware's; with that one off
+// by up to two steps both are right for every mantissa (all of them tried). (The compiler's division is 14 instructions for
+// each, of every lane: 20480 x 650 f16 14 us with them.)
 struct Scale {
     float s, inv;
     __device__ __forceinline__ explicit Scale(uint32_t top) {
@@ -123,7 +133,8 @@ struct Scale {
         if (top >= 0x7F800000u) s = __uint_as_float(0x7FC00000u), inv = 0.f;
     }
 };
-// A value times k, rounded once: f16's by the multiply-add that widens an operand (plus -0, so that a zero keeps its sign), 8192 x 2048 10.4 -> 10.0 us.
+// A value times k, rounded once: f16's by the multiply-add that widens an operand (plus -0, so that a zero keeps its sign),
+// 8192 x 2048 10.4 -> 10.0 us.
 template <int DT> __device__ __forceinline__ float scaled(const uint32_t* v, int i, float k) {
     if constexpr (DT == F16) {
         float r;
@@ -186,7 +197,8 @@ __global__ __launch_bounds__(WG) void k_f8_quant_rows(Exl3c4DevF8 a, Slots sl) {
         const uint32_t m = magnitude<DT>(v[j]);
         const Scale k(DT == F32 ? max32(m) : max16(m));
         if (first + j * WG >= sl.count) continue;
-        if (C * at[j] < a.code_cols) store_codes<DT, ONCE>(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + C * at[j], v[j], k);
+        if (C * at[j] < a.code_cols)
+            store_codes<DT, ONCE>(a.codes + w[j].mat * a.codes_stride + w[j].row * a.codes_pitch + C * at[j], v[j], k);
         if ((at[j] & ((1u << BLOCK_LOG2) - 1)) == 0)
             *(float*)((char*)a.scales + w[j].mat * a.scales_stride + w[j].row * a.scales_pitch + (at[j] >> BLOCK_LOG2) * 4) = k.s;
     }
@@ -226,7 +238,8 @@ __global__ __launch_bounds__(WG) void k_f8_quant_blocks(Exl3c4DevF8 a, uint32_t 
     for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int h = 0; h < H; ++h)
-            if (r0 + 16 * j < a.rows && c + 64 * h < a.code_cols) store_codes<DT, false>(q + (r0 + 16 * j) * a.codes_pitch + 64 * h, v[j][h], k);
+            if (r0 + 16 * j < a.rows && c + 64 * h < a.code_cols)
+                store_codes<DT, false>(q + (r0 + 16 * j) * a.codes_pitch + 64 * h, v[j][h], k);
     if (threadIdx.x == 0) *(float*)((char*)a.scales + m * a.scales_stride + rb * a.scales_pitch + cb * 4) = k.s;
 }
 
@@ -248,7 +261,8 @@ __global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, Slots sl) {
             const uint2 u = *(const uint2*)p;
             q[j][0] = u.x, q[j][1] = u.y;
         }
-        scale[j] = *(const float*)((const char*)a.scales + w[j].mat * a.scales_stride + (w[j].row >> a.block_log2) * a.scales_pitch + (at[j] >> BLOCK_LOG2) * 4);
+        scale[j] = *(const float*)((const char*)a.scales + w[j].mat * a.scales_stride + (w[j].row >> a.block_log2) * a.scales_pitch +
+                                   (at[j] >> BLOCK_LOG2) * 4);
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -266,9 +280,11 @@ __global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, Slots sl) {
         for (int i = 0; i < 4; ++i) {
             if constexpr (DT == F32) o[i] = __float_as_uint(f[i]);
             else if constexpr (DT == F16)
-                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]) << 16;
+                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i]) |
+                       (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]) << 16;
             else
-                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) << 16;
+                o[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i]) |
+                       (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) << 16;
         }
         if (c + C <= a.cols) {
             if constexpr (ONCE) __builtin_nontemporal_store(o, (u32x4_at2*)p);
@@ -286,11 +302,13 @@ __global__ __launch_bounds__(WG) void k_f8_dequant(Exl3c4DevF8 a, Slots sl) {
 
 int launched() { return hipGetLastError() == hipSuccess ? 0 : EXL3C4_E_DEVICE; }
 
-// All the matrices' rows in launches whose slots fit 31 bits (8 G columns each: one launch in all but the largest cases). lanes: at least 2 a row.
+// All the matrices' rows in launches whose slots fit 31 bits (8 G columns each: one launch in all but the largest cases).
+// lanes: at least 2 a row.
 template <class K>
 int each_part(K kernel, const Exl3c4DevF8& a, uint32_t lanes, hipStream_t st) {
     const uint32_t all = a.n * a.rows, most = (uint32_t)((SLOTS - 1) / lanes < 1 ? 1 : (SLOTS - 1) / lanes);
-    uint32_t l = 1;                                              // ceil(log2 lanes): ceil(2^(31 + l) / lanes) fits 32 bits, and its product is exact below 2^31
+    // l: ceil(log2 lanes), so that ceil(2^(31 + l) / lanes) fits 32 bits, and its product is exact below 2^31
+    uint32_t l = 1;
     while (((uint32_t)1 << l) < lanes) ++l;
     const uint32_t mul = (uint32_t)((((uint64_t)1 << (31 + l)) + lanes - 1) / lanes);
     for (uint32_t r = 0; r < all;) {
@@ -323,8 +341,8 @@ extern "C" int exl3c4_dev_f8_quant(const Exl3c4DevF8* a, int32_t dtype, void* st
 }
 
 extern "C" int exl3c4_dev_f8_dequant(const Exl3c4DevF8* a, int32_t dtype, void* stream) {
-    // Past the caches what the one behind L2 (256 MiB) does not hold anyway; less may be read there by what comes next. Rows that are no 16-byte units go through
-    // the caches, which join their pieces (20480 x 650 f32 14.7 us past them, 11.9 so).
+    // Past the caches what the one behind L2 (256 MiB) does not hold anyway; less may be read there by what comes next. Rows
+    // that are no 16-byte units go through the caches, which join their pieces (20480 x 650 f32 14.7 us past them, 11.9 so).
     const uint64_t bytes = (uint64_t)a->n * a->rows * a->cols * (dtype == F32 ? 4 : 2);
     const bool once = bytes > 256u << 20 && (((uintptr_t)a->v | (uint64_t)a->v_pitch | (uint64_t)a->v_stride) & 15) == 0;
     const auto f = dtype == F32   ? (once ? k_f8_dequant<F32, true> : k_f8_dequant<F32, false>)

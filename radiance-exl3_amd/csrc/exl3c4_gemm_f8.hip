@@ -1,19 +1,20 @@
-// exl3c4_gemm_f8.hip -- the products of routed experts whose weights are F8 (e4m3 codes, an f32 scale each 128 x 128), against x in F8 (a
-// scale each row and 128 columns), f16 or bf16, on gfx950 (wave64): y[i] = W_e x[row i] over the sorted rows of each expert's run, with SwiGLU
-// where asked (include/exl3c4.h). No counterpart in the reference.
+// exl3c4_gemm_f8.hip -- the products of routed experts whose weights are F8 (e4m3 codes, an f32 scale each 128 x 128), against
+// x in F8 (a scale each row and 128 columns), f16 or bf16, on gfx950 (wave64): y[i] = W_e x[row i] over the sorted rows of each
+// expert's run, with SwiGLU where asked (include/exl3c4.h). No counterpart in the reference.
 //
-// THE MATRIX STEP. A block of 128 columns is one step: y += sw sx (sum over the block of w x). Scales are any f32 numbers, so they come in as a
-// multiply-add of the sum, which begins at zero. It is taken in one of two ways:
-//   widened   the codes become 16-bit floats, which hold every e4m3 (f16 for f16 x, else bf16), and four v_mfma_f32_16x16x32 add their products, each
-//             exact in f32.
-//   as codes  one v_mfma_f32_16x16x128_f8f6f4, at some three times the rate. It adds eight neighbouring columns' products on a grid: each is cut
-//             towards zero to a multiple of 2^(E - 13), E the largest of the eight sums of the two codes' exponents; the eights are then added in
-//             f32 (found by giving it one product at a time beside a large one). A subnormal code's exponent is -6, however small it is: a sum is
-//             off by less than 7 x 2^-13 of each eight's largest product of magnitudes that count as 2^-6 at least; of normally distributed rows
-//             by 1.4e-5 of the products' norm.
-// Few rows against many weights are bound by memory, and widen. Tiles take F8 x as codes where y has 16 bits, whose own rounding (2^-9 or 2^-12 of the
-// value) and the codes' (2^-4) are far larger: from 64 bits bf16 rows are as far either way (1.7e-3 of the norm). Codes / widened, us: 8192 tokens
-// over 8 experts, 2816 x 2048 111 / 246; 4096 over 512 214 / 393; 1500 172 / 225; 800 over 8 16.5 / 20.8; 613 Zipf 147 / 153. Where y is f32 they widen.
+// THE MATRIX STEP. A block of 128 columns is one step: y += sw sx (sum over the block of w x). Scales are any f32 numbers, so
+// they come in as a multiply-add of the sum, which begins at zero. It is taken in one of two ways:
+//   widened   the codes become 16-bit floats, which hold every e4m3 (f16 for f16 x, else bf16), and four v_mfma_f32_16x16x32
+//             add their products, each exact in f32.
+//   as codes  one v_mfma_f32_16x16x128_f8f6f4, at some three times the rate. It adds eight neighbouring columns' products on a
+//             grid: each is cut towards zero to a multiple of 2^(E - 13), E the largest of the eight sums of the two codes'
+//             exponents; the eights are then added in f32 (found by giving it one product at a time beside a large one). A
+//             subnormal code's exponent is -6, however small it is: a sum is off by less than 7 x 2^-13 of each eight's largest
+//             product of magnitudes that count as 2^-6 at least; of normally distributed rows by 1.4e-5 of the products' norm.
+// Few rows against many weights are bound by memory, and widen. Tiles take F8 x as codes where y has 16 bits, whose own
+// rounding (2^-9 or 2^-12 of the value) and the codes' (2^-4) are far larger: from 64 bits bf16 rows are as far either way
+// (1.7e-3 of the norm). Codes / widened, us: 8192 tokens over 8 experts, 2816 x 2048 111 / 246; 4096 over 512 214 / 393; 1500
+// 172 / 225; 800 over 8 16.5 / 20.8; 613 Zipf 147 / 153. Where y is f32 they widen.
 // Lane l holds of row l % 16, with g = l / 16, the 16 columns from 16 g and those from 64 + 16 g of the block.
 #include <hip/hip_runtime.h>
 
@@ -33,11 +34,12 @@ constexpr int F8 = EXL3C4_F8;
 // A lane's 32 codes of a row's block.
 struct Codes { uint4 h[2]; };
 
-// A weights' scale as f 2^(byte - 127), f of magnitude 1 to 2 and the byte as the matrix unit and the conversions take it. A sum of codes' products, with F8 x
-// the product of the two scales as well, may be no f32 number, or one of few bits, though the other factors bring it back: so the power comes in before
-// the sum, in the matrix unit or with the codes as they widen, and f32 multiplies by f (x's scale times f) behind it. With f16 x both stay in f32's
-// range anyway. The power ends at 2^-108 and 2^102, between which f32 holds every sum of codes (f takes what is beyond, as it does zeros, infinities
-// and NaN). (Splitting x's scale too, a row each: the tiles of codes 109 -> 114 us, 66 -> 69.)
+// A weights' scale as f 2^(byte - 127), f of magnitude 1 to 2 and the byte as the matrix unit and the conversions take it. A
+// sum of codes' products, with F8 x the product of the two scales as well, may be no f32 number, or one of few bits, though the
+// other factors bring it back: so the power comes in before the sum, in the matrix unit or with the codes as they widen, and
+// f32 multiplies by f (x's scale times f) behind it. With f16 x both stay in f32's range anyway. The power ends at 2^-108 and
+// 2^102, between which f32 holds every sum of codes (f takes what is beyond, as it does zeros, infinities and NaN). (Splitting
+// x's scale too, a row each: the tiles of codes 109 -> 114 us, 66 -> 69.)
 struct Scale {
     float f;
     int byte;
@@ -50,8 +52,10 @@ struct Scale {
 
 // The products times 2^(by - 127).
 __device__ __forceinline__ f32x4 mma_f8(const Codes& a, const Codes& b, int by, f32x4 c) {
-    const i32x8 A = { (int)a.h[0].x, (int)a.h[0].y, (int)a.h[0].z, (int)a.h[0].w, (int)a.h[1].x, (int)a.h[1].y, (int)a.h[1].z, (int)a.h[1].w };
-    const i32x8 B = { (int)b.h[0].x, (int)b.h[0].y, (int)b.h[0].z, (int)b.h[0].w, (int)b.h[1].x, (int)b.h[1].y, (int)b.h[1].z, (int)b.h[1].w };
+    const i32x8 A = { (int)a.h[0].x, (int)a.h[0].y, (int)a.h[0].z, (int)a.h[0].w,
+                      (int)a.h[1].x, (int)a.h[1].y, (int)a.h[1].z, (int)a.h[1].w };
+    const i32x8 B = { (int)b.h[0].x, (int)b.h[0].y, (int)b.h[0].z, (int)b.h[0].w,
+                      (int)b.h[1].x, (int)b.h[1].y, (int)b.h[1].z, (int)b.h[1].w };
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 0, 0, 0, by, 0, 127);
 }
 
@@ -84,11 +88,13 @@ __device__ __forceinline__ float word(const uint4& v, int i) { return __uint_as_
 __device__ __forceinline__ int64_t scale_row(int n, int half, int n_out) { return (n >> 7) + (int64_t)half * ((n_out + 127) >> 7); }
 
 // ------------------------------------------------------------------------------------------ few rows an expert
-// A workgroup: a chunk of up to 16 rows against NS strips of 16 weight rows (with SwiGLU half of them gate rows and half their up rows), each wave
-// a part of k; the weights go from memory straight to the matrix units' operands, each byte read once, and the parts' sums meet in LDS in a
-// fixed order. x is the A operand (rows of D), W the B operand: lane l ends with D[m = 4 g + r][n = l % 16].
-// What bounds it: for one token the start (offsets, rows, the first loads) and the last round trip, 8.6 us and 2.4 TB/s of 10 experts' 1024 x 2048; then memory, one
-// row against 8192 x 8192 16.4 us, 4.1 TB/s. Four steps ahead or loads past the caches: within 1%.
+// A workgroup: a chunk of up to 16 rows against NS strips of 16 weight rows (with SwiGLU half of them gate rows and half their
+// up rows), each wave a part of k; the weights go from memory straight to the matrix units' operands, each byte read once, and
+// the parts' sums meet in LDS in a fixed order. x is the A operand (rows of D), W the B operand: lane l ends with D[m = 4 g +
+// r][n = l % 16].
+// What bounds it: for one token the start (offsets, rows, the first loads) and the last round trip, 8.6 us and 2.4 TB/s of 10
+// experts' 1024 x 2048; then memory, one row against 8192 x 8192 16.4 us, 4.1 TB/s. Four steps ahead or loads past the caches:
+// within 1%.
 constexpr int ROWS_LOG2 = 4;
 constexpr int WAVES = 4;
 
@@ -135,7 +141,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_f8_rows(Exl3c4DevGemm a) {
             for (int s = 0; s < NS; ++s)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    q[s].h[h] = whole || (int64_t)t * 128 + 64 * h + 16 * g < a.K ? load16(w[s] + at + ((int64_t)t * 128 + 64 * h)) : uint4{ 0, 0, 0, 0 };
+                    q[s].h[h] = whole || (int64_t)t * 128 + 64 * h + 16 * g < a.K ? load16(w[s] + at + ((int64_t)t * 128 + 64 * h))
+                                                                                  : uint4{ 0, 0, 0, 0 };
         };
         auto load_x = [&](uint4* v, int t, bool whole) {
 #pragma unroll
@@ -155,7 +162,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_f8_rows(Exl3c4DevGemm a) {
                 f32x4 p = { 0, 0, 0, 0 };
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    p = mma<WIDER<XT>>(XT == F8 ? widen_part<BF16>(Codes{ v[0], v[1] }, j) : v[j], widen_part<WIDER<XT>>(q[s], j, XT == F16 ? 1.f : k.power()), p);
+                    p = mma<WIDER<XT>>(XT == F8 ? widen_part<BF16>(Codes{ v[0], v[1] }, j) : v[j],
+                                       widen_part<WIDER<XT>>(q[s], j, XT == F16 ? 1.f : k.power()), p);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(p[r], XT == F8 ? sx[r] * k.f : XT == BF16 ? k.f : sw[s], acc[s][r]);
             }
@@ -231,20 +239,22 @@ template <int T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // ------------------------------------------------------------------------------------------ many rows an expert
-// A workgroup: a tile of MT rows of one expert against NT weight rows (with SwiGLU 16 gate rows and their 16 up rows in turn, so that a lane holds
-// both), k in stages of one block of 128 columns. A stage's rows and scales go from memory to LDS without registers. A wave reads its weight rows into
-// registers at the start of a stage and then uses them for all its rows of x, so one place for weights is enough: once every wave has read them
-// (a barrier among the products) the next stage's come in under the rest of the products. x has XB places, XB - 1 stages ahead. So a workgroup's LDS stays
-// small and a CU holds several, one at its start or end under another's products.
+// A workgroup: a tile of MT rows of one expert against NT weight rows (with SwiGLU 16 gate rows and their 16 up rows in turn,
+// so that a lane holds both), k in stages of one block of 128 columns. A stage's rows and scales go from memory to LDS without
+// registers. A wave reads its weight rows into registers at the start of a stage and then uses them for all its rows of x, so
+// one place for weights is enough: once every wave has read them (a barrier among the products) the next stage's come in under
+// the rest of the products. x has XB places, XB - 1 stages ahead. So a workgroup's LDS stays small and a CU holds several, one
+// at its start or end under another's products.
 //
-// LDS. A row of a stage is 128 bytes (16-bit x: two such halves). The loads write lane after lane, 16 bytes each, so the order within a row is chosen
-// at the source: place p of row r holds the chunk q = p ^ (r & 7), in a half of a 16-bit row the chunk whose number is q's with its highest bit moved to the end,
-// so that lane groups g and g + 1 read places that differ in their lowest bit: the 16 rows and four lane groups that read a matrix operand then fall on all the
-// banks evenly (16-bit rows by q itself: 39% of the LDS cycles were conflicts, 1% so; 4096 tokens over 8 experts 56.0 -> 54.4 us). Behind x's rows a scale for
+// LDS. A row of a stage is 128 bytes (16-bit x: two such halves). The loads write lane after lane, 16 bytes each, so the order
+// within a row is chosen at the source: place p of row r holds the chunk q = p ^ (r & 7), in a half of a 16-bit row the chunk
+// whose number is q's with its highest bit moved to the end, so that lane groups g and g + 1 read places that differ in their
+// lowest bit: the 16 rows and four lane groups that read a matrix operand then fall on all the banks evenly (16-bit rows by q
+// itself: 39% of the LDS cycles were conflicts, 1% so; 4096 tokens over 8 experts 56.0 -> 54.4 us). Behind x's rows a scale for
 // each; behind the weights' those of the tile's blocks of weight rows.
 //
-// Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, so that a sum's scale is one number of the
-// lane's row of x times one that the wave shares.
+// Weights are the A operand here (rows of D): a lane ends with 4 consecutive columns of one row of y, so that a sum's scale is
+// one number of the lane's row of x times one that the wave shares.
 template <int XT, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB> struct Tile {
     static constexpr int MT = 1 << MT_LOG2, WAVES_ = WM * WN;
     static constexpr int XROW = XT == F8 ? 128 : 256;                        // bytes of a row of x a stage
@@ -254,8 +264,11 @@ template <int XT, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB> struct T
     static constexpr int NX = XL + XSL, NW = WL + 1;                         // a wave's loads of x and of weights, every stage
     static constexpr int AT_XS = XG * 1024, XSLOT = AT_XS + XS * 256, AT_W = XB * XSLOT, AT_WS = AT_W + WG * 1024, LDS = AT_WS + 256;
     static constexpr int TM = MT / WM / 16, TN = NT / WN / 16;               // matrix tiles a wave
-    // Rows of y past the caches, of larger tiles: 1500 tokens 188 -> 172, 2048 Zipf 222 -> 213, 4096 216 -> 210, 8192 over 8 experts, 2048 x 1408 71 -> 64, and whole layers of
-    // 1500 to 4096 tokens by 4% (in tiles of 32 rows 400 tokens 162 -> 165, a layer of 613 456 -> 464).
+    // Rows of y go past the caches from tiles of more than 32 rows. Through them / past them, us:
+    //   the product alone    512 experts, 1500 tokens 188 / 172, 2048 Zipf 222 / 213, 4096 216 / 210; 8 experts, 8192, 2048 x 1408 71 / 64
+    //   whole layers         512 experts, 1500 tokens 350 / 329, 2048 371 / 345, 4096 460 / 450; 64 experts, 8192 686 / 684;
+    //                        8 experts, 2000 99.6 / 97.0, 4096 163.5 / 163.0, 8192 267.1 / 267.8
+    //   in tiles of 32 rows  400 tokens 162 / 165, a layer of 613 456 / 464: through them
     static constexpr bool LATER = MT_LOG2 > 5;
     // waves a SIMD, by the workgroups whose LDS a CU holds: what the compiler may use registers for
     static constexpr int GROUPS = 160 * 1024 / (LDS + 4 * MT + 1024), EU = GROUPS * WAVES_ / 4, WAVES_EU = EU > 8 ? 8 : EU;
@@ -263,7 +276,8 @@ template <int XT, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB> struct T
     static_assert((NT == 128 || NT == 256) && (XB == 2 || XB == 3), "one or two blocks of weight rows; places of x");
 };
 
-template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB, bool ONCE, class G = Tile<XT, SW, MT_LOG2, NT, WM, WN, XB>>
+template <int XT, bool WIDE, bool SW, int MT_LOG2, int NT, int WM, int WN, int XB, bool ONCE,
+          class G = Tile<XT, SW, MT_LOG2, NT, WM, WN, XB>>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G::WAVES_EU, G::WAVES_EU))) void k_f8_tile(Exl3c4DevGemm a) {
     constexpr int MT = G::MT, WV = WM * WN, TM = G::TM, TN = G::TN;
     __shared__ __align__(1024) char lds[G::LDS];
@@ -285,7 +299,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
     __syncthreads();
     if (ch.expert >= 0) {
         const gaddr we = entry(a.w, a.w_stride, ch.expert), wse = entry(a.ws, a.ws_stride, ch.expert);
-        // Each of the wave's loads of a stage: where it reads next, for this lane (lane l takes place l % 8 of row l / 8). A stage is 128 columns on.
+        // Each of the wave's loads of a stage: where it reads next, for this lane (lane l takes place l % 8 of row l / 8). A
+        // stage is 128 columns on.
         gaddr xp[G::NX], wp[G::NW];
         auto x_chunk = [&](int) {
             const int q = (lane & 7) ^ (lane >> 3);
@@ -302,8 +317,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             xp[G::XL + i] = (gaddr)a.xs + (int64_t)max(rows_x[(64 * ((wave + i * WV) % max(G::XS, 1)) + lane) % MT], 0) * a.xs_pitch;
 #pragma unroll
         for (int i = 0; i < G::WL; ++i) wp[i] = we + (int64_t)w_row(8 * (wave + i * WV) + (lane >> 3)) * a.w_pitch + 16 * w_chunk(i);
-        // the scales of the tile's weight rows: even lanes of its first block (SwiGLU: of the gate rows), odd lanes of the second (of the up rows);
-        // every wave the same ones, so that a wait counts alike in all
+        // the scales of the tile's weight rows: even lanes of its first block (SwiGLU: of the gate rows), odd lanes of the
+        // second (of the up rows); every wave the same ones, so that a wait counts alike in all
         wp[G::WL] = wse + (SW ? scale_row(n0, lane & 1, a.n_out) : scale_row(min(n0 + (lane & 1) * 128, a.N - 1), 0, a.N)) * a.ws_pitch;
         const int stages = (a.K + 127) / 128, past = a.K - 128 * (stages - 1);          // columns of the last stage
         const uint32_t at0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -346,7 +361,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             const float* XS = (const float*)(X + G::AT_XS);
             const float* WS = (const float*)(lds + G::AT_WS);
             auto codes = [&](const char* p, int row) {
-                return Codes{ *(const uint4*)(p + row * 128 + 16 * (g ^ (l16 & 7))), *(const uint4*)(p + row * 128 + 16 * ((4 + g) ^ (l16 & 7))) };
+                return Codes{ *(const uint4*)(p + row * 128 + 16 * (g ^ (l16 & 7))),
+                              *(const uint4*)(p + row * 128 + 16 * ((4 + g) ^ (l16 & 7))) };
             };
             // (a wave's weight rows lie in one block of 128; with SwiGLU its even tiles in the gate's, its odd ones in the up's)
             const float sw[2] = { WS[SW ? 0 : (wn * TN * 16) >> 7], WS[1] };
@@ -385,8 +401,9 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                     }
                 }
             } else {
-                // x's eights j of columns: 16 g + 8 j of the block's first half, then of its second. (The weights' power comes in with x's codes where it is
-                // one for all: with the weights' a register more, and a spill's reload waits for the loads ahead, 34.0 -> 36.2 us of 300 rows of 4096 x 4096.)
+                // x's eights j of columns: 16 g + 8 j of the block's first half, then of its second. (The weights' power comes
+                // in with x's codes where it is one for all: with the weights' a register more, and a spill's reload waits for
+                // the loads ahead, 34.0 -> 36.2 us of 300 rows of 4096 x 4096.)
                 uint4 xv[TM][4];
                 float sx[TM];
 #pragma unroll
@@ -399,7 +416,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            xv[m][j] = *(const uint4*)(X + ((xr >> 3) + 2 * m) * 2048 + (j >> 1) * 1024 + (l16 & 7) * 128 + 16 * ((g + 4 * (j & 1)) ^ (l16 & 7)));
+                            xv[m][j] = *(const uint4*)(X + ((xr >> 3) + 2 * m) * 2048 + (j >> 1) * 1024 + (l16 & 7) * 128 +
+                                                       16 * ((g + 4 * (j & 1)) ^ (l16 & 7)));
                     }
                 }
 #pragma unroll
@@ -439,9 +457,10 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             asm volatile("" ::: "memory");
             if (t + 2 == stages) end_w();
             if (t + XB == stages) end_x();
-            const uint32_t to_x = at0 + (slot_x == 0 ? XB - 1 : slot_x - 1) * G::XSLOT;  // the place of x of stage t - 1, read by all before the barrier
-            // Behind the last stage no lane loads: a branch would keep the products of one row tile from running on beside the next one's (8192 tokens
-            // over 8 experts, 2816 x 2048: 123 us for 114, when one workgroup filled a CU).
+            // the place of x of stage t - 1, read by all before the barrier
+            const uint32_t to_x = at0 + (slot_x == 0 ? XB - 1 : slot_x - 1) * G::XSLOT;
+            // Behind the last stage no lane loads: a branch would keep the products of one row tile from running on beside the
+            // next one's (8192 tokens over 8 experts, 2816 x 2048: 123 us for 114, when one workgroup filled a CU).
             const int more_w = there(t + 1), more_x = there(t + XB - 1);
             multiply(slot_x, [&](int s) {
                 constexpr int AT = SLOTS > 1 ? 1 : 0;                        // the loads follow in one to four slots
@@ -463,9 +482,10 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
             slot_x = slot_x + 1 == XB ? 0 : slot_x + 1;
         }
     }
-    // A lane holds columns 16 n + 4 g .. + 3 of row 16 m + l16 of the wave's (SwiGLU: of gate tile 2 n and up tile 2 n + 1). PM row tiles at a time cross
-    // LDS in y's type, so that whole rows of the tile go out by 16 bytes a lane (8192 tokens over 8 experts, 2048 x 1408: 78 us with 8 bytes a lane
-    // from each wave's own columns, 68 so; 2816 x 2048 with SwiGLU 115 and 111; 2560 x 640 over 512 experts the same).
+    // A lane holds columns 16 n + 4 g .. + 3 of row 16 m + l16 of the wave's (SwiGLU: of gate tile 2 n and up tile 2 n + 1). PM
+    // row tiles at a time cross LDS in y's type, so that whole rows of the tile go out by 16 bytes a lane (8192 tokens over 8
+    // experts, 2048 x 1408: 78 us with 8 bytes a lane from each wave's own columns, 68 so; 2816 x 2048 with SwiGLU 115 and 111;
+    // 2560 x 640 over 512 experts the same).
     constexpr int TO = SW ? TN / 2 : TN, OC = 16 * TO * WN, MOST = WIDE ? 4 : 2;      // (y is f32 where the codes are widened only)
     constexpr int FIT = G::LDS / (16 * (OC * MOST + 16)), PM = FIT >= TM ? TM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
     static_assert(WM == 1 && FIT >= 1 && TM % PM == 0, "a pass's rows fit");
@@ -484,7 +504,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(G:
                 if (SW) v = swiglu4(v, acc[SW ? 2 * n + 1 : n][m]);
                 char* p = lds + ((m - m0) * 16 + l16) * pitch + ((wn * TO * 16 + 16 * n + 4 * g) << size_log2);
                 if (size_log2 == 2) *(f32x4*)p = v;
-                else *(uint2*)p = a.y_type == BF16 ? uint2{ pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]) } : uint2{ pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]) };
+                else *(uint2*)p = a.y_type == BF16 ? uint2{ pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]) }
+                                                   : uint2{ pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]) };
             }
         __syncthreads();
         for (int i = threadIdx.x; i < 16 * PM << row_log2; i += 64 * WV) {
@@ -525,34 +546,42 @@ int launch_tile(Exl3c4DevGemm& a, hipStream_t st) {
     a.tiles = (a.n_out + cols - 1) / cols;
     const int64_t grid = (chunk_bound(a.T, a.n_expert, 1 << MT_LOG2) * a.tiles + 7) / 8 * 8;
     if (grid > THREADS / (64 * WM * WN)) return EXL3C4_E_SHAPE;
-    // Weights of runs that are one chunk, which no other workgroup reads, go past the caches where those of all experts that can be live are more than the one behind
-    // L2 holds (256 MiB), so that the next pass does not find them there; and then faster. Six sets of weights in turn, us: bf16 x, 32 tokens 95 -> 86; F8 x,
-    // 100 158 -> 138, 400 184 -> 163, 613 Zipf 2560 x 640 163 -> 158, 1500 194 -> 188. Of fewer, one set again and again, 8 tokens 27 -> 33, 64/6 32 tokens 23 -> 30.
-    // (For all runs' weights 2048 Zipf takes 241 for 226.) The choice is a branch at each load: 3% of a batch that does not need it, hence a kernel of its own, and in
-    // tiles of 128 rows more than it gives (4096 tokens 218 -> 226).
+    // Weights of runs that are one chunk, which no other workgroup reads, go past the caches where those of all experts that
+    // can be live are more than the one behind L2 holds (256 MiB), so that the next pass does not find them there. Through them
+    // / past them, us:
+    //   six sets of weights in turn    bf16 x, 32 tokens 95 / 86; F8 x, 100 158 / 138, 400 184 / 163, 613 Zipf 2560 x 640 163 /
+    //                                  158, 1500 194 / 188
+    //   fewer, one set again and again 8 tokens 27 / 33, 64/6 32 tokens 23 / 30: through them
+    //   runs of more chunks as well    2048 Zipf 226 / 241: through them
+    // The choice is a branch at each load: 3% of a batch that does not need it, hence a kernel of its own, and in tiles of 128
+    // rows more than it gives (4096 tokens 218 / 226).
     const int64_t live = a.n_expert < a.T ? a.n_expert : a.T;
     const bool once = MT_LOG2 < 7 && live * a.N > ((int64_t)256 << 20) / a.K;
-    const auto f = once ? k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB, (MT_LOG2 < 7)> : k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB, false>;
+    const auto f = once ? k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB, (MT_LOG2 < 7)>
+                        : k_f8_tile<XT, WIDE, SW, MT_LOG2, NT, WM, WN, XB, false>;
     hipLaunchKernelGGL(f, dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, a);
     return launched();
 }
 
-// Which kernel, and how large a tile: by the types, the sizes and the rows that an expert has at least on average, r = T / min(E, T) -- never by
-// the routing, which is on the device. Larger tiles read weights and rows less often; smaller ones waste less of a chunk, make more workgroups and
-// start sooner; the rows kernel splits k over its waves, so that few workgroups are enough. `units`: workgroups of a tile, each expert half a chunk
-// short of whole ones. Measured on one card, us, the product alone (E / top-k, N x K, tokens; 512/10, 1024 x 2048 with SwiGLU where nothing else is said):
-//   rows against 32        bf16 x: 1 token 8.6 / 13.3, 4 19.6 / 20.0, 8 30 / 27, 32 102 / 83; F8 x: 8 30 / 26, 16 55 / 56, 32 98 / 79.
-//                          64/6, 32 tokens 30 / 23; 8/2, 200 20 / 13. One expert, bf16 x: 2048 x 2048, 77 rows 10.7 / 13.2, 300 22 / 18;
-//                          8192 x 8192, 64 rows 48 / 57; 4096 x 4096, 16 rows 11.7 / 22, 300 74 / 35.
-//   2 strips against 4     one row, 8192 x 8192 16.5 / 23.6; 4096 x 4096, 16 rows 11.7 / 15.5; 8192 x 8192, 64 rows 61 / 48, which read the weights
-//                          once for each 16 rows, mostly from L2.
-//   32 rows against 64     as codes: 400 tokens 160 / 165, 613 Zipf 2560 x 640 148 / 156, 1500 202 / 171, 8/2 800 15.9 / 21. bf16 x: 400 164 / 187,
-//                          613 Zipf 2560 x 640 156 / 172, 1500 200 / 191, 8/2 800 19 / 28. F8 x, f32 y: 200 161 / 200, 1500 217 / 215.
-//   64 against 128         as codes: 1500 172 / 200, 2048 Zipf 211 / 222, 4096 271 / 210, 64/6 2000 52 / 40, 8/2 8192 2816 x 2048 143 / 104,
-//                          2048 x 1408, sorted rows in, 79 / 64.
-// As codes a tile of 256 x 256 with a CU to itself took 131 there before the loads went among the products and 114 to 118 since, and was slower
-// everywhere else; 128 x 128 130 (73 for 77 at 2048 x 1408, sorted rows in); weights in two places 232 at 64 rows, and 2% less at 32 rows and 100 to 400
-// tokens. Widened: 128 x 128 in eight waves 344, 128 x 256 211 against 202 of 64 x 256.
+// Which kernel, and how large a tile: by the types, the sizes and the rows that an expert has at least on average, r = T /
+// min(E, T) -- never by the routing, which is on the device. Larger tiles read weights and rows less often; smaller ones waste
+// less of a chunk, make more workgroups and start sooner; the rows kernel splits k over its waves, so that few workgroups are
+// enough. `units`: workgroups of a tile, each expert half a chunk short of whole ones. Measured on one card, us, the product
+// alone (E / top-k, N x K, tokens; 512/10, 1024 x 2048 with SwiGLU where nothing else is said):
+//   rows against 32        bf16 x: 1 token 8.6 / 13.3, 4 19.6 / 20.0, 8 30 / 27, 32 102 / 83; F8 x: 8 30 / 26, 16 55 / 56, 32
+//                          98 / 79. 64/6, 32 tokens 30 / 23; 8/2, 200 20 / 13. One expert, bf16 x: 2048 x 2048, 77 rows 10.7 /
+//                          13.2, 300 22 / 18; 8192 x 8192, 64 rows 48 / 57; 4096 x 4096, 16 rows 11.7 / 22, 300 74 / 35.
+//   2 strips against 4     one row, 8192 x 8192 16.5 / 23.6; 4096 x 4096, 16 rows 11.7 / 15.5; 8192 x 8192, 64 rows 61 / 48,
+//                          which read the weights once for each 16 rows, mostly from L2.
+//   32 rows against 64     as codes: 400 tokens 160 / 165, 613 Zipf 2560 x 640 148 / 156, 1500 202 / 171, 8/2 800 15.9 / 21.
+//                          bf16 x: 400 164 / 187, 613 Zipf 2560 x 640 156 / 172, 1500 200 / 191, 8/2 800 19 / 28. F8 x, f32 y:
+//                          200 161 / 200, 1500 217 / 215.
+//   64 against 128         as codes: 1500 172 / 200, 2048 Zipf 211 / 222, 4096 271 / 210, 64/6 2000 52 / 40, 8/2 8192 2816 x
+//                          2048 143 / 104, 2048 x 1408, sorted rows in, 79 / 64.
+// As codes a tile of 256 x 256 with a CU to itself took 131 there before the loads went among the products and 114 to 118
+// since, and was slower everywhere else; 128 x 128 130 (73 for 77 at 2048 x 1408, sorted rows in); weights in two places 232 at
+// 64 rows, and 2% less at 32 rows and 100 to 400 tokens. Widened: 128 x 128 in eight waves 344, 128 x 256 211 against 202 of
+// 64 x 256.
 // Returns a tile's rows (32, 64, 128), or for few rows an expert the strips of a workgroup (2, 4).
 int choose(bool wide, bool swiglu, int64_t T, int64_t n_expert, int64_t n_out, int64_t K) {
     const int64_t live = n_expert < T ? n_expert : T;

@@ -1,9 +1,8 @@
-// exl3c4_route.hip -- the routing around the routed-expert ops, on gfx950 (wave64): the router (softmax over all
-// logits, top_k, renormalisation), moe_scatter (a stable counting sort of the flat (token, slot) pairs by expert) and
-// moe_gather (each token's slots weighted and summed in f32, ascending slot order, cast to f16); and moe_route, the router by scores, with a bias
-// and groups. The contract of the first three is
-// radiance's (include/exl3_abi.h:90-158; the scatter as tests/ref/exl3_numpy.py:223-242 states it); the reference
-// device library leaves these to its engine.
+// exl3c4_route.hip -- the routing around the routed-expert ops, on gfx950 (wave64): the router (softmax over all logits, top_k,
+// renormalisation), moe_scatter (a stable counting sort of the flat (token, slot) pairs by expert) and moe_gather (each token's
+// slots weighted and summed in f32, ascending slot order, cast to f16); and moe_route, the router by scores, with a bias and
+// groups. The contract of the first three is radiance's (include/exl3_abi.h:90-158; the scatter as
+// tests/ref/exl3_numpy.py:223-242 states it); the reference device library leaves these to its engine.
 #include <hip/hip_runtime.h>
 
 #include <float.h>
@@ -247,7 +246,8 @@ __global__ __launch_bounds__(SC_THREADS) void k_scatter(const int32_t* ids, uint
     __syncthreads();
     uint32_t counted = 0;
     if constexpr (LOADS == 16) {
-        // whole rounds of four ids a thread, four rounds' loads out together; a wave's 256 ids lie before the segment or not (it starts at a multiple)
+        // whole rounds of four ids a thread, four rounds' loads out together; a wave's 256 ids lie before the segment or not
+        // (it starts at a multiple)
         struct __attribute__((packed, aligned(4))) Four { int32_t v[4]; };
         constexpr uint32_t ROUND = 4 * SC_THREADS;
         auto count = [&](const Four& q, uint32_t i0) {
@@ -332,19 +332,26 @@ __global__ __launch_bounds__(SC_THREADS) void k_scatter(const int32_t* ids, uint
     for (uint32_t i = live + blockIdx.x * SC_THREADS + tid; i < T; i += gridDim.x * SC_THREADS) sorted[i] = -1;
 }
 
-// moe_scatter by experts: a workgroup takes PO_EXPERTS or fewer neighbouring experts and reads every pair's id, each wave a part of the pairs. It counts the
-// pairs of lower experts, whose sum is its first row, and lists its own in LDS in their order; what the waves before it found then places each. Three
-// instructions an id (two comparisons and a count) in place of an LDS atomic, and no ranks among the pairs of a segment. What bounds it: every CU reads
-// all ids, 3.8 us of L2's rate for 81,920 pairs, and the same again goes into the pairs found.
-// k_scatter against it, us a launch (pairs, experts): 1, 512 2.8 / 3.2; 10, 512 2.9 / 3.3; 32, 8 3.2 / 3.3; 80, 512 3.9 / 3.5; 1,280 4.9 / 3.6; 6,130 6.3 / 4.2;
-// 20,480 7.7 / 5.8; 81,920 13.1 / 11.1 (a fifth of them on one expert 22 / 23, all 75 / 54); 200,000 28 / 22 (50 / 129: a list no longer holds a wave's own);
-// 49,152, 64 9.6 / 9.3 (20 / 14). Pairs of which seven eighths are no expert's, whose places one workgroup fills: 81,920, 64 12.5 / 13.1; 65,536, 32 9.4 / 11.7;
-// 131,072 pairs of 8 experts 31 / 93, for few workgroups place.
-constexpr uint32_t PO_LEAST = 33, PO_MOST = 1 << 17, PO_EACH = 1024;     // pairs from which on it is taken and up to which, and how many an expert
+// moe_scatter by experts: a workgroup takes PO_EXPERTS or fewer neighbouring experts and reads every pair's id, each wave a
+// part of the pairs. It counts the pairs of lower experts, whose sum is its first row, and lists its own in LDS in their order;
+// what the waves before it found then places each. Three instructions an id (two comparisons and a count) in place of an LDS
+// atomic, and no ranks among the pairs of a segment. What bounds it: every CU reads all ids, 3.8 us of L2's rate for 81,920
+// pairs, and the same again goes into the pairs found.
+// k_scatter / this, us a launch, pairs over experts evenly unless something is said:
+//   512 experts     1 pair 2.8 / 3.2, 10 2.9 / 3.3, 80 3.9 / 3.5, 1,280 4.9 / 3.6, 6,130 6.3 / 4.2, 20,480 7.7 / 5.8, 81,920
+//                   12.9 / 10.9, 200,000 28 / 22
+//   8, 64 experts   32 pairs 3.2 / 3.3; 49,152 9.6 / 9.3
+//   uneven          81,920 of 512: a fifth of them on one expert 21.6 / 19.4, all 75 / 54, Zipf in the order of the ids 21.4 /
+//                   23.7, moe_route's choice of random tokens with a bias (0 to 2,468 an expert) 15.0 / 15.6; 200,000, a fifth
+//                   on one 50 / 129: a list no longer holds a wave's own
+//   no expert's     seven eighths of 81,920 of 64 12.5 / 13.1, of 65,536 of 32 9.4 / 11.7, of 131,072 of 8 31 / 93: few
+//                   workgroups place, one fills the rest
+constexpr uint32_t PO_LEAST = 33, PO_MOST = 1 << 17, PO_EACH = 1024;     // pairs that take it: from, up to, and how many an expert
 constexpr int PO_THREADS = 1024, PO_WAVES = PO_THREADS / 64, PO_EXPERTS = 4, PO_LIST = 2048;
 template <bool BASE>
-__global__ __launch_bounds__(PO_THREADS) void k_pairs_by_expert(const int32_t* ids, uint32_t T, int32_t base, int32_t n_expert, uint32_t per, uint32_t seg,
-                                                                int32_t* sorted, int32_t* off, int32_t* count, int32_t* row_of) {
+__global__ __launch_bounds__(PO_THREADS) void k_pairs_by_expert(const int32_t* ids, uint32_t T, int32_t base, int32_t n_expert,
+                                                                uint32_t per, uint32_t seg, int32_t* sorted, int32_t* off,
+                                                                int32_t* count, int32_t* row_of) {
     __shared__ int tot[PO_WAVES][PO_EXPERTS + 1];                 // a wave's pairs of each own expert, and of lower ones
     __shared__ uint16_t list[PO_WAVES][PO_LIST];                  // its own pairs in order, from its part's first on: 4 pair + expert
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -385,7 +392,8 @@ __global__ __launch_bounds__(PO_THREADS) void k_pairs_by_expert(const int32_t* i
         if ((hit[0] | hit[1] | hit[2] | hit[3]) == 0) return;
         uint32_t at = listed;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) at = __builtin_amdgcn_mbcnt_hi((uint32_t)(hit[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[j], at));
+        for (int j = 0; j < 4; ++j)
+            at = __builtin_amdgcn_mbcnt_hi((uint32_t)(hit[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[j], at));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (hit[j] == 0) continue;                            // (uniform)
@@ -459,7 +467,8 @@ __global__ __launch_bounds__(PO_THREADS) void k_pairs_by_expert(const int32_t* i
         for (int e = 0; e < PO_EXPERTS; ++e) {
             if (e >= (int)n) break;
             const uint64_t m = __ballot(x == (uint32_t)e);
-            if (x == (uint32_t)e) pos = next[e] + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+            if (x == (uint32_t)e)
+                pos = next[e] + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
             next[e] += __popcll(m);
         }
         if (pos >= 0) {
@@ -543,16 +552,21 @@ __global__ __launch_bounds__(1024) void k_route_scatter(const void* logits, int3
 }
 
 // ------------------------------------------------------------------------------------------ moe_route
-// The order of experts and of groups is that of their values in 64 bits, for among thousands of tokens there are always experts whose values f32 would
-// not tell apart. f32 finds who can be among the first (all within its error of them), f64 ranks those: one evaluation a lane. Groups whose place f32 leaves
-// open, and more than 64 such experts, are evaluated in f64 as a whole. Weights come out of the f64 scores, rounded once.
-// What bounds it: the VALU, some 800 instructions a token of 512 experts (of them the scores 110, the order of the lanes' largest 110, the candidates'
-// scores and ranks in f64 200); 16 MiB of logits are 3.4 us. 8192 tokens, 8 groups of 64 experts of which 4 stay, top-10 with a bias 13.5 us, 22 with f64 for
-// every expert; without groups 13.8 (softmax); 256 experts 10.5; one token 4.9 with its scatter, the whole of it latency. A group's place that stays open
-// is two groups' values in f64, in one token of some thousands: 613 tokens 5.2 us without one, 7.4 with (13.3 when every group was evaluated again).
-
-// e^x for x <= 0 (below -800: 0): x = n ln 2 + r with ln 2 in two parts (its first 37 bits, so that n times them is exact, and the rest), |r| <= ln 2 / 2,
-// and the exponential series up to r^13, whose rest is below 2^-52 of e^r.
+// The order of experts and of groups is that of their values in 64 bits, for among thousands of tokens there are always experts
+// whose values f32 would not tell apart. f32 finds who can be among the first (all within its error of them), f64 ranks those:
+// one evaluation a lane. Groups whose place f32 leaves open, and more than 64 such experts, are evaluated in f64 as a whole.
+// Weights come out of the f64 scores, rounded once.
+// What bounds it: the VALU (86% busy), some 800 instructions a token of 512 experts: the scores 110, the order of the lanes'
+// largest 110, the candidates' scores and ranks in f64 200. The groups' values are read from LDS with bank conflicts (lanes of
+// all groups meet the same banks: 61% of LDS's cycles, which are 18% of all). 16 MiB of logits are 3.4 us.
+// Alone, top-10 or top-8 with a bias, us:
+//   8192 tokens      512 experts in 8 groups 13.3 (22 with f64 for every expert; 15.6 in the trace of a whole pass), 256
+//                    experts in 8 10.4; 512 without groups, softmax 13.8
+//   one token        4.9 with its scatter: latency
+//   a group's place that f32 leaves open, in one token of some thousands: 613 tokens 5.4 without one, 7.4 with (13.3 with every
+//   group in f64)
+// e^x for x <= 0 (below -800: 0): x = n ln 2 + r with ln 2 in two parts (its first 37 bits, so that n times them is exact, and
+// the rest), |r| <= ln 2 / 2, and the exponential series up to r^13, whose rest is below 2^-52 of e^r.
 __device__ __forceinline__ double exp64(double x) {
     x = fmax(x, -800.0);
     constexpr double LN2_HI = 0x1.62e42fefap-1, LN2_LO = 0x1.cf79abc9e3b3ap-40;
@@ -617,8 +631,8 @@ __device__ __forceinline__ double score64(const Exl3c4DevRoute& a, const Soft& s
     if (a.score == EXL3C4_SCORE_SIGMOID) return sigmoid64(l);
     return exp64(l == sm.m ? 0.0 : (double)l - (double)sm.m) * sm.inv;             // (infinity - infinity is none)
 }
-// An f32 score is within 2^-21 of its value: sigmoid's exponent, exponential, sum, reciprocal and product lose 5 steps of 2^-24 together, softmax's (from f64
-// exponentials) 3. A choice is off by that and its own rounding; a sum of two by twice as much.
+// An f32 score is within 2^-21 of its value: sigmoid's exponent, exponential, sum, reciprocal and product lose 5 steps of 2^-24
+// together, softmax's (from f64 exponentials) 3. A choice is off by that and its own rounding; a sum of two by twice as much.
 __device__ __forceinline__ float error_of(float c) { return 0x1p-21f + 0x1p-23f * fabsf(c); }
 __device__ __forceinline__ float sigmoid32(float l) {
     const float t = __builtin_amdgcn_exp2f(fabsf(l) * -1.44269504088896340736f), q = __builtin_amdgcn_rcpf(1.f + t);
@@ -672,8 +686,8 @@ __device__ __forceinline__ uint64_t groups64(const Exl3c4DevRoute& a, const Soft
 
 // A candidate's key, id, logit and bias; behind the ranking its id and score.
 struct Cand { double s; float l, b; int id; };
-// One token by one wave: the experts e = lane + 64 j in registers. Lane r < top_k ends with the r-th expert and its weight. cand: the wave's 64 places
-// of LDS; value: its 64 RPL places (GROUPS).
+// One token by one wave: the experts e = lane + 64 j in registers. Lane r < top_k ends with the r-th expert and its weight.
+// cand: the wave's 64 places of LDS; value: its 64 RPL places (GROUPS).
 template <int RPL, bool GROUPS>
 __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row, int lane, Cand* cand, float* value) {
     // (loads past the last expert repeat it: a mask for each load would cost as much as the score)
@@ -695,7 +709,8 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
 #pragma unroll
         for (int j = 0; j < RPL; ++j) h[j] = p[at[j]];
 #pragma unroll
-        for (int j = 0; j < RPL; ++j) l[j] = a.type == EXL3C4_BF16 ? __uint_as_float((uint32_t)h[j] << 16) : (float)__builtin_bit_cast(_Float16, h[j]);
+        for (int j = 0; j < RPL; ++j)
+            l[j] = a.type == EXL3C4_BF16 ? __uint_as_float((uint32_t)h[j] << 16) : (float)__builtin_bit_cast(_Float16, h[j]);
     }
     const bool biased = a.bias != nullptr, soft = a.score == EXL3C4_SCORE_SOFTMAX, top2 = GROUPS && a.group_score == EXL3C4_GROUP_TOP2;
 #pragma unroll
@@ -743,7 +758,8 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
         c[j] = fminf(l[j], b[j]) > -INFINITY ? c[j] : __builtin_nanf("");
     }
     if constexpr (GROUPS) {
-        // the values by expert through LDS; then of 2^groups_log2 lanes, 64 >> groups_log2 times over, lane g finds group g's two largest in a part of it
+        // the values by expert through LDS; then of 2^groups_log2 lanes, 64 >> groups_log2 times over, lane g finds group g's
+        // two largest in a part of it
         const bool exact = !biased && !top2;
 #pragma unroll
         for (int j = 0; j < RPL; ++j) value[lane + 64 * j] = c[j] != c[j] ? -INFINITY : biased || exact ? c[j] : s[j];
@@ -766,10 +782,11 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
         if (a.groups_log2 < 4) meet(xor_lanef<8>(v1, lane), xor_lanef<8>(v2, lane));
         if (a.groups_log2 < 3) meet(xor_lanef<4>(v1, lane), xor_lanef<4>(v2, lane));
         if (a.groups_log2 < 2) meet(xor_lanef<2>(v1, lane), xor_lanef<2>(v2, lane));
-        // TOP2 by halves: two choices near f32's end, as masks by the type's lowest value are, leave f32 in their sum and not in half of it. The value that
-        // is meant lies from lo to hi, by the group's own choices' errors (of a half sum: half of both), the sum's rounding and these two's, so that a group
-        // of such choices leaves no other open (8192 tokens 34.6 -> 13.2 us; of 64 groups, whose two ends each are read, 15.8 -> 17.0). A group without an
-        // expert is below all others, whatever they are.
+        // TOP2 by halves: two choices near f32's end, as masks by the type's lowest value are, leave f32 in their sum and not
+        // in half of it. The value that is meant lies from lo to hi, by the group's own choices' errors (of a half sum: half of
+        // both), the sum's rounding and these two's, so that a group of such choices leaves no other open (8192 tokens 34.6 ->
+        // 13.2 us; of 64 groups, whose two ends each are read, 15.8 -> 17.0). A group without an expert is below all others,
+        // whatever they are.
         const bool live = v1 > -INFINITY, two = top2 && v2 > -INFINITY;
         const float gv = top2 ? 0.5f * v1 + (two ? 0.5f * v2 : 0.f) : v1, err = error_of(v1) + (two ? 0x1p-23f * fabsf(v2) : 0.f);
         const float hi = live ? gv + err : -INFINITY, lo = !live || gv == INFINITY ? gv : fmaxf(gv - err, -FLT_MAX);
@@ -806,8 +823,9 @@ __device__ __forceinline__ Pick score_token(const Exl3c4DevRoute& a, int64_t row
             if (!((word >> (of & 31)) & 1)) c[j] = __builtin_nanf("");
         }
     }
-    // At least top_k experts have a choice of thr, the top_k-th largest of the lanes' own largest. Whoever is among the first top_k is so by less than twice
-    // the error below it: those are gathered one a lane and ranked in f64, equal ones by id; more than 64 of them by top_k rounds of a wave maximum.
+    // At least top_k experts have a choice of thr, the top_k-th largest of the lanes' own largest. Whoever is among the first
+    // top_k is so by less than twice the error below it: those are gathered one a lane and ranked in f64, equal ones by id;
+    // more than 64 of them by top_k rounds of a wave maximum.
     float most = c[0];
 #pragma unroll
     for (int j = 1; j < RPL; ++j) most = fmaxf(most, c[j]);
@@ -1023,8 +1041,9 @@ extern "C" int exl3c4_dev_scatter(const int32_t* ids, int64_t T, int64_t base, i
     if (row_of != ids && T >= PO_LEAST && T <= PO_MOST && T <= (int64_t)PO_EACH * n_expert && base >= -(1 << 30) && base <= 1 << 30) {
         // (ids written over by row_of while other workgroups read them, and bases that 32 bits do not take from every id, are k_scatter's)
         const uint32_t by = ((uint32_t)n_expert + SC_MAX_WG - 1) / SC_MAX_WG, n = ((uint32_t)n_expert + by - 1) / by;
-        hipLaunchKernelGGL(base == 0 ? k_pairs_by_expert<false> : k_pairs_by_expert<true>, dim3(n), dim3(PO_THREADS), 0, (hipStream_t)stream, ids, (uint32_t)T, (int32_t)base, n_expert, by,
-                           ((uint32_t)T + n - 1) / n, sorted, off, count, row_of);
+        hipLaunchKernelGGL(base == 0 ? k_pairs_by_expert<false> : k_pairs_by_expert<true>, dim3(n), dim3(PO_THREADS), 0,
+                           (hipStream_t)stream, ids, (uint32_t)T, (int32_t)base, n_expert, by, ((uint32_t)T + n - 1) / n, sorted, off,
+                           count, row_of);
         return launched();
     }
     const bool far = base < INT32_MIN || base > INT32_MAX;
