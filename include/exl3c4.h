@@ -348,7 +348,8 @@ typedef struct Exl3c4F8 {
  * scale = a / 448, codes = x * (448 / a) to the nearest e4m3, ties to even, each of the two quotients and the product rounded once to f32. A block
  * that holds an infinity or a NaN: scale NaN, codes 0. The codes of a row up to a multiple of 16 columns are written (zeros behind cols), and each
  * block's scale; what lies behind them is left. Values and planes share no memory, here and in f8_dequant. Refusals, also f8_dequant's: INVAL (another
- * block, a null pointer), DTYPE, SHAPE (extents below zero, cols below one, more than 2^31 rows in all, more than a launch holds), STRIDE, ALIGN
+ * block, a null pointer), DTYPE, SHAPE (extents below zero, cols below one, more than 2^31 rows in all, more than a launch holds), STRIDE (a pitch
+ * or a stride below what it steps over: rows do not overlap, and matrices lie one behind the other, never in each other's rows), ALIGN
  * (codes and their pitch and stride in 16s, values and scales to their type). */
 int exl3c4_f8_quant(const void* x, int32_t x_dtype, int64_t x_pitch, int64_t x_stride, const Exl3c4F8* q, void* stream);
 

@@ -113,7 +113,7 @@ class F8:
     weights of a SwiGLU product hold gate and up as matrices of their own, one behind the other: quantise them as values [..., 2, rows / 2, cols],
     and view codes as [..., rows, cols] and scales as [..., 2 ceil(rows / 2 / 128), ...]. Its attributes are fixed, and the planes keep their sizes
     and strides; where their memory is, is read at each call. Leading dimensions have to step evenly as one for the conversions (for moe_gemm they need
-    not)."""
+    not), by at least a matrix's rows."""
     __slots__ = ("codes", "scales", "cols", "block", "shape", "rows", "mats", "device", "_planes")
 
     def __init__(self, codes, scales, cols: int, block: int):
